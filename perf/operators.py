@@ -1,0 +1,394 @@
+"""The elementwise gated recurrence, the RMS norm with a residual and the product of 8-bit rows: the three steps of a
+gated-recurrence layer whose projections run in 8 bits, each over the range a model calls it with.
+
+``listed()`` names the cases, ``draw(rng)`` gives another one of the same ranges, ``prepare(case, seed)`` makes what a
+program holds before the call, ``run(state)`` is one pass (``own``: through this package, otherwise in elementary torch
+operations), ``work(case)`` what a pass cannot do without, and ``exact(case, seed)`` the result in 64 bits."""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+E4M3_MAX = 448.0      # largest finite value of the 8-bit type (torch.float8_e4m3fn)
+AMAX_MIN = 1e-30      # rows whose largest magnitude is below this are scaled as if it were this
+EPS = 1e-5
+DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+BYTES = {"bf16": 2, "fp16": 2, "fp32": 4}
+
+
+def _scan(name, mode, batch, tokens, dim, dtype="bf16", gates=True, gate_dtype=None, bound=False, packed=0, state=True):
+    """``mode``: step (one token, state updated in place), forward, train; ``gates``: the operands are pre-activations;
+    otherwise g holds log decays in ``gate_dtype``; ``bound``: a lower bound per channel; ``packed``: sequences in a
+    packed batch (0: ``batch`` sequences of equal length); ``state``: an initial state is given."""
+    c = {"op": "scan", "mode": mode, "batch": batch, "tokens": tokens, "dim": dim, "dtype": dtype, "gates": gates,
+         "gate_dtype": gate_dtype or dtype, "bound": bound, "packed": packed, "state": state}
+    return c if name is None else dict(c, name=name)
+
+
+def _norm(name, mode, rows, dim, dtype="bf16", residual=None):
+    """``mode``: train (gradients of everything), quant (an output in 8 bits); ``residual``: its type."""
+    c = {"op": "norm", "mode": mode, "rows": rows, "dim": dim, "dtype": dtype, "residual": residual or dtype}
+    return c if name is None else dict(c, name=name)
+
+
+def _linear(name, rows, out, inner, dtype="bf16", bias=True, act="none", residual=False):
+    c = {"op": "linear", "rows": rows, "out": out, "inner": inner, "dtype": dtype, "bias": bias, "act": act, "residual": residual}
+    return c if name is None else dict(c, name=name)
+
+
+def listed():
+    return [
+        # The next token of a small serving batch: launch and host time.
+        _scan("scan_step", "step", 32, 1, 2048),
+        # One prompt of an odd length taken in before decoding: few channels, a long time axis.
+        _scan("scan_prompt", "forward", 1, 8191, 2048),
+        # A batch of long sequences, log decays as a caller of the operator hands them over.
+        _scan("scan_forward", "forward", 8, 4096, 2048, gates=False, gate_dtype="fp32"),
+        # A pre-training step: pre-activations, a learned lower bound, all gradients.
+        _scan("scan_train", "train", 8, 4096, 2048, bound=True, state=False),
+        # Fine-tuning on documents of very different lengths packed into one batch, half precision, ragged channels.
+        _scan("scan_packed_train", "train", 1, 16384, 1000, dtype="fp16", gates=False, packed=12),
+        # The norm in front of a decode step's projections: 8-bit rows and the residual stream.
+        _norm("norm_step", "quant", 32, 2048),
+        # The same for a prompt.
+        _norm("norm_prompt", "quant", 8192, 4096),
+        # The pre-norm of a training step.
+        _norm("norm_train", "train", 16384, 2048),
+        # Half precision with the residual stream kept in 32 bits, odd numbers of rows and columns.
+        _norm("norm_ragged_train", "train", 5003, 1001, dtype="fp16", residual="fp32"),
+        # A single token's projection: the weights' bytes.
+        _linear("linear_step", 1, 4096, 2048),
+        # The output projection of a decode batch, added to the residual stream.
+        _linear("linear_batch", 48, 2048, 8192, residual=True),
+        # The input projection of a prompt, activation in the epilogue.
+        _linear("linear_prompt", 8191, 8192, 2048, act="silu"),
+    ]
+
+
+def _spread(rng, lo, hi):
+    """A whole number of lo..hi, even over its logarithm."""
+    return min(hi, max(lo, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def _cost(case):
+    w = work(case)
+    return max(w["bytes"] / 4e12, w["flops"] / 1e15)
+
+
+def draw(rng):
+    most = max(_cost(c) for c in listed())
+    while True:
+        op = rng.choice(["scan", "scan", "norm", "linear", "linear"])
+        dtype = rng.choice(["bf16", "bf16", "fp16", "fp32"])
+        if op == "scan":
+            mode = rng.choice(["step", "forward", "train"])
+            dim = rng.choice([8 * _spread(rng, 8, 512), _spread(rng, 64, 4096)])
+            packed = rng.choice([0, 0, _spread(rng, 2, 40)]) if mode != "step" else 0
+            gates = rng.random() < 0.5
+            case = _scan(None, mode, 1 if packed else _spread(rng, 1, 256 if mode == "step" else 16),
+                         1 if mode == "step" else _spread(rng, max(16, packed), 32768), dim, dtype, gates,
+                         rng.choice([dtype, "fp32"]), gates and rng.random() < 0.5, packed, mode == "step" or rng.random() < 0.6)
+        elif op == "norm":
+            dim = rng.choice([8 * _spread(rng, 8, 1024), _spread(rng, 64, 8192)])
+            case = _norm(None, rng.choice(["quant", "train"]), _spread(rng, 1, 32768), dim, dtype, rng.choice([dtype, "fp32"]))
+        else:
+            case = _linear(None, rng.choice([_spread(rng, 1, 64), _spread(rng, 65, 16384)]), _spread(rng, 256, 16384),
+                           16 * _spread(rng, 16, 512), dtype, rng.random() < 0.5, rng.choice(["none", "silu", "gelu", "relu"]),
+                           rng.random() < 0.5)
+        if _cost(case) <= most:
+            return case
+
+
+# ---------------------------------------------------------------------------------------------------- inputs
+def _rows8(x):
+    """Rows in 8 bits with a scale each."""
+    scale = x.abs().amax(-1).clamp_min(AMAX_MIN) / E4M3_MAX
+    return (x / scale[..., None]).to(torch.float8_e4m3fn), scale
+
+
+def _lengths(case):
+    """The sequence lengths of a packed batch: some short, some long, at least one token each."""
+    n, total = case["packed"], case["tokens"]
+    share = [1 + 7 * ((i * 5 + 3) % 8) ** 2 for i in range(n)]
+    lens = [1 + (total - n) * s // sum(share) for s in share]
+    lens[-1] += total - sum(lens)
+    return lens
+
+
+def prepare(case, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    dtype = DTYPES[case["dtype"]]
+
+    def normal(*shape, std=1.0, mean=0.0, dtype=dtype):
+        return torch.randn(*shape, generator=gen, device="cuda").mul_(std).add_(mean).to(dtype)
+
+    s = {"case": case}
+    if case["op"] == "scan":
+        B, T, D = case["batch"], case["tokens"], case["dim"]
+        n = case["packed"] or B
+        s["x"] = normal(B, T, D)
+        if case["gates"]:
+            s["g"] = normal(B, T, D, mean=1.0, std=1.5, dtype=DTYPES[case["gate_dtype"]])   # decays around 0.7
+        else:
+            g = torch.nn.functional.logsigmoid(torch.randn(B, T, D, generator=gen, device="cuda")) / 16
+            s["g"] = g.to(DTYPES[case["gate_dtype"]])
+        s["bound"] = torch.rand(D, generator=gen, device="cuda") * 0.9 if case["bound"] else None
+        s["h0"] = normal(n, D, dtype=torch.float32) if case["state"] else None
+        s["offsets"] = None
+        if case["packed"]:
+            s["offsets"] = torch.tensor([0] + _lengths(case), device="cuda").cumsum(0)
+        if case["mode"] == "train":
+            s["do"] = normal(B, T, D)
+            s["dht"] = normal(n, D, dtype=torch.float32)
+            for k in ("x", "g", "bound", "h0"):
+                if s[k] is not None:
+                    s[k].requires_grad_()
+    elif case["op"] == "norm":
+        M, N = case["rows"], case["dim"]
+        s["x"], s["residual"] = normal(M, N), normal(M, N, std=2.0, dtype=DTYPES[case["residual"]])
+        s["w"] = normal(N, std=0.2, mean=1.0)
+        if case["mode"] == "train":
+            s["dy"], s["ds"] = normal(M, N), normal(M, N, dtype=DTYPES[case["residual"]])
+            for k in ("x", "residual", "w"):
+                s[k].requires_grad_()
+    else:
+        M, N, K = case["rows"], case["out"], case["inner"]
+        s["x"] = _rows8(normal(M, K, dtype=torch.float32))
+        s["w"] = _rows8(normal(N, K, std=K ** -0.5, dtype=torch.float32))
+        s["bias"] = normal(N, std=0.5) if case["bias"] else None
+        s["residual"] = normal(M, N) if case["residual"] else None
+    return s
+
+
+# ---------------------------------------------------------------------------------------------------- plain forms
+def _affine_scan(a, u):
+    """h_t = a_t h_{t-1} + u_t over dim 1 from h = 0: spans of 1, 2, 4, ... tokens joined."""
+    span, T = 1, a.shape[1]
+    while span < T:
+        u = torch.cat([u[:, :span], torch.addcmul(u[:, span:], a[:, span:], u[:, :-span])], 1)
+        if 2 * span < T:
+            a = torch.cat([a[:, :span], a[:, span:] * a[:, :-span]], 1)
+        span *= 2
+    return u
+
+
+def _ends(s):
+    """Rows of the first and last token of every sequence in the flattened [B*T] order."""
+    B, T, _ = s["x"].shape
+    if s["offsets"] is not None:
+        return s["offsets"][:-1], s["offsets"][1:] - 1
+    first = torch.arange(B, device="cuda") * T
+    return first, first + T - 1
+
+
+def _scan_plain(s):
+    case, (B, T, D) = s["case"], s["x"].shape
+    x, g = s["x"].detach().float(), s["g"].detach().float()
+    lb = None if s["bound"] is None else s["bound"].detach()
+    if case["gates"]:
+        sig, si = torch.sigmoid(g), torch.sigmoid(x)
+        a = sig if lb is None else lb + (1 - lb) * sig
+        keep = torch.sigmoid(-g) if lb is None else (1 - lb) * torch.sigmoid(-g)      # 1 - a
+        u = keep * x * si
+    else:
+        a, u = torch.exp(g), x
+    if T == 1:      # a step: the state is updated where it lies
+        h = a[:, 0] * s["h0"] + u[:, 0]
+        s["h0"].copy_(h)
+        return h[:, None].to(s["x"].dtype), s["h0"]
+    first, last = _ends(s)
+    h0 = torch.zeros(first.numel(), D, device="cuda") if s["h0"] is None else s["h0"].detach()
+    a0 = a.reshape(-1, D)[first]
+    cut = a.reshape(-1, D).index_fill(0, first, 0.0).view(B, T, D)                     # a sequence's first token drops what is before it
+    h = _affine_scan(cut, u.reshape(-1, D).index_add(0, first, a0 * h0).view(B, T, D))
+    ht = h.reshape(-1, D)[last]
+    if case["mode"] != "train":
+        return h.to(s["x"].dtype), ht
+    # l_t = do_t + a_{t+1} l_{t+1}: the same recurrence from the right
+    do = s["do"].float().reshape(-1, D).index_add(0, last, s["dht"]).view(B, T, D)
+    later = torch.cat([cut[:, 1:], torch.zeros_like(cut[:, :1])], 1)
+    lam = _affine_scan(later.flip(1), do.flip(1)).flip(1)
+    dh0 = a0 * lam.reshape(-1, D)[first]
+    before = torch.cat([torch.zeros_like(h[:, :1]), h[:, :-1]], 1).reshape(-1, D).index_copy(0, first, h0).view(B, T, D)
+    out = [h.to(s["x"].dtype), ht]
+    if case["gates"]:
+        da = lam * (before - x * si)
+        dsig = da if lb is None else da * (1 - lb)
+        out += [(lam * keep * si * (1 + x * (1 - si))).to(s["x"].dtype), (dsig * sig * torch.sigmoid(-g)).to(s["g"].dtype)]
+        out += [] if lb is None else [(da * torch.sigmoid(-g)).sum((0, 1))]
+    else:
+        out += [lam.to(s["x"].dtype), (lam * before * a).to(s["g"].dtype)]
+    return out + ([] if s["h0"] is None else [dh0])
+
+
+def _norm_plain(s):
+    x, r, w = s["x"].detach().float(), s["residual"].detach().float(), s["w"].detach().float()
+    t = x + r
+    rstd = torch.rsqrt(t.square().mean(-1, keepdim=True) + EPS)
+    y = t * rstd * w
+    kept = t.to(s["residual"].dtype)
+    if s["case"]["mode"] == "quant":
+        return (*_rows8(y), kept)
+    xh = kept.float() * rstd
+    dy = s["dy"].float()
+    wdy = dy * w
+    dt = (wdy - xh * (xh * wdy).mean(-1, keepdim=True)) * rstd + s["ds"].float()
+    return y.to(s["x"].dtype), kept, dt.to(s["x"].dtype), dt.to(s["residual"].dtype), (dy * xh).sum(0).to(s["w"].dtype)
+
+
+def _act(y, act):
+    if act == "silu":
+        return y * torch.sigmoid(y)
+    if act == "gelu":
+        return y * 0.5 * (1 + torch.erf(y * 0.5 ** 0.5))
+    return y.clamp_min(0) if act == "relu" else y
+
+
+def _linear_plain(s):
+    case, (xq, xs), (wq, ws) = s["case"], s["x"], s["w"]
+    y = (xq.float() @ wq.float().t()) * xs[:, None] * ws
+    if s["bias"] is not None:
+        y = y + s["bias"].float()
+    y = _act(y, case["act"])
+    if s["residual"] is not None:
+        y = y + s["residual"].float()
+    return y.to(DTYPES[case["dtype"]])
+
+
+# ---------------------------------------------------------------------------------------------------- the package
+def _package():
+    path = os.path.join(os.getcwd(), "flash-linear-attention_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import fla_amd
+    return fla_amd
+
+
+def _scan_own(s):
+    hgrn, case = _package().ops.hgrn, s["case"]
+    how = {"use_gate_in_kernel": case["gates"], "lower_bound": s["bound"], "initial_state": s["h0"], "output_final_state": True}
+    if case["mode"] == "step":
+        return hgrn.fused_recurrent_hgrn(s["x"], s["g"], inplace_state=True, **how)
+    o, ht = hgrn.chunk_hgrn(s["x"], s["g"], cu_seqlens=s["offsets"], **how)
+    if case["mode"] != "train":
+        return o, ht
+    leaves = [s[k] for k in ("x", "g", "bound", "h0") if s[k] is not None]
+    return [o, ht, *torch.autograd.grad((o, ht), leaves, (s["do"], s["dht"]))]
+
+
+def _norm_own(s):
+    modules = _package().modules
+    if s["case"]["mode"] == "quant":
+        (q, scale), kept = modules.rms_norm(s["x"], s["w"], residual=s["residual"], prenorm=True, eps=EPS, quantize=True)
+        return q, scale, kept
+    y, kept = modules.rms_norm(s["x"], s["w"], residual=s["residual"], prenorm=True, eps=EPS)
+    return [y, kept, *torch.autograd.grad((y, kept), (s["x"], s["residual"], s["w"]), (s["dy"], s["ds"]))]
+
+
+def _linear_own(s):
+    case = s["case"]
+    return _package().modules.quant_linear(s["x"], s["w"], s["bias"], activation=None if case["act"] == "none" else case["act"],
+                                           residual=s["residual"], output_dtype=DTYPES[case["dtype"]])
+
+
+def run(state):
+    op = state["case"]["op"]
+    if own:
+        return {"scan": _scan_own, "norm": _norm_own, "linear": _linear_own}[op](state)
+    return {"scan": _scan_plain, "norm": _norm_plain, "linear": _linear_plain}[op](state)
+
+
+# ---------------------------------------------------------------------------------------------------- work
+def work(case):
+    """Every input read once, every output written once."""
+    e = BYTES[case["dtype"]]
+    if case["op"] == "scan":
+        n = case["batch"] * case["tokens"] * case["dim"]
+        states = (case["packed"] or case["batch"]) * case["dim"] * 4
+        g = BYTES[case["gate_dtype"]]
+        train = case["mode"] == "train"
+        return {"bytes": n * (2 * e + g + (2 * e + g if train else 0)) + states * (1 + case["state"]) * (2 if train else 1),
+                "flops": n * (2 + 10 * case["gates"]) * (3 if train else 1)}
+    if case["op"] == "norm":
+        n, r = case["rows"] * case["dim"], BYTES[case["residual"]]
+        if case["mode"] == "quant":
+            return {"bytes": n * (e + 2 * r + 1), "flops": 6 * n}
+        return {"bytes": n * (e + 2 * r + e) + n * (e + r + e + r), "flops": 16 * n}
+    M, N, K = case["rows"], case["out"], case["inner"]
+    return {"bytes": (M + N) * K + M * N * e * (1 + case["residual"]) + 4 * (M + N), "flops": 2 * M * N * K}
+
+
+# ---------------------------------------------------------------------------------------------------- 64 bits
+def _scan_exact(s):
+    """One token after the other."""
+    case, (B, T, D) = s["case"], s["x"].shape
+    x, g = s["x"].detach().double(), s["g"].detach().double()
+    lb = None
+    if case["gates"]:
+        lb = torch.zeros(D, device="cuda", dtype=torch.float64) if s["bound"] is None else s["bound"].detach().double()
+        sf, si = 1 / (1 + torch.exp(-g)), 1 / (1 + torch.exp(-x))
+        a = lb + (1 - lb) * sf
+        u = (1 - lb) * (1 / (1 + torch.exp(g))) * x * si
+    else:
+        a, u = torch.exp(g), x
+    bounds = s["offsets"].tolist() if s["offsets"] is not None else [0, T]
+    per = B if s["offsets"] is None else 1
+    n = per * (len(bounds) - 1)
+    h0 = torch.zeros(n, D, device="cuda", dtype=torch.float64) if s["h0"] is None else s["h0"].detach().double()
+    h, before, ht, dh0 = torch.empty_like(u), torch.empty_like(u), torch.empty_like(h0), torch.empty_like(h0)
+    lam = torch.empty_like(u) if case["mode"] == "train" else None
+    for q, (lo, hi) in enumerate(zip(bounds[:-1], bounds[1:])):
+        rows = slice(q * per, (q + 1) * per)
+        c = h0[rows]
+        for t in range(lo, hi):
+            before[:, t] = c
+            c = a[:, t] * c + u[:, t]
+            h[:, t] = c
+        ht[rows] = c
+        if lam is not None:
+            m = s["dht"].double()[rows]
+            for t in range(hi - 1, lo - 1, -1):
+                l = s["do"][:, t].double() + m
+                lam[:, t] = l
+                m = a[:, t] * l
+            dh0[rows] = m
+    if lam is None:
+        return h, ht
+    out = [h, ht]
+    if case["gates"]:
+        da = lam * (before - x * si)
+        out += [lam * (1 - a) * (si + x * si * (1 - si)), da * (1 - lb) * sf * (1 - sf)]
+        out += [] if s["bound"] is None else [(da * (1 - sf)).sum((0, 1))]
+    else:
+        out += [lam, lam * before * a]
+    return out + ([] if s["h0"] is None else [dh0])
+
+
+def _norm_exact(s):
+    x, r, w = (s[k].detach().double().requires_grad_() for k in ("x", "residual", "w"))
+    t = x + r
+    y = t / torch.sqrt((t * t).mean(-1, keepdim=True) + EPS) * w
+    if s["case"]["mode"] == "quant":
+        scale = y.abs().amax(-1).clamp_min(AMAX_MIN) / E4M3_MAX
+        return None, scale.detach(), t.detach()      # the 8-bit rows: values next to a rounding border go either way
+    grads = torch.autograd.grad((y, t), (x, r, w), (s["dy"].double(), s["ds"].double()))
+    return [y.detach(), t.detach(), *grads]
+
+
+def _linear_exact(s):
+    case, (xq, xs), (wq, ws) = s["case"], s["x"], s["w"]
+    y = torch.mm(xq.double() * xs.double()[:, None], (wq.double() * ws.double()[:, None]).t().contiguous())
+    y = y if s["bias"] is None else y + s["bias"].double()
+    y = {"none": lambda v: v, "silu": lambda v: v / (1 + torch.exp(-v)), "relu": torch.relu,
+         "gelu": lambda v: v * (1 - torch.erfc(v / math.sqrt(2.0)) / 2)}[case["act"]](y)
+    return y if s["residual"] is None else y + s["residual"].double()
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    if case["op"] == "scan" and case["tokens"] * (1 + (case["mode"] == "train")) > 70000:
+        return None
+    return {"scan": _scan_exact, "norm": _norm_exact, "linear": _linear_exact}[case["op"]](s)
