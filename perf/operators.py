@@ -96,7 +96,7 @@ def draw(rng):
             case = _norm(None, rng.choice(["quant", "train"]), _spread(rng, 1, 32768), dim, dtype, rng.choice([dtype, "fp32"]))
         else:
             case = _linear(None, rng.choice([_spread(rng, 1, 64), _spread(rng, 65, 16384)]), _spread(rng, 256, 16384),
-                           16 * _spread(rng, 16, 512), dtype, rng.random() < 0.5, rng.choice(["none", "silu", "gelu", "relu"]),
+                           16 * _spread(rng, 16, 512), rng.choice(["bf16", "fp16"]), rng.random() < 0.5, rng.choice(["none", "silu", "gelu", "relu"]),
                            rng.random() < 0.5)
         if _cost(case) <= most:
             return case
