@@ -1,0 +1,184 @@
+// The elementwise gated recurrence h_t = a_t h_{t-1} + u_t, what its forward and backward launches share.
+//
+// A step is an affine map of the state, so a run of steps is one too: (A, H) with h -> A h + H, joined in order.  A workgroup
+// owns 64 channels of a segment of a sequence and goes through it in tiles of 256 tokens (backward: 128): eight waves of 32 rows, a lane
+// four (two) rows of eight channels (16 bytes a load in 16 bits, a wave's load covers eight whole 128-byte rows).  A tile is joined in
+// three levels: the lane's rows in registers, the eight row groups of a wave by shuffles, the eight waves through LDS (one
+// barrier a tile).  Between tiles the state stays in a register of the lane with that channel's number.
+//
+// Sequences are cut into segments where (sequence, 64 channels) pairs would leave CUs idle; a first launch then forms each
+// segment's map, and every workgroup of the second joins the maps of the segments ahead of its own (a fixed order, no atomics,
+// nothing waits for another workgroup).
+#pragma once
+#include "fla_common.h"
+#include "row_vec.h"
+
+namespace {
+
+constexpr int kCh = 64;                           // channels of a workgroup
+constexpr int kWaves = 8, kGroups = 8;            // waves, row groups of a wave
+constexpr int kFwdRows = 4, kBwdRows = 2;         // rows of a lane: what fits its registers
+constexpr int kKept = FLA_HGRN_STATE_ROWS;        // rows from one kept state to the next
+static_assert(kKept == kGroups * kBwdRows, "a wave of the backward starts from a kept state");
+static_assert(FLA_HGRN_TILE == kWaves * kGroups * kFwdRows, "segments are whole tiles");
+
+struct HgrnParams {
+  const void* x;        // u, or the pre-activations i  [B,T,D], rows ldx apart
+  const void* g;        // log a, or the pre-activations f, rows ldg apart
+  const float* lb;      // [D] or NULL
+  const float* h0;      // [N,D] or NULL
+  void* o;              // [B,T,D]
+  float* ht;            // [N,D] or NULL
+  float* states;        // [B*T / 16 + N + 1, D] or NULL: the state ahead of every 16 rows of a sequence
+  float* maps;          // [segments, 2, D] or NULL (uncut)
+  // backward
+  const void* dout;     // [B,T,D] or NULL (zeros)
+  const float* dht;     // [N,D] or NULL (zeros)
+  void* dx;
+  void* dg;
+  float* dh0;           // [N,D] or NULL
+  float* dlb;           // [segments, D] or NULL
+  const int64_t* offsets;
+  const int64_t* indices;       // [NT,2] (sequence, segment)
+  const int64_t* chunk_offsets; // [N+1] first segment of a sequence
+  int64_t NT, segment, T, ldx, ldg;
+  int D, ncb, nseg;     // nseg: segments of a sequence of a batch without offsets
+};
+
+struct Segment {
+  int64_t n, c, count, first;   // sequence, number in it, segments of it, its first one
+  int64_t bos, begin, len;      // rows: the sequence's first, the segment's first, the segment's number
+  int64_t id;                   // n's segment c among all
+};
+// Segment number `id`; of a packed batch's numbers from NT on, NT + n stands for sequence n if that is empty.
+FLA_DEVICE Segment find_segment(const HgrnParams& p, int64_t id, bool* exists) {
+  Segment s;
+  s.id = id;
+  *exists = true;
+  if (!p.offsets) {
+    s.n = id / p.nseg;
+    s.c = id % p.nseg;
+    s.count = p.nseg;
+    s.first = s.n * p.nseg;
+    s.bos = s.n * p.T;
+    s.begin = s.bos + s.c * p.segment;
+    s.len = p.T - s.c * p.segment;
+  } else if (id < p.NT) {
+    s.n = p.indices[2 * id];
+    s.c = p.indices[2 * id + 1];
+    s.first = p.chunk_offsets[s.n];
+    s.count = p.chunk_offsets[s.n + 1] - s.first;
+    s.bos = p.offsets[s.n];
+    s.begin = s.bos + s.c * p.segment;
+    s.len = p.offsets[s.n + 1] - s.begin;
+  } else {
+    s.n = id - p.NT;
+    s.c = 0;
+    s.first = 0;
+    s.count = 1;
+    s.bos = s.begin = p.offsets[s.n];
+    s.len = 0;
+    *exists = p.offsets[s.n + 1] == s.bos;
+  }
+  if (s.len > p.segment) s.len = p.segment;
+  return s;
+}
+// The kept states of sequence n, which begins at row bos, start here: no two sequences share a slot.
+FLA_DEVICE int64_t state_slot(const Segment& s) { return s.bos / kKept + s.n; }
+
+// sigmoid(x) and 1 - sigmoid(x), each to its own relative precision: from e^{-|x|}, which neither overflows nor cancels
+FLA_DEVICE void sigmoid_both(float x, float* s, float* rest) {
+  const float z = __expf(-__builtin_fabsf(x)), r = __builtin_amdgcn_rcpf(1.f + z), small = z * r;
+  *s = x >= 0.f ? r : small;
+  *rest = x >= 0.f ? small : r;
+}
+
+// The decay of a step, and with GATES the weight 1 - a of its input
+template <bool GATES>
+FLA_DEVICE float decay_of(float g, float lb, float* keep) {
+  if (!GATES) {
+    *keep = 1.f;
+    return __expf(g);
+  }
+  float s, rest;
+  sigmoid_both(g, &s, &rest);
+  *keep = (1.f - lb) * rest;
+  return fmaf(1.f - lb, s, lb);
+}
+
+// A map on its way through the eight row groups of a wave: joined with those of lower (UP) or higher groups, own group included
+template <bool UP>
+FLA_DEVICE void join_groups(float A[VEC], float H[VEC], int group) {
+#pragma unroll
+  for (int d = 1; d < kGroups; d *= 2) {
+    const bool has = UP ? group >= d : group + d < kGroups;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const float a = UP ? __shfl_up(A[i], 8 * d, 64) : __shfl_down(A[i], 8 * d, 64);
+      const float h = UP ? __shfl_up(H[i], 8 * d, 64) : __shfl_down(H[i], 8 * d, 64);
+      H[i] = has ? fmaf(A[i], h, H[i]) : H[i];
+      A[i] = has ? A[i] * a : A[i];
+    }
+  }
+}
+
+// What the waves of a tile exchange: their maps (two tiles' worth: one barrier a tile), and a wave's own entering state.
+struct TileShare {
+  float A[2][kWaves][kCh], H[2][kWaves][kCh];
+  float in[kWaves][kCh];
+};
+// Leaves a wave's map, whose eight channels the lanes of one group hold, and returns the state that enters this wave; `carry`,
+// the state that enters the tile, becomes the one that leaves it (both for the channel with the lane's number), and `all` the
+// product of the decays.  UP: waves in ascending order.
+template <bool UP>
+FLA_DEVICE float join_waves(TileShare& sh, int buf, const float A[VEC], const float H[VEC], bool holds, int wave, int lane, float* carry,
+                            float* all) {
+  if (holds) {
+    const int c = (lane & 7) * VEC;
+    *(f32x4*)&sh.A[buf][wave][c] = f32x4{A[0], A[1], A[2], A[3]};
+    *(f32x4*)&sh.A[buf][wave][c + 4] = f32x4{A[4], A[5], A[6], A[7]};
+    *(f32x4*)&sh.H[buf][wave][c] = f32x4{H[0], H[1], H[2], H[3]};
+    *(f32x4*)&sh.H[buf][wave][c + 4] = f32x4{H[4], H[5], H[6], H[7]};
+  }
+  lds_barrier();
+  float c = *carry, mine = c, prod = *all;
+#pragma unroll
+  for (int k = 0; k < kWaves; ++k) {
+    const int w = UP ? k : kWaves - 1 - k;
+    if (w == wave) mine = c;
+    const float a = sh.A[buf][w][lane];
+    c = fmaf(a, c, sh.H[buf][w][lane]);
+    prod *= a;
+  }
+  *carry = c;
+  *all = prod;
+  return mine;
+}
+// The lane's eight channels of a value that lanes hold by channel number (within the wave: LDS operations of one wave are in order)
+FLA_DEVICE void spread(TileShare& sh, float v, int wave, int lane, float o[VEC]) {
+  sh.in[wave][lane] = v;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  const int c = (lane & 7) * VEC;
+  const f32x4 a = *(const f32x4*)&sh.in[wave][c], b = *(const f32x4*)&sh.in[wave][c + 4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    o[i] = a[i];
+    o[4 + i] = b[i];
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+}
+// joins the map of a run of steps onto the state ahead of it
+FLA_DEVICE float onto(float A, float H, float h) { return fmaf(A, h, H); }
+
+// the types of (x, g)
+#define HGRN_TYPES(D) \
+  D(FLA_BF16, bf16, FLA_BF16, bf16) D(FLA_BF16, bf16, FLA_F32, float) D(FLA_F16, f16, FLA_F16, f16) \
+  D(FLA_F16, f16, FLA_F32, float) D(FLA_F32, float, FLA_F32, float)
+
+// whether rows ld apart can be read 16 bytes at a time
+inline bool wide_rows(const void* p, int64_t ld, int64_t D, int type) {
+  const int64_t e = type == FLA_F32 ? 4 : 2;
+  return (uintptr_t)p % 16 == 0 && ld * e % 16 == 0 && D % VEC == 0;
+}
+
+}  // namespace

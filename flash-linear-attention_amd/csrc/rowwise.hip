@@ -10,90 +10,9 @@
 // walked with a grid-stride loop so that the per-column weight/bias gradients of the gated
 // norm are accumulated in registers and leave the chip once per workgroup.
 #include "fla_common.h"
+#include "row_vec.h"
 
 namespace {
-
-constexpr int VEC = 8;
-
-template <typename T>
-struct Row8;
-template <>
-struct Row8<float> {
-  struct raw {
-    f32x4 a, b;
-  };
-  static FLA_DEVICE raw load_raw(const float* p) { return raw{*(const f32x4*)p, *(const f32x4*)(p + 4)}; }
-  static FLA_DEVICE void unpack(const raw& r, float* o) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      o[i] = r.a[i];
-      o[4 + i] = r.b[i];
-    }
-  }
-  static FLA_DEVICE void load(const float* p, float* o) {
-    f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      o[i] = a[i];
-      o[4 + i] = b[i];
-    }
-  }
-  static FLA_DEVICE void store(float* p, const float* v) {
-    *(f32x4*)p = f32x4{v[0], v[1], v[2], v[3]};
-    *(f32x4*)(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
-  }
-};
-template <>
-struct Row8<bf16> {
-  typedef bf16x8 raw;
-  static FLA_DEVICE raw load_raw(const bf16* p) { return *(const bf16x8*)p; }
-  static FLA_DEVICE void unpack(const raw& r, float* o) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = (float)r[i];
-  }
-  static FLA_DEVICE void load(const bf16* p, float* o) {
-    bf16x8 a = *(const bf16x8*)p;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = (float)a[i];
-  }
-  static FLA_DEVICE void store(bf16* p, const float* v) {
-    bf16x8 a;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = (bf16)v[i];
-    *(bf16x8*)p = a;
-  }
-};
-template <>
-struct Row8<f16> {
-  typedef f16x8 raw;
-  static FLA_DEVICE raw load_raw(const f16* p) { return *(const f16x8*)p; }
-  static FLA_DEVICE void unpack(const raw& r, float* o) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = (float)r[i];
-  }
-  static FLA_DEVICE void load(const f16* p, float* o) {
-    f16x8 a = *(const f16x8*)p;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = (float)a[i];
-  }
-  static FLA_DEVICE void store(f16* p, const float* v) {
-    f16x8 a;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = (f16)v[i];
-    *(f16x8*)p = a;
-  }
-};
-
-// sum over the LPR lanes of a group (LPR a power of two <= 64), result in every lane
-template <int LPR>
-FLA_DEVICE float group_sum(float x) {
-#pragma unroll
-  for (int m = LPR / 2; m >= 1; m >>= 1) x += __shfl_xor(x, m, 64);
-  return x;
-}
-
-// the hardware reciprocal (1 ulp) instead of an IEEE division: ten instructions less per element
-FLA_DEVICE float sigmoidf(float x) { return __builtin_amdgcn_rcpf(1.f + __expf(-x)); }
 
 // ------------------------------------------------------------------ l2norm
 // NP column passes of 8*LPR elements cover a row; lanes past the end of the row idle.

@@ -634,6 +634,96 @@ struct NormGateNode : torch::autograd::Function<NormGateNode> {
   }
 };
 
+// ---------------------------------------------------------------------------------------------------- elementwise recurrence
+// Rows of a [B,T,D] operand as the kernels take them: elements next to each other, all rows one pitch apart (a slice of a wider
+// projection is such a one).  Anything else is copied first.
+Tensor pitched(const Tensor& x, int64_t* ld) {
+  const int64_t B = x.size(0), T = x.size(1), D = x.size(2);
+  const int64_t pitch = T > 1 ? x.stride(1) : B > 1 ? x.stride(0) : D;
+  const bool fits = (D == 1 || x.stride(2) == 1) && pitch >= D && (T == 1 || B == 1 || x.stride(0) == T * x.stride(1));
+  *ld = fits ? pitch : D;
+  return fits ? x : x.contiguous();
+}
+
+struct HgrnArgs {
+  PlanPtr plan;           // chunks of `segment` tokens
+  int64_t B, T, D, N, segment;
+  bool gates, want_ht;
+  // whether some sequence has more than one segment
+  bool cut() const {
+    if (!plan) return T > segment;
+    int64_t used = 0;
+    for (int64_t i = 0; i < plan->N; ++i) used += plan->host[i + 1] > plan->host[i];
+    return plan->NT > used;
+  }
+  int64_t segments() const { return plan ? plan->NT : B * ((T + segment - 1) / segment); }
+  Tensor maps(const Tensor& like) const { return cut() ? fresh({segments(), 2, D}, like, at::kFloat) : Tensor(); }
+  // rows of a packed batch that belong to no sequence are zeros
+  Tensor rows(const Tensor& like) const {
+    return !plan || plan->covers(0, T) ? at::empty({B, T, D}, like.options()) : at::zeros({B, T, D}, like.options());
+  }
+};
+
+Tensor hgrn_forward(const Tensor& x_, const Tensor& g_, const Tensor& lb, const Tensor& h0, const HgrnArgs& a, Tensor* ht, Tensor* states) {
+  int64_t ldx, ldg;
+  const Tensor x = pitched(x_, &ldx), g = pitched(g_, &ldg);
+  Tensor o = a.rows(x), maps = a.maps(x);
+  if (a.want_ht && !ht->defined()) *ht = fresh({a.N, a.D}, x, at::kFloat);
+  if (states) *states = fresh({a.B * a.T / FLA_HGRN_STATE_ROWS + a.N + 1, a.D}, x, at::kFloat);
+  if (a.T == 1 && !a.plan && !states)
+    check(fla_hgrn_step(ptr(x), ptr(g), fptr(lb), fptr(h0), ptr(o), fptr(*ht), a.gates, dt(x), dt(g), a.N, a.D, ldx, ldg, stream_of(x)),
+          "fla_hgrn_step");
+  else
+    check(fla_hgrn_fwd(ptr(x), ptr(g), fptr(lb), fptr(h0), ptr(o), fptr(*ht), states ? fptr(*states) : nullptr, fptr(maps), offs(a.plan),
+                       idx(a.plan), coff(a.plan), a.plan ? a.plan->NT : 0, a.segment, a.gates, dt(x), dt(g), a.B, a.T, a.D, a.N, ldx, ldg,
+                       stream_of(x)),
+          "fla_hgrn_fwd");
+  return o;
+}
+
+struct HgrnNode : torch::autograd::Function<HgrnNode> {
+  struct Rest {
+    HgrnArgs a;
+    bool has_h0;
+  };
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& g, const Maybe& lb_, const Maybe& h0_,
+                               const Maybe& offsets, const HgrnArgs& a) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const Tensor lb = given(lb_), h0 = given(h0_);
+    Tensor ht, states;
+    Tensor o = hgrn_forward(x, g, lb, h0, a, &ht, &states);
+    ctx->save_for_backward({x, g, lb, states, given(offsets)});
+    ctx->set_materialize_grads(false);
+    hold(ctx, Rest{a, h0.defined()});
+    return a.want_ht ? variable_list{o, ht} : variable_list{o};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const auto saved = ctx->get_saved_variables();
+    const Rest& r = held<Rest>(ctx);
+    const HgrnArgs& a = r.a;
+    int64_t ldx, ldg;
+    const Tensor x = pitched(saved[0], &ldx), g = pitched(saved[1], &ldg);
+    const Tensor &lb = saved[2], &states = saved[3];
+    c10::DeviceGuard on_device(x.device());
+    const Tensor dout = grads[0].defined() ? as(grads[0], x.scalar_type()).contiguous() : Tensor();
+    const Tensor dht = a.want_ht ? f32(grads[1]) : Tensor();
+    Tensor dx = a.rows(x), dg = a.rows(g), maps = a.maps(x);
+    Tensor dh0 = r.has_h0 ? fresh({a.N, a.D}, x, at::kFloat) : Tensor();
+    const int64_t segments = a.segments();
+    Tensor part = lb.defined() && segments > 0 ? fresh({segments, a.D}, x, at::kFloat) : Tensor();
+    check(fla_hgrn_bwd(ptr(x), ptr(g), fptr(lb), fptr(states), ptr(dout), fptr(dht), ptr(dx), ptr(dg), fptr(dh0), fptr(part), fptr(maps),
+                       offs(a.plan), idx(a.plan), coff(a.plan), a.plan ? a.plan->NT : 0, a.segment, a.gates, dt(x), dt(g), a.B, a.T, a.D,
+                       a.N, ldx, ldg, stream_of(x)),
+          "fla_hgrn_bwd");
+    Tensor dlb;
+    if (part.defined()) dlb = sum_partials(part, {a.D}, at::kFloat);
+    else if (lb.defined()) dlb = at::zeros({a.D}, x.options().dtype(at::kFloat));
+    return {dx, dg, dlb, dh0, Tensor(), Tensor()};
+  }
+};
+
 // ---------------------------------------------------------------------------------------------------- Python entries
 Tensor arg_tensor(PyObject* o) {
   if (o == Py_None) return Tensor();
@@ -953,6 +1043,78 @@ PyObject* py_norm_gate(PyObject*, PyObject* const* p, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+bool floating(const Tensor& x) { return is16(x) || x.scalar_type() == at::kFloat; }
+void need_gpu(std::initializer_list<const Tensor*> ts) {
+  const Tensor* first = nullptr;
+  for (const Tensor* t : ts) {
+    if (!t->defined()) continue;
+    TORCH_CHECK(t->is_cuda(), "fla_amd: the HIP kernels need tensors on a GPU device; there is no CPU fallback");
+    if (!first) first = t;
+    TORCH_CHECK_VALUE(t->device() == first->device(), "fla_amd: operands on ", first->device(), " and ", t->device());
+  }
+}
+
+// hgrn(x, g, lower_bound | None, h0 | None, want_ht, plan, segment, gates, inplace, offsets)
+PyObject* py_hgrn(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 10);
+  const Tensor x = arg_tensor(p[0]), offsets = arg_tensor(p[9]);
+  Tensor g = arg_tensor(p[1]), lb = arg_tensor(p[2]), h0 = arg_tensor(p[3]);
+  HgrnArgs a{};
+  a.want_ht = arg_bool(p[4]);
+  a.plan = arg_plan(p[5]);
+  a.gates = arg_bool(p[7]);
+  const bool inplace = arg_bool(p[8]);
+  TORCH_CHECK_VALUE(x.defined() && g.defined() && x.dim() == 3 && g.sizes() == x.sizes(),
+                    "fla_amd hgrn: x and g are [B, T, D] of one shape");
+  TORCH_CHECK_TYPE(floating(x) && g.is_floating_point() && (!lb.defined() || lb.is_floating_point()) &&
+                       (!h0.defined() || h0.is_floating_point()),
+                   "fla_amd hgrn: x in bf16, fp16 or fp32, the other operands in a floating type");
+  TORCH_CHECK_VALUE(!lb.defined() || a.gates, "fla_amd hgrn: a lower bound goes with use_gate_in_kernel=True");
+  a.B = x.size(0), a.T = x.size(1), a.D = x.size(2);
+  a.N = a.plan ? a.plan->N : a.B;
+  TORCH_CHECK_VALUE(!lb.defined() || lb.numel() == a.D, "fla_amd hgrn: lower_bound holds one value per channel, ", a.D);
+  TORCH_CHECK_VALUE(!h0.defined() || (h0.dim() == 2 && h0.size(0) == a.N && h0.size(1) == a.D), "fla_amd hgrn: initial_state is [", a.N, ", ",
+                    a.D, "]");
+  TORCH_CHECK_VALUE(!a.plan || (a.plan->host.front() >= 0 && a.plan->host.back() <= a.T), "fla_amd hgrn: offsets leave the ", a.T, " rows");
+  need_gpu({&x, &g, &lb, &h0});
+  const bool grad = wants_grad({&x, &g, &lb, &h0});
+  if (inplace) {
+    TORCH_CHECK_VALUE(h0.defined() && a.want_ht && h0.scalar_type() == at::kFloat && h0.is_contiguous(),
+                      "fla_amd hgrn: inplace_state needs a contiguous fp32 initial_state and output_final_state=True");
+    TORCH_CHECK_VALUE(!grad, "fla_amd hgrn: inplace_state where a gradient is wanted");
+  }
+  c10::DeviceGuard on_device(x.device());
+  if (g.scalar_type() != at::kFloat && g.scalar_type() != x.scalar_type()) g = g.to(at::kFloat);
+  if (lb.defined()) lb = f32(lb).reshape({a.D});
+  if (h0.defined()) h0 = f32(h0);
+  if (x.numel() == 0 || a.N == 0) {   // no token: the states stay
+    Tensor o = at::zeros(x.sizes(), x.options());
+    Tensor ht;
+    if (a.want_ht) ht = inplace ? h0 : h0.defined() ? h0.clone() : at::zeros({a.N, a.D}, x.options().dtype(at::kFloat));
+    return pair(o, ht);
+  }
+  if (p[6] == Py_None) {
+    a.segment = fla_hgrn_segment(a.B, a.B * a.T, a.T, a.D);
+  } else {
+    a.segment = PyLong_AsLongLong(p[6]);
+    if (a.segment == -1 && PyErr_Occurred()) throw python_error();
+  }
+  if (grad) {
+    auto out = HgrnNode::apply(x, g, maybe(lb), maybe(h0), maybe(offsets), a);
+    return pair(out[0], a.want_ht ? out[1] : Tensor());
+  }
+  at::AutoDispatchBelowADInplaceOrView guard;
+  Tensor ht;
+  // A step writes each state where it read it; a scan's workgroups may still read the initial one when the final one is there
+  const bool direct = inplace && a.T == 1 && !a.plan;
+  if (direct) ht = h0;
+  Tensor o = hgrn_forward(x, g, lb, h0, a, &ht, nullptr);
+  if (inplace && !direct) ht = h0.copy_(ht);
+  return pair(o, ht);
+  END_HANDLE_TH_ERRORS
+}
+
 #define ENTRY(name, fn) {name, (PyCFunction)(void (*)(void))fn, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {
     ENTRY("plan", py_plan),
@@ -966,6 +1128,7 @@ PyMethodDef kMethods[] = {
     ENTRY("causal_conv1d_update", py_conv_update<false>),
     ENTRY("short_conv_step", py_conv_update<true>),
     ENTRY("norm_swish_gate", py_norm_gate),
+    ENTRY("hgrn", py_hgrn),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fla_host", nullptr, -1, kMethods};
 

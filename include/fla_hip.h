@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define FLA_ABI_VERSION 18
+#define FLA_ABI_VERSION 19
 
 enum fla_dtype { FLA_F32 = 0, FLA_BF16 = 1, FLA_F16 = 2 };
 
@@ -795,6 +795,36 @@ int fla_gdn_gate_fwd(const void* a, const void* b, const float* A_log, const flo
 int fla_gdn_gate_bwd(const void* a, const void* b, const float* A_log, const float* dt_bias, const float* dg,
                      const void* dbeta, void* da, void* db, float* partials, int64_t M, int64_t H, int a_dtype,
                      int b_dtype, fla_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * The elementwise gated recurrence (interface of chunk_hgrn / fused_recurrent_hgrn, fla/ops/hgrn):
+ *   h_t = e^{g_t} h_{t-1} + x_t,  o = h
+ * per channel, or with `gates` from the pre-activations i = x and f = g of the layer and a lower bound lb [D] (fp32, or NULL: 0):
+ *   a = lb + (1 - lb) sigmoid(f),  h_t = a h_{t-1} + (1 - a) i sigmoid(i).
+ * x, o, dx, dout [B,T,D] in x_dtype; g, dg in g_dtype (x_dtype, or fp32); rows of x and g ldx and ldg elements apart, those of
+ * the others D.  h0, ht, dht, dh0 fp32 [N,D], may be NULL; dout too (zeros).  States are fp32 throughout.
+ * Packed batches: B == 1, offsets, and indices / chunk_offsets built for chunks of `segment` tokens; rows that belong to no sequence
+ * are not written.  Any D; D and the row pitches in multiples of 16 bytes take the wide loads.
+ *
+ * fla_hgrn_segment: tokens of a segment (a multiple of FLA_HGRN_TILE) for n_seqs sequences of `tokens` in all, the longest
+ * `longest`; `longest` or more: sequences are not cut (host arithmetic).  Sequences of more than one segment need the workspace
+ * maps, fp32 [segments, 2, D] (segments: NT, or B times those of a sequence).
+ * states: fp32 [B*T / FLA_HGRN_STATE_ROWS + N + 1, D] or NULL, kept by a forward for its backward.
+ * dlb_partials: fp32 [segments, D] or NULL, its column sums are the gradient of lb (segments: as above).
+ * fla_hgrn_step: one token for each of N sequences, x, g, o [N, D]; ht may be h0. */
+#define FLA_HGRN_TILE 256
+#define FLA_HGRN_STATE_ROWS 16
+int64_t fla_hgrn_segment(int64_t n_seqs, int64_t tokens, int64_t longest, int64_t D);
+int fla_hgrn_fwd(const void* x, const void* g, const float* lower_bound, const float* h0, void* o, float* ht, float* states,
+                 float* maps, const int64_t* offsets, const int64_t* indices, const int64_t* chunk_offsets, int64_t NT,
+                 int64_t segment, int gates, int x_dtype, int g_dtype, int64_t B, int64_t T, int64_t D, int64_t N, int64_t ldx,
+                 int64_t ldg, fla_stream_t stream);
+int fla_hgrn_bwd(const void* x, const void* g, const float* lower_bound, const float* states, const void* dout, const float* dht,
+                 void* dx, void* dg, float* dh0, float* dlb_partials, float* maps, const int64_t* offsets, const int64_t* indices,
+                 const int64_t* chunk_offsets, int64_t NT, int64_t segment, int gates, int x_dtype, int g_dtype, int64_t B,
+                 int64_t T, int64_t D, int64_t N, int64_t ldx, int64_t ldg, fla_stream_t stream);
+int fla_hgrn_step(const void* x, const void* g, const float* lower_bound, const float* h0, void* o, float* ht, int gates,
+                  int x_dtype, int g_dtype, int64_t N, int64_t D, int64_t ldx, int64_t ldg, fla_stream_t stream);
 
 /* Diagnostics: C[M,N] (fp32) = A[M,Kd] * B[N,Kd]^T with bf16 operands, computed
  * with the same MFMA fragment helpers the kernels use (mode 0: 32x32x16 tiles,
