@@ -1,0 +1,332 @@
+// RMS norm with the residual's addition in front of it, forward and backward, and an output in 8 bits with a scale per row:
+//   s = x + r,   rstd = 1 / sqrt(mean s^2 + eps),   y = s rstd w (+ b)
+//   8 bits:   scale = max(max|y|, 1e-30) / 448,   q = e4m3(y / scale)
+//   ds = (w dy - xh mean(xh w dy)) rstd + ds_out,   dw = sum dy xh,   db = sum dy,   xh = s rstd
+// HBM-streaming: every operand is read once and every result written once, a row stays in the registers of the lanes that hold
+// it (8 elements a lane and pass).  s is summed and normalised in fp32; what is kept of it (residual_out, in the residual's type) is what
+// the backward reads, so xh there carries the rounding of the residual stream and no other.
+#include "fla_common.h"
+#include "row_vec.h"
+
+namespace {
+
+constexpr float kE4M3Max = 448.f, kAmaxMin = 1e-30f;
+
+struct RmsParams {
+  const void* x;        // [M,N]
+  const void* res;      // [M,N] or NULL
+  const void* w;        // [N] or NULL
+  const void* b;        // [N] or NULL
+  void* y;              // [M,N] (or the 8-bit rows)
+  float* scale;         // [M], 8-bit rows only
+  void* res_out;        // [M,N] or NULL
+  float* rstd;          // [M] or NULL; backward: read
+  // backward: x is what the forward normalised, in the type of `kept_f32`
+  const void* dy;
+  const void* dres;     // [M,N] in the kept type, or NULL
+  void* dx;
+  void* dres_in;        // a copy of dx in the kept type, or NULL
+  float* dw_part;       // [gridDim.x, N] or NULL
+  float* db_part;
+  int64_t M;
+  int N;
+  float eps;
+  int res_f32, res_out_f32, w_f32, kept_f32, plain;   // plain: rows are not normalised (8-bit rows of x itself)
+};
+
+template <typename T, bool WIDE>
+FLA_DEVICE void load8_of(const void* base, int f32, int64_t at, int valid, float* o) {
+  if (f32) Row8<float>::unpack(load_raw8<float, WIDE>((const float*)base + at, valid), o);
+  else Row8<T>::unpack(load_raw8<T, WIDE>((const T*)base + at, valid), o);
+}
+template <typename T, bool WIDE>
+FLA_DEVICE void store8_of(void* base, int f32, int64_t at, int valid, const float* v) {
+  if (f32) store8<float, WIDE>((float*)base + at, v, valid);
+  else store8<T, WIDE>((T*)base + at, v, valid);
+}
+
+// Sum or maximum over the TPR threads that hold a row, in every one of them.  Rows of more than a wave go through LDS, `turn`
+// alternating so that a value is not overwritten while another wave still reads it (one barrier an exchange).
+template <int TPR, bool MAX>
+FLA_DEVICE float row_reduce(float v, float (*lds)[TPR > 64 ? TPR / 64 : 1], int turn) {
+  constexpr int W = TPR < 64 ? TPR : 64;
+#pragma unroll
+  for (int m = W / 2; m >= 1; m >>= 1) {
+    const float o = __shfl_xor(v, m, 64);
+    v = MAX ? fmaxf(v, o) : v + o;
+  }
+  if (TPR > 64) {
+    if ((threadIdx.x & 63) == 0) lds[turn][threadIdx.x >> 6] = v;
+    lds_barrier();
+    v = lds[turn][0];
+#pragma unroll
+    for (int i = 1; i < (TPR > 64 ? TPR / 64 : 1); ++i) v = MAX ? fmaxf(v, lds[turn][i]) : v + lds[turn][i];
+  }
+  return v;
+}
+
+// A row for TPR threads, NP passes of 8 elements each; QUANT: the output in 8 bits.
+template <typename T, int TPR, int NP, bool WIDE, bool QUANT>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_fwd_kernel(RmsParams p) {
+  constexpr int BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR;
+  __shared__ float lds[2][TPR > 64 ? TPR / 64 : 1];
+  const int sub = threadIdx.x % TPR, N = p.N;
+  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
+  if (row >= p.M) return;      // (all threads of a row together; a row of several waves is a block's only one)
+  float v[NP][VEC];
+  float ss = 0.f;
+#pragma unroll
+  for (int q = 0; q < NP; ++q) {
+    const int col = (q * TPR + sub) * VEC, valid = N - col;
+    load8_of<T, WIDE>(p.x, 0, row * N + col, valid, v[q]);
+  }
+  if (p.res) {
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+      const int col = (q * TPR + sub) * VEC, valid = N - col;
+      float r[VEC];
+      load8_of<T, WIDE>(p.res, p.res_f32, row * N + col, valid, r);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[q][i] += r[i];
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < NP; ++q) {
+    const int col = (q * TPR + sub) * VEC, valid = N - col;
+    if (p.res_out) store8_of<T, WIDE>(p.res_out, p.res_out_f32, row * N + col, valid, v[q]);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) ss = fmaf(v[q][i], v[q][i], ss);
+  }
+  float rstd = 1.f;
+  if (!p.plain) {
+    rstd = rsqrtf(row_reduce<TPR, false>(ss, lds, 0) / (float)N + p.eps);
+    if (p.rstd && sub == 0) p.rstd[row] = rstd;
+  }
+  float amax = 0.f;
+#pragma unroll
+  for (int q = 0; q < NP; ++q) {
+    const int col = (q * TPR + sub) * VEC, valid = N - col;
+    float w[VEC], b[VEC];
+    if (p.w) load8_of<T, WIDE>(p.w, p.w_f32, col, valid, w);
+    if (p.b) load8_of<T, WIDE>(p.b, p.w_f32, col, valid, b);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      v[q][i] *= rstd;
+      if (p.w) v[q][i] *= w[i];
+      if (p.b) v[q][i] += b[i];
+      if (QUANT) amax = fmaxf(amax, __builtin_fabsf(v[q][i]));
+    }
+    if (!QUANT) store8<T, WIDE>((T*)p.y + row * N + col, v[q], valid);
+  }
+  if (QUANT) {
+    const float scale = fmaxf(row_reduce<TPR, true>(amax, lds, 1), kAmaxMin) / kE4M3Max;
+    if (sub == 0) p.scale[row] = scale;
+    const float inv = 1.f / scale;
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+      const int col = (q * TPR + sub) * VEC, valid = N - col;
+      int pk[2] = {0, 0};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        pk[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[q][4 * h] * inv, v[q][4 * h + 1] * inv, pk[h], false);
+        pk[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[q][4 * h + 2] * inv, v[q][4 * h + 3] * inv, pk[h], true);
+      }
+      uint8_t* at = (uint8_t*)p.y + row * N + col;
+      if (WIDE) {
+        if (valid > 0) *(int2*)at = int2{pk[0], pk[1]};
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (i < valid) at[i] = (uint8_t)(pk[i / 4] >> (8 * (i % 4)));
+      }
+    }
+  }
+}
+
+// Rows are walked so that the column sums of the weight gradients stay in registers and leave once per workgroup.
+template <typename T, int TPR, int NP, bool WIDE>
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_bwd_kernel(RmsParams p) {
+  constexpr int BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR;
+  __shared__ float lds[2][TPR > 64 ? TPR / 64 : 1];
+  __shared__ float sum[RPB > 1 ? RPB : 1][RPB > 1 ? TPR * VEC : 1];
+  const int sub = threadIdx.x % TPR, rl = threadIdx.x / TPR, N = p.N;
+  float dw[NP][VEC], db[NP][VEC];
+#pragma unroll
+  for (int q = 0; q < NP; ++q)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) dw[q][i] = db[q][i] = 0.f;
+  int turn = 0;
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  // every thread makes as many rounds: rows of several waves exchange through a barrier
+  for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < p.M; row0 += step, turn ^= 1) {
+    const int64_t row = row0 + rl;
+    const bool in = row < p.M;
+    float s[NP][VEC], d[NP][VEC];
+    const float rstd = in ? p.rstd[row] : 0.f;
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+      const int col = (q * TPR + sub) * VEC, valid = in ? N - col : 0;
+      load8_of<T, WIDE>(p.x, p.kept_f32, row * N + col, valid, s[q]);
+      load8_of<T, WIDE>(p.dy, 0, row * N + col, valid, d[q]);
+    }
+    float c = 0.f;
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+      const int col = (q * TPR + sub) * VEC;
+      float w[VEC];
+      if (p.w) load8_of<T, WIDE>(p.w, p.w_f32, col, N - col, w);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        s[q][i] *= rstd;
+        dw[q][i] = fmaf(d[q][i], s[q][i], dw[q][i]);
+        db[q][i] += d[q][i];
+        if (p.w) d[q][i] *= w[i];
+        c = fmaf(d[q][i], s[q][i], c);
+      }
+    }
+    c = row_reduce<TPR, false>(c, lds, turn) / (float)N;
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+      const int col = (q * TPR + sub) * VEC, valid = in ? N - col : 0;
+      float r[VEC];
+      if (p.dres) load8_of<T, WIDE>(p.dres, p.kept_f32, row * N + col, valid, r);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        d[q][i] = (d[q][i] - s[q][i] * c) * rstd;
+        if (p.dres) d[q][i] += r[i];
+      }
+      store8<T, WIDE>((T*)p.dx + row * N + col, d[q], valid);
+      if (p.dres_in) store8_of<T, WIDE>(p.dres_in, p.kept_f32, row * N + col, valid, d[q]);
+    }
+  }
+  for (int which = 0; which < 2; ++which) {
+    float* part = which ? p.db_part : p.dw_part;
+    if (!part) continue;   // uniform
+    part += (int64_t)blockIdx.x * N;
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+      const float* mine = which ? db[q] : dw[q];
+      const int col = (q * TPR + sub) * VEC;
+      if (RPB == 1) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (col + i < N) part[col + i] = mine[i];
+      } else {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sum[rl][sub * VEC + i] = mine[i];
+        __syncthreads();
+        for (int k = threadIdx.x; k < TPR * VEC; k += BLOCK) {
+          float t = 0.f;
+#pragma unroll
+          for (int r = 0; r < RPB; ++r) t += sum[r][k];
+          if (q * TPR * VEC + k < N) part[q * TPR * VEC + k] = t;
+        }
+      }
+    }
+  }
+}
+
+// (threads to a row, passes) by the row's length
+#define RMS_SHAPES(CALL)               \
+  if (N <= 64) CALL(8, 1)              \
+  else if (N <= 128) CALL(16, 1)       \
+  else if (N <= 256) CALL(32, 1)       \
+  else if (N <= 512) CALL(64, 1)       \
+  else if (N <= 1024) CALL(64, 2)      \
+  else if (N <= 2048) CALL(64, 4)      \
+  else if (N <= 4096) CALL(256, 2)     \
+  else if (N <= 8192) CALL(256, 4)     \
+  else CALL(512, 4)
+
+int rows_per_block(int64_t N) {
+  const int threads = N <= 64 ? 8 : N <= 128 ? 16 : N <= 256 ? 32 : N <= 2048 ? 64 : 256;
+  return 256 / threads;
+}
+constexpr int64_t kMaxN = 512 * 4 * VEC;
+
+template <typename T, bool WIDE, bool QUANT>
+int launch_fwd(const RmsParams& p, hipStream_t st) {
+  const int N = p.N;
+  const dim3 grid((unsigned)fla_cdiv(p.M, rows_per_block(N)));
+#define CALL(TPR, NP) hipLaunchKernelGGL((rms_fwd_kernel<T, TPR, NP, WIDE, QUANT>), grid, dim3(TPR > 256 ? TPR : 256), 0, st, p);
+  RMS_SHAPES(CALL)
+#undef CALL
+  FLA_CHECK_LAUNCH();
+  return FLA_OK;
+}
+template <typename T, bool WIDE>
+int launch_bwd(const RmsParams& p, int grid, hipStream_t st) {
+  const int N = p.N;
+#define CALL(TPR, NP) hipLaunchKernelGGL((rms_bwd_kernel<T, TPR, NP, WIDE>), dim3(grid), dim3(TPR > 256 ? TPR : 256), 0, st, p);
+  RMS_SHAPES(CALL)
+#undef CALL
+  FLA_CHECK_LAUNCH();
+  return FLA_OK;
+}
+// whether rows of N elements behind each of the pointers can be read 16 bytes at a time
+bool wide(int64_t N, std::initializer_list<const void*> ps) {
+  uintptr_t any = 0;
+  for (const void* p : ps) any |= (uintptr_t)p;
+  return any % 16 == 0 && N % VEC == 0;
+}
+bool type_ok(int t, int dtype) { return t == dtype || t == FLA_F32; }
+
+}  // namespace
+
+extern "C" int fla_rms_norm_fwd(const void* x, const void* residual, int residual_dtype, const void* weight, const void* bias,
+                                int weight_dtype, void* y, float* scale, void* residual_out, int residual_out_dtype, float* rstd,
+                                int64_t M, int64_t N, float eps, int normalise, int dtype, fla_stream_t stream) {
+  FLA_REQUIRE(x && y && M >= 0 && N > 0 && (normalise || (!weight && !bias && !rstd)), FLA_E_INVALID);
+  FLA_REQUIRE(normalise || scale, FLA_E_INVALID);
+  FLA_REQUIRE(N <= kMaxN && M <= 0x7fffffffLL, FLA_E_UNSUPPORTED);
+  FLA_REQUIRE(!residual || type_ok(residual_dtype, dtype), FLA_E_UNSUPPORTED);
+  FLA_REQUIRE(!residual_out || type_ok(residual_out_dtype, dtype), FLA_E_UNSUPPORTED);
+  FLA_REQUIRE((!weight && !bias) || type_ok(weight_dtype, dtype), FLA_E_UNSUPPORTED);
+  if (M == 0) return FLA_OK;
+  RmsParams p{};
+  p.x = x, p.res = residual, p.w = weight, p.b = bias, p.y = y, p.scale = scale, p.res_out = residual_out, p.rstd = rstd;
+  p.M = M, p.N = (int)N, p.eps = eps, p.plain = !normalise;
+  p.res_f32 = residual_dtype == FLA_F32, p.res_out_f32 = residual_out_dtype == FLA_F32, p.w_f32 = weight_dtype == FLA_F32;
+  const bool w = wide(N, {x, residual, weight, bias, y, residual_out});
+  hipStream_t st = (hipStream_t)stream;
+#define D_(E, T)                                                                                   \
+  if (dtype == E) {                                                                                \
+    if (scale) return w ? launch_fwd<T, true, true>(p, st) : launch_fwd<T, false, true>(p, st);    \
+    return w ? launch_fwd<T, true, false>(p, st) : launch_fwd<T, false, false>(p, st);             \
+  }
+  D_(FLA_BF16, bf16)
+  D_(FLA_F16, f16)
+  D_(FLA_F32, float)
+#undef D_
+  return FLA_E_UNSUPPORTED;
+}
+
+extern "C" int fla_rms_norm_workgroups(int64_t M, int64_t N) {
+  if (M <= 0 || N <= 0) return 1;
+  const int64_t g = fla_cdiv(M, rows_per_block(N));
+  return (int)(g < 1024 ? g : 1024);
+}
+
+extern "C" int fla_rms_norm_bwd(const void* dy, const void* kept, int kept_dtype, const void* weight, int weight_dtype, const float* rstd,
+                                const void* dresidual, void* dx, void* dresidual_in, float* dw_partial, float* db_partial, int64_t M,
+                                int64_t N, int dtype, fla_stream_t stream) {
+  FLA_REQUIRE(dy && kept && rstd && dx && M >= 0 && N > 0, FLA_E_INVALID);
+  FLA_REQUIRE(N <= kMaxN && M <= 0x7fffffffLL && type_ok(kept_dtype, dtype), FLA_E_UNSUPPORTED);
+  FLA_REQUIRE(!weight || type_ok(weight_dtype, dtype), FLA_E_UNSUPPORTED);
+  if (M == 0) return FLA_OK;
+  RmsParams p{};
+  p.x = kept, p.w = weight, p.rstd = (float*)rstd, p.dy = dy, p.dres = dresidual, p.dx = dx, p.dres_in = dresidual_in;
+  p.dw_part = dw_partial, p.db_part = db_partial, p.M = M, p.N = (int)N;
+  p.kept_f32 = kept_dtype == FLA_F32, p.w_f32 = weight_dtype == FLA_F32;
+  const bool w = wide(N, {dy, kept, weight, dresidual, dx, dresidual_in});
+  const int grid = fla_rms_norm_workgroups(M, N);
+  hipStream_t st = (hipStream_t)stream;
+#define D_(E, T) \
+  if (dtype == E) return w ? launch_bwd<T, true>(p, grid, st) : launch_bwd<T, false>(p, grid, st);
+  D_(FLA_BF16, bf16)
+  D_(FLA_F16, f16)
+  D_(FLA_F32, float)
+#undef D_
+  return FLA_E_UNSUPPORTED;
+}

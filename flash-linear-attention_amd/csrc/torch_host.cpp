@@ -724,6 +724,70 @@ struct HgrnNode : torch::autograd::Function<HgrnNode> {
   }
 };
 
+// ---------------------------------------------------------------------------------------------------- RMS norm
+struct RmsArgs {
+  double eps;
+  std::optional<at::ScalarType> kept_type;   // of the sum x + residual; none: nothing is added and x itself is what is normalised
+  bool quantize, normalise;
+};
+struct RmsOut {
+  Tensor y, scale, kept, rstd;
+};
+// Any shape [..., N], contiguous operands
+RmsOut rms_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& res, const RmsArgs& a, bool want_rstd) {
+  const int64_t N = x.size(-1), M = x.numel() / N;
+  RmsOut o;
+  o.y = a.quantize ? fresh(x.sizes(), x, at::kFloat8_e4m3fn) : fresh_like(x);
+  if (a.quantize) o.scale = fresh(x.sizes().slice(0, x.dim() - 1), x, at::kFloat);
+  if (a.kept_type) o.kept = fresh(x.sizes(), x, *a.kept_type);
+  if (want_rstd) o.rstd = fresh({M}, x, at::kFloat);
+  if (M == 0) return o;
+  const Tensor& any_w = w.defined() ? w : b;
+  check(fla_rms_norm_fwd(ptr(x), ptr(res), res.defined() ? dt(res) : dt(x), ptr(w), ptr(b), any_w.defined() ? dt(any_w) : dt(x), ptr(o.y),
+                         fptr(o.scale), ptr(o.kept), o.kept.defined() ? dt(o.kept) : dt(x), fptr(o.rstd), M, N, (float)a.eps, a.normalise,
+                         dt(x), stream_of(x)),
+        "fla_rms_norm_fwd");
+  return o;
+}
+
+struct RmsNode : torch::autograd::Function<RmsNode> {
+  struct Rest {
+    bool w, b, res;
+    at::ScalarType type;
+  };
+  static variable_list forward(AutogradContext* ctx, const Tensor& x_, const Maybe& w_, const Maybe& b_, const Maybe& res_, const RmsArgs& a) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const Tensor x = x_.contiguous(), w = given(w_), b = given(b_), res = res_ ? res_->contiguous() : Tensor();
+    RmsOut o = rms_forward(x, w, b, res, a, true);
+    ctx->save_for_backward({o.kept.defined() ? o.kept : x, w, b, o.rstd});
+    ctx->set_materialize_grads(false);
+    hold(ctx, Rest{w.defined(), b.defined(), res.defined(), x.scalar_type()});
+    return o.kept.defined() ? variable_list{o.y, o.kept} : variable_list{o.y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &kept = saved[0], &w = saved[1], &b = saved[2], &rstd = saved[3];
+    const Rest& r = held<Rest>(ctx);
+    c10::DeviceGuard on_device(kept.device());
+    const int64_t N = kept.size(-1), M = kept.numel() / N;
+    const Tensor dy = grads[0].defined() ? as(grads[0], r.type).contiguous() : at::zeros(kept.sizes(), kept.options().dtype(r.type));
+    const Tensor dres = grads.size() > 1 && grads[1].defined() ? as(grads[1], kept.scalar_type()).contiguous() : Tensor();
+    Tensor dx = fresh(kept.sizes(), kept, r.type);
+    Tensor dres_in = r.res && kept.scalar_type() != r.type ? fresh_like(kept) : Tensor();
+    if (M == 0)
+      return {dx, r.w ? at::zeros_like(w) : Tensor(), r.b ? at::zeros_like(b) : Tensor(), r.res ? (dres_in.defined() ? dres_in : dx) : Tensor(),
+              Tensor()};
+    const int64_t parts = fla_rms_norm_workgroups(M, N);
+    Tensor dw = r.w ? fresh({parts, N}, kept, at::kFloat) : Tensor(), db = r.b ? fresh({parts, N}, kept, at::kFloat) : Tensor();
+    check(fla_rms_norm_bwd(ptr(dy), ptr(kept), dt(kept), ptr(w), w.defined() ? dt(w) : dt(kept), fptr(rstd), ptr(dres), ptr(dx),
+                           ptr(dres_in), fptr(dw), fptr(db), M, N, dt(dx), stream_of(kept)),
+          "fla_rms_norm_bwd");
+    return {dx, r.w ? sum_partials(dw, w.sizes(), w.scalar_type()) : Tensor(), r.b ? sum_partials(db, b.sizes(), b.scalar_type()) : Tensor(),
+            r.res ? (dres_in.defined() ? dres_in : dx) : Tensor(), Tensor()};
+  }
+};
+
 // ---------------------------------------------------------------------------------------------------- Python entries
 Tensor arg_tensor(PyObject* o) {
   if (o == Py_None) return Tensor();
@@ -1115,6 +1179,63 @@ PyObject* py_hgrn(PyObject*, PyObject* const* p, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// rms_norm(x, weight | None, bias | None, residual | None, eps, prenorm, residual_in_fp32, quantize, normalise)
+//   -> y, (y, residual_out), (q, scale) or ((q, scale), residual_out)
+PyObject* py_rms_norm(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 9);
+  Tensor x = arg_tensor(p[0]), w = arg_tensor(p[1]), b = arg_tensor(p[2]), res = arg_tensor(p[3]);
+  RmsArgs a{};
+  a.eps = arg_double(p[4]);
+  const bool prenorm = arg_bool(p[5]), in_f32 = arg_bool(p[6]);
+  a.quantize = arg_bool(p[7]);
+  a.normalise = arg_bool(p[8]);
+  TORCH_CHECK_VALUE(x.defined() && x.dim() >= 1 && x.size(-1) > 0, "fla_amd rms_norm: x is [..., N], N at least 1");
+  TORCH_CHECK_TYPE(floating(x), "fla_amd rms_norm: x in bf16, fp16 or fp32, not ", x.scalar_type());
+  const int64_t N = x.size(-1);
+  for (const Tensor* t : {&w, &b}) {
+    if (!t->defined()) continue;
+    TORCH_CHECK_TYPE(t->is_floating_point(), "fla_amd rms_norm: weight and bias in a floating type");
+    TORCH_CHECK_VALUE(t->numel() == N && t->dim() == 1, "fla_amd rms_norm: weight and bias hold ", N, " values");
+  }
+  if (res.defined()) {
+    TORCH_CHECK_VALUE(res.sizes() == x.sizes(), "fla_amd rms_norm: the residual has x's shape");
+    TORCH_CHECK_TYPE(res.scalar_type() == x.scalar_type() || res.scalar_type() == at::kFloat,
+                     "fla_amd rms_norm: the residual is in x's type or in fp32");
+  }
+  TORCH_CHECK_NOT_IMPLEMENTED(N <= 16384, "fla_amd rms_norm: rows of at most 16384 elements, not ", N);
+  need_gpu({&x, &w, &b, &res});
+  const bool grad = wants_grad({&x, &w, &b, &res});
+  TORCH_CHECK(!(grad && a.quantize), "fla_amd: rows in 8 bits have no gradient; call it under torch.no_grad()");
+  c10::DeviceGuard on_device(x.device());
+  // one type for both, x's or fp32
+  auto fits = [&](const Tensor& t) { return !t.defined() || t.scalar_type() == x.scalar_type(); };
+  if (!fits(w) || !fits(b)) w = f32(w), b = f32(b);
+  if (w.defined()) w = w.contiguous();
+  if (b.defined()) b = b.contiguous();
+  if (res.defined()) a.kept_type = res.scalar_type();
+  else if (in_f32 && prenorm && x.scalar_type() != at::kFloat) a.kept_type = at::kFloat;
+  if (!prenorm && !grad) a.kept_type.reset();   // nobody asks for the sum
+  Tensor y, scale, kept;
+  if (grad) {
+    auto out = RmsNode::apply(x, maybe(w), maybe(b), maybe(res), a);
+    y = out[0];
+    if (out.size() > 1) kept = out[1];
+  } else {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    RmsOut o = rms_forward(x.contiguous(), w, b, res.defined() ? res.contiguous() : res, a, false);
+    y = o.y, scale = o.scale, kept = o.kept;
+  }
+  PyObject* first = a.quantize ? pair(y, scale) : THPVariable_Wrap(y);
+  if (!prenorm) return first;
+  PyObject* t = PyTuple_New(2);
+  if (!first || !t) throw python_error();
+  PyTuple_SET_ITEM(t, 0, first);
+  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(kept.defined() ? kept : x));
+  return t;
+  END_HANDLE_TH_ERRORS
+}
+
 #define ENTRY(name, fn) {name, (PyCFunction)(void (*)(void))fn, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {
     ENTRY("plan", py_plan),
@@ -1129,6 +1250,7 @@ PyMethodDef kMethods[] = {
     ENTRY("short_conv_step", py_conv_update<true>),
     ENTRY("norm_swish_gate", py_norm_gate),
     ENTRY("hgrn", py_hgrn),
+    ENTRY("rms_norm", py_rms_norm),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fla_host", nullptr, -1, kMethods};
 

@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define FLA_ABI_VERSION 19
+#define FLA_ABI_VERSION 20
 
 enum fla_dtype { FLA_F32 = 0, FLA_BF16 = 1, FLA_F16 = 2 };
 
@@ -825,6 +825,25 @@ int fla_hgrn_bwd(const void* x, const void* g, const float* lower_bound, const f
                  int64_t T, int64_t D, int64_t N, int64_t ldx, int64_t ldg, fla_stream_t stream);
 int fla_hgrn_step(const void* x, const void* g, const float* lower_bound, const float* h0, void* o, float* ht, int gates,
                   int x_dtype, int g_dtype, int64_t N, int64_t D, int64_t ldx, int64_t ldg, fla_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * RMS norm of rows with the residual's addition (interface of RMSNorm / rms_norm, fla/modules/layernorm.py):
+ *   s = x + residual,  y = s / sqrt(mean s^2 + eps) * weight (+ bias).
+ * x, y, dy, dx [M,N] in `dtype`, N <= 16384, any N and address (multiples of 8 and of 16 bytes take the wide loads); residual,
+ * residual_out, kept, dresidual, dresidual_in [M,N] in `dtype` or fp32; weight, bias [N] in `dtype` or fp32 (one type for both).
+ * residual, weight, bias, residual_out (receives s), rstd (fp32 [M], for the backward) may be NULL.
+ * scale (fp32 [M]) not NULL: y receives rows in 8 bits, e4m3 (finite up to 448): scale = max(max|y|, 1e-30) / 448, y / scale.
+ * normalise == 0: y = s (8-bit rows of s itself; no weight, bias or rstd).
+ * Backward: kept is what the forward normalised (x, or residual_out) in kept_dtype; dresidual, the gradient that arrived for
+ * residual_out (in kept_dtype, or NULL), is added to dx; dresidual_in (in kept_dtype, or NULL) receives a copy of dx.  dw_partial,
+ * db_partial: fp32 [fla_rms_norm_workgroups(M, N), N] or NULL, their column sums are the gradients of weight and bias. */
+int fla_rms_norm_workgroups(int64_t M, int64_t N);
+int fla_rms_norm_fwd(const void* x, const void* residual, int residual_dtype, const void* weight, const void* bias,
+                     int weight_dtype, void* y, float* scale, void* residual_out, int residual_out_dtype, float* rstd, int64_t M,
+                     int64_t N, float eps, int normalise, int dtype, fla_stream_t stream);
+int fla_rms_norm_bwd(const void* dy, const void* kept, int kept_dtype, const void* weight, int weight_dtype, const float* rstd,
+                     const void* dresidual, void* dx, void* dresidual_in, float* dw_partial, float* db_partial, int64_t M,
+                     int64_t N, int dtype, fla_stream_t stream);
 
 /* Diagnostics: C[M,N] (fp32) = A[M,Kd] * B[N,Kd]^T with bf16 operands, computed
  * with the same MFMA fragment helpers the kernels use (mode 0: 32x32x16 tiles,
