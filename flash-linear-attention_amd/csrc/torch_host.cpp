@@ -1236,6 +1236,57 @@ PyObject* py_rms_norm(PyObject*, PyObject* const* p, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// quant_linear(x, x_scale, weight, weight_scale, bias | None, residual | None, activation, bf16)
+PyObject* py_quant_linear(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 8);
+  Tensor x = arg_tensor(p[0]), sx = arg_tensor(p[1]), w = arg_tensor(p[2]), sw = arg_tensor(p[3]), bias = arg_tensor(p[4]),
+         res = arg_tensor(p[5]);
+  const long act = PyLong_AsLong(p[6]);
+  if (act == -1 && PyErr_Occurred()) throw python_error();
+  const auto type = arg_bool(p[7]) ? at::kBFloat16 : at::kHalf;
+  TORCH_CHECK_TYPE(x.defined() && w.defined() && sx.defined() && sw.defined() && x.scalar_type() == at::kFloat8_e4m3fn &&
+                       w.scalar_type() == at::kFloat8_e4m3fn && sx.scalar_type() == at::kFloat && sw.scalar_type() == at::kFloat,
+                   "fla_amd quant_linear: x and weight are pairs of rows in torch.float8_e4m3fn and their fp32 scales");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && w.size(1) == x.size(-1) && w.size(0) > 0,
+                    "fla_amd quant_linear: x is [..., K], weight [N, K]");
+  const int64_t K = x.size(-1), N = w.size(0);
+  TORCH_CHECK_VALUE(sx.sizes() == x.sizes().slice(0, x.dim() - 1) && sw.dim() == 1 && sw.size(0) == N,
+                    "fla_amd quant_linear: one scale for every row of x and of weight");
+  TORCH_CHECK_NOT_IMPLEMENTED(K > 0 && K % 16 == 0, "fla_amd quant_linear: rows of a multiple of 16 elements, not ", K);
+  if (bias.defined()) {
+    TORCH_CHECK_VALUE(bias.dim() == 1 && bias.size(0) == N, "fla_amd quant_linear: bias holds ", N, " values");
+    TORCH_CHECK_TYPE(bias.is_floating_point(), "fla_amd quant_linear: bias in a floating type");
+  }
+  auto shape = x.sizes().vec();
+  shape.back() = N;
+  if (res.defined()) {
+    TORCH_CHECK_VALUE(res.sizes() == at::IntArrayRef(shape), "fla_amd quant_linear: residual is [..., N]");
+    TORCH_CHECK_TYPE(res.scalar_type() == type || res.scalar_type() == at::kFloat,
+                     "fla_amd quant_linear: the residual is in the output's type or in fp32");
+  }
+  need_gpu({&x, &sx, &w, &sw, &bias, &res});
+  TORCH_CHECK(!wants_grad({&x, &sx, &w, &sw, &bias, &res}),
+              "fla_amd: products of 8-bit rows have no gradient; call them under torch.no_grad()");
+  c10::DeviceGuard on_device(x.device());
+  at::AutoDispatchBelowADInplaceOrView guard;
+  auto aligned = [](const Tensor& t) {
+    const Tensor c = t.contiguous();
+    return (uintptr_t)c.data_ptr() % 16 == 0 ? c : c.clone();
+  };
+  Tensor y = at::empty(shape, x.options().dtype(type));
+  if (y.numel() == 0) return THPVariable_Wrap(y);
+  x = aligned(x), w = aligned(w), sx = sx.contiguous(), sw = sw.contiguous();
+  if (bias.defined()) bias = (bias.scalar_type() == type ? bias : f32(bias)).contiguous();
+  if (res.defined()) res = res.contiguous();
+  const int64_t M = x.numel() / K;
+  check(fla_quant_linear(ptr(x), fptr(sx), ptr(w), fptr(sw), ptr(bias), bias.defined() ? dt(bias) : FLA_F32, ptr(res),
+                         res.defined() ? dt(res) : FLA_F32, ptr(y), M, N, K, (int)act, dt(y), stream_of(x)),
+        "fla_quant_linear");
+  return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
 #define ENTRY(name, fn) {name, (PyCFunction)(void (*)(void))fn, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {
     ENTRY("plan", py_plan),
@@ -1251,6 +1302,7 @@ PyMethodDef kMethods[] = {
     ENTRY("norm_swish_gate", py_norm_gate),
     ENTRY("hgrn", py_hgrn),
     ENTRY("rms_norm", py_rms_norm),
+    ENTRY("quant_linear", py_quant_linear),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fla_host", nullptr, -1, kMethods};
 

@@ -1,0 +1,64 @@
+"""Projections with operands in 8 bits, for serving: rows of ``x`` and of the weight in ``torch.float8_e4m3fn`` with a scale each, bias, activation
+and residual in the product's epilogue."""
+from __future__ import annotations
+
+from typing import Optional, Tuple, Union
+
+import torch
+import torch.nn as nn
+
+from .._native import host
+from .layernorm import quantize_rows
+
+_ACTIVATIONS = {None: 0, "silu": 1, "swish": 1, "gelu": 2, "relu": 3}
+Rows = Tuple[torch.Tensor, torch.Tensor]
+
+
+def quant_linear(x: Rows, weight: Rows, bias: Optional[torch.Tensor] = None, activation: Optional[str] = None,
+                 residual: Optional[torch.Tensor] = None, output_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``act(x @ weight.T + bias) + residual`` for ``x`` ``[..., K]`` and ``weight`` ``[N, K]``, each a pair ``(q, scale)`` as
+    :func:`quantize_rows` and :func:`rms_norm` with ``quantize=True`` return it.
+
+    ``activation``: ``None``, ``"silu"`` (``"swish"``), ``"gelu"`` (of the error function) or ``"relu"``; ``residual`` ``[..., N]`` and ``bias`` in the
+    output's type or in fp32; ``output_dtype`` bf16 or fp16 (the matrix instruction's sums of 8-bit products hold about 16 bits, fp32
+    results are refused).  ``K`` in multiples of 16.  Sums in fp32; one launch.  There is no gradient, and a call that wants one is refused."""
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"fla_amd quant_linear: unknown activation {activation!r}")
+    if output_dtype not in (torch.bfloat16, torch.float16):
+        raise NotImplementedError(f"fla_amd quant_linear: results in bf16 or fp16, not {output_dtype}")
+    return host().quant_linear(x[0], x[1], weight[0], weight[1], bias, residual, _ACTIVATIONS[activation], output_dtype is torch.bfloat16)
+
+
+class QuantLinear(nn.Module):
+    """A ``torch.nn.Linear`` for serving with its weight in 8 bits: ``forward(x, residual=None)`` takes 16-bit or fp32 rows, which it quantises first,
+    or the pair that a norm with ``quantize=True`` returned."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, activation: Optional[str] = None,
+                 output_dtype: torch.dtype = torch.bfloat16, device=None):
+        super().__init__()
+        if activation not in _ACTIVATIONS:
+            raise ValueError(f"fla_amd quant_linear: unknown activation {activation!r}")
+        self.in_features, self.out_features, self.activation, self.output_dtype = in_features, out_features, activation, output_dtype
+        self.register_buffer("weight", torch.zeros(out_features, in_features, device=device).to(torch.float8_e4m3fn))
+        self.register_buffer("weight_scale", torch.zeros(out_features, device=device))
+        self.register_buffer("bias", torch.zeros(out_features, device=device) if bias else None)
+
+    @classmethod
+    @torch.no_grad()
+    def from_linear(cls, linear: nn.Linear, activation: Optional[str] = None, output_dtype: Optional[torch.dtype] = None) -> "QuantLinear":
+        """The layer with ``linear``'s weight rounded to 8 bits, row by row, on its device."""
+        if output_dtype is None:
+            output_dtype = linear.weight.dtype if linear.weight.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
+        new = cls(linear.in_features, linear.out_features, linear.bias is not None, activation, output_dtype, linear.weight.device)
+        new.weight, new.weight_scale = quantize_rows(linear.weight)
+        if linear.bias is not None:
+            new.bias = linear.bias.detach().clone()
+        return new
+
+    def extra_repr(self) -> str:
+        return f"{self.in_features}, {self.out_features}, bias={self.bias is not None}, activation={self.activation}"
+
+    def forward(self, x: Union[torch.Tensor, Rows], residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if isinstance(x, torch.Tensor):
+            x = quantize_rows(x)
+        return quant_linear(x, (self.weight, self.weight_scale), self.bias, self.activation, residual, self.output_dtype)
