@@ -30,115 +30,143 @@ struct LinearParams {
   bool wide;             // rows of y and of the residual can be taken 16 bytes at a time
 };
 
-enum { kNone = FLA_ACT_NONE, kSilu = FLA_ACT_SILU, kGelu = FLA_ACT_GELU, kRelu = FLA_ACT_RELU };
-FLA_DEVICE float activate(float v, int act) {
-  if (act == kSilu) return v * __builtin_amdgcn_rcpf(1.f + __expf(-v));
-  if (act == kGelu) return 0.5f * v * (1.f + erff(v * 0.70710678f));
-  if (act == kRelu) return v < 0.f ? 0.f : v;      // (NaN stays)
+template <int ACT>
+FLA_DEVICE float activate(float v) {
+  if (ACT == FLA_ACT_SILU) return v * __builtin_amdgcn_rcpf(1.f + __expf(-v));
+  if (ACT == FLA_ACT_GELU) return 0.5f * v * (1.f + erff(v * 0.70710678f));
+  if (ACT == FLA_ACT_RELU) return v < 0.f ? 0.f : v;      // (NaN stays)
   return v;
 }
 
-FLA_DEVICE f32x4 mfma8(i32x8 a, i32x8 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0);   // both e4m3, no block scales
+// both e4m3, no block scales
+FLA_DEVICE f32x4 mfma8(i32x8 a, i32x8 b, f32x4 c) { return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0); }
+
+// COUNT values at any element address; unless FULL, the first `valid` of them one by one
+template <typename T, int COUNT, bool FULL>
+FLA_DEVICE void load_some(const T* p, int valid, float* o) {
+  if (FULL) {
+    typedef T vec __attribute__((ext_vector_type(COUNT), aligned(alignof(T))));
+    const vec v = *(const vec*)p;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) o[i] = (float)v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) o[i] = i < valid ? (float)p[i] : 0.f;
+  }
 }
 
-// COUNT (4, 8 or 16) consecutive n of row m from their sums
-template <typename T, int COUNT>
-FLA_DEVICE void finish(const LinearParams& p, int64_t m, int64_t n0, const float* acc) {
-  if (m >= p.M || n0 >= p.N) return;
-  const float sx = p.sx[m];
-  float v[COUNT];
-#pragma unroll
-  for (int i = 0; i < COUNT; ++i) {
-    const int64_t n = n0 + i < p.N ? n0 + i : p.N - 1;
-    float t = acc[i] * (sx * p.sw[n]);
-    if (p.bias) t += p.bias_f32 ? ((const float*)p.bias)[n] : (float)((const T*)p.bias)[n];
-    v[i] = activate(t, p.act);
-  }
-  const int64_t at = m * p.N + n0;
-  if (p.wide && n0 + COUNT <= p.N) {
-    typedef T out_t __attribute__((ext_vector_type(COUNT < 8 ? COUNT : 8)));
-    constexpr int W = COUNT < 8 ? COUNT : 8;
-#pragma unroll
-    for (int h = 0; h < COUNT; h += W) {
-      if (p.res) {
-        if (p.res_f32) {
-#pragma unroll
-          for (int i = 0; i < W; i += 4) {
-            const f32x4 r = *(const f32x4*)((const float*)p.res + at + h + i);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[h + i + j] += r[j];
-          }
-        } else {
-          const out_t r = *(const out_t*)((const T*)p.res + at + h);
-#pragma unroll
-          for (int i = 0; i < W; ++i) v[h + i] += (float)r[i];
-        }
-      }
-      out_t o;
-#pragma unroll
-      for (int i = 0; i < W; ++i) o[i] = (T)v[h + i];
-      *(out_t*)((T*)p.y + at + h) = o;
-    }
-    return;
+// COUNT (4 or 8) consecutive n of row m from their sums.  FULL: all of them exist, and they can be taken 16 bytes at a time.
+template <typename T, int COUNT, int ACT, bool FULL>
+FLA_DEVICE void finish(const LinearParams& p, int64_t m, int64_t n, const float* acc, float sx, const float* sw, const float* bias) {
+  const int valid = FULL || p.N - n > COUNT ? COUNT : (int)(p.N - n);
+  if (m >= p.M || (!FULL && valid <= 0)) return;
+  float v[COUNT], r[COUNT];
+  const int64_t at = m * p.N + n;
+  if (p.res) {
+    if (p.res_f32) load_some<float, COUNT, FULL>((const float*)p.res + at, valid, r);
+    else load_some<T, COUNT, FULL>((const T*)p.res + at, valid, r);
   }
 #pragma unroll
-  for (int i = 0; i < COUNT; ++i) {
-    if (n0 + i >= p.N) break;
-    if (p.res) v[i] += p.res_f32 ? ((const float*)p.res)[at + i] : (float)((const T*)p.res)[at + i];
-    ((T*)p.y)[at + i] = (T)v[i];
+  for (int i = 0; i < COUNT; ++i) v[i] = activate<ACT>(fmaf(acc[i], sx * sw[i], bias[i]));
+  if (p.res)
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) v[i] += r[i];
+  T* y = (T*)p.y + at;
+  if (FULL) {
+    typedef T vec __attribute__((ext_vector_type(COUNT)));
+    vec o;
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) o[i] = (T)v[i];
+    *(vec*)y = o;
+  } else {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i)
+      if (i < valid) y[i] = (T)v[i];
   }
+}
+template <typename T>
+FLA_DEVICE float bias_of(const LinearParams& p, int64_t n) {
+  return !p.bias || n >= p.N ? 0.f : p.bias_f32 ? ((const float*)p.bias)[n] : (float)((const T*)p.bias)[n];
+}
+
+// the activation as a constant: one branch a tile instead of one an element
+template <int V>
+struct Const {
+  static constexpr int value = V;
+};
+template <typename F>
+FLA_DEVICE void with_activation(int act, const F& f) {
+  if (act == FLA_ACT_SILU) f(Const<FLA_ACT_SILU>());
+  else if (act == FLA_ACT_GELU) f(Const<FLA_ACT_GELU>());
+  else if (act == FLA_ACT_RELU) f(Const<FLA_ACT_RELU>());
+  else f(Const<FLA_ACT_NONE>());
 }
 
 // ------------------------------------------------------------------------------------------------ tiles
 __device__ const i32x4 kZeros = {0, 0, 0, 0};
 
-// A BM x BN tile of y for WM x WN waves; slices of 128 bytes of K go through LDS, two of them: one is read while the next arrives
-// straight from memory (a wave's copy instruction fills 1024 bytes: eight rows of 128).  The 16-byte pieces of a row are permuted within it by
-// a key of the row, so that eight lanes that read the same piece of eight rows meet all banks.
-template <typename T, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LinearParams p) {
-  constexpr int THREADS = WM * WN * 64, WAVES = WM * WN, BK = 128;
+// A BM x BN tile of y for WM x WN waves.  Slices of 128 bytes of K go through LDS, two of them: one is read while the next arrives
+// straight from memory (a wave's copy instruction fills 1024 bytes: eight rows of 128).  The 16-byte pieces of a row are permuted within it by a key
+// of the row: a b128 read serves lanes 0-3, 12-15, 20-27 together, then 4-11, 16-19, 28-31, and the same of the upper half (found by timing
+// patterns), and with these keys each sixteen meet all 64 banks once.
+template <typename T, int BM, int BN, int WM, int WN, int PER_SIMD>
+__global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(PER_SIMD))) void linear_tile_kernel(LinearParams p) {
+  constexpr int WAVES = WM * WN, BK = 128;
   constexpr int MT = BM / WM / 16, NT = BN / WN / 16;          // 16 x 16 tiles of a wave
   constexpr int CX = BM / 8 / WAVES, CW = BN / 8 / WAVES;      // copy instructions of a wave for a slice
-  static_assert(CX >= 1 && CW >= 1 && BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "whole copies");
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2][(BM + BN) * BK];
+  static_assert(NT % 2 == 0 && CX >= 1 && CW >= 1 && BM % (8 * WAVES) == 0 && BN % (8 * WAVES) == 0, "whole copies");
+  // (One array: the compiler tells apart the members of several, and then waits for copies in flight ahead of every read.)
+  constexpr int SLICE = (BM + BN) * BK;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * SLICE + (BM + 2 * BN) * 4];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave / WN, wn = wave % WN;
+  const int wm = wave / WN, wn = wave % WN, lr = lane & 15, lq = lane >> 4;
 
   // Neighbouring workgroup numbers go to different XCDs: each XCD takes a run of tiles, eight rows of tiles deep, that share operands in its L2
-  const int64_t tm_all = (p.M + BM - 1) / BM, tn_all = (p.N + BN - 1) / BN, total = tm_all * tn_all;
-  const int64_t bid = blockIdx.x, xcd = bid % 8, per = total / 8, rest = total % 8;
-  const int64_t id = xcd * per + (xcd < rest ? xcd : rest) + bid / 8;
-  const int64_t deep = 8, band = id / (deep * tn_all), in = id % (deep * tn_all);
-  const int64_t rows_in = tm_all - band * deep < deep ? tm_all - band * deep : deep;
-  const int64_t m0 = (band * deep + in % rows_in) * BM, n0 = in / rows_in * BN;
+  const uint32_t tm_all = (uint32_t)((p.M + BM - 1) / BM), tn_all = (uint32_t)((p.N + BN - 1) / BN), total = tm_all * tn_all;
+  const uint32_t xcd = blockIdx.x % 8, per = total / 8, rest = total % 8;
+  const uint32_t id = xcd * per + (xcd < rest ? xcd : rest) + blockIdx.x / 8;
+  const uint32_t deep = tm_all < 8 ? tm_all : 8, band = id / (deep * tn_all), in = id - band * deep * tn_all;
+  const uint32_t rows_in = tm_all - band * deep < deep ? tm_all - band * deep : deep, col = in / rows_in;
+  const int64_t m0 = (int64_t)(band * deep + in - col * rows_in) * BM, n0 = (int64_t)col * BN;
+
+  // slices of K for this workgroup
+  const int per_split = (int)((p.K + BK - 1) / BK + p.splits - 1) / p.splits * BK;
+  const int k_first = blockIdx.y * per_split, k_end = p.K - k_first < per_split ? (int)p.K : k_first + per_split;
+
+  // what the epilogue multiplies and adds, out of memory's latency by then
+  float *sxs = (float*)(lds + 2 * SLICE), *sws = sxs + BM, *bs = sws + BN;
+  for (int i = tid; i < BM; i += WAVES * 64) sxs[i] = m0 + i < p.M ? p.sx[m0 + i] : 0.f;
+  for (int i = tid; i < BN; i += WAVES * 64) {
+    sws[i] = n0 + i < p.N ? p.sw[n0 + i] : 0.f;
+    bs[i] = bias_of<T>(p, n0 + i);
+  }
 
   // what this lane copies: piece `lane % 8` of LDS row r holds piece (lane % 8) ^ key(r) of the matrix row
-  const uint8_t* src[CX + CW];
-  int piece[CX + CW];
+  auto w_key = [](int r) { return (r & 3) | (r >> 3 & 1) << 2; };
+  const uint8_t *xb = p.x + m0 * p.K, *wb = p.w + n0 * p.K;
+  const int K = (int)p.K, rows_m = p.M - m0 < BM ? (int)(p.M - m0) : BM, rows_n = p.N - n0 < BN ? (int)(p.N - n0) : BN;
+  uint32_t at[CX + CW];
 #pragma unroll
   for (int q = 0; q < CX; ++q) {
     const int r = (wave * CX + q) * 8 + lane / 8;
-    const int64_t m = m0 + r < p.M ? m0 + r : p.M - 1;
-    piece[q] = ((lane & 7) ^ (r & 7)) * 16;
-    src[q] = p.x + m * p.K;
+    at[q] = (uint32_t)(r < rows_m ? r : rows_m - 1) * K + ((lane & 7) ^ (r & 7)) * 16;
   }
 #pragma unroll
   for (int q = 0; q < CW; ++q) {
     const int r = (wave * CW + q) * 8 + lane / 8;
-    const int64_t n = n0 + r < p.N ? n0 + r : p.N - 1;
-    piece[CX + q] = ((lane & 7) ^ ((r & 3) | (r / (4 * NT) & 1) << 2)) * 16;
-    src[CX + q] = p.w + n * p.K;
+    at[CX + q] = (uint32_t)(r < rows_n ? r : rows_n - 1) * K + ((lane & 7) ^ w_key(r)) * 16;
   }
-  auto copy = [&](int64_t k0, int buf) {
+  auto copy = [&](int k0, int buf) {
 #pragma unroll
     for (int q = 0; q < CX + CW; ++q) {
-      const int64_t k = k0 + piece[q];
-      const uint8_t* from = k < p.K ? src[q] + k : (const uint8_t*)&kZeros;
       const int row = q < CX ? (wave * CX + q) * 8 : BM + (wave * CW + q - CX) * 8;
+      const uint8_t* from = (q < CX ? xb : wb) + k0 + at[q];
+      if (k0 + BK > K) {   // (uniform) beyond the end of K, in multiples of 16: zeros
+        const int piece = ((lane & 7) ^ (q < CX ? row + lane / 8 & 7 : w_key(row - BM + lane / 8))) * 16;
+        if (k0 + piece >= K) from = (const uint8_t*)&kZeros;
+      }
       __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                       (__attribute__((address_space(3))) void*)&lds[buf][row * BK], 16, 0, 0);
+                                       (__attribute__((address_space(3))) void*)(lds + buf * SLICE + row * BK), 16, 0, 0);
     }
   };
 
@@ -147,44 +175,91 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_tile_kernel(LinearParams 
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  const int lr = lane & 15, lq = lane >> 4;
+  // 32 bytes of a row's slice: pieces lq and lq + 4
   auto fragment = [&](const uint8_t* base, int row, int key) {
     const uint8_t* r = base + row * BK;
-    const i32x4 a = *(const i32x4*)(r + ((2 * lq) ^ key) * 16), b = *(const i32x4*)(r + ((2 * lq + 1) ^ key) * 16);
+    const i32x4 a = *(const i32x4*)(r + (lq ^ key) * 16), b = *(const i32x4*)(r + ((lq + 4) ^ key) * 16);
     return i32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   };
-  copy(0, 0);
+  copy(k_first, 0);
   int buf = 0;
-  for (int64_t k0 = 0; k0 < p.K; k0 += BK, buf ^= 1) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // this wave's part of the slice has arrived
-    __builtin_amdgcn_s_barrier();                      // everybody's has, and the other buffer is no longer read
-    if (k0 + BK < p.K) copy(k0 + BK, buf ^ 1);
-    const uint8_t *xs = lds[buf], *ws = lds[buf] + BM * BK;
-    i32x8 wf[NT];
+  for (int k0 = k_first; k0 < k_end; k0 += BK, buf ^= 1) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // this wave's part of the slice has arrived
+    __builtin_amdgcn_s_barrier();                                 // everybody's has, and the other buffer is no longer read
+    if (k0 + BK < k_end) copy(k0 + BK, buf ^ 1);
+    const uint8_t *xs = lds + buf * SLICE, *ws = xs + BM * BK;
+    i32x8 wf[NT], xf[MT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      // lane row lr of tile j is row 4 NT (lr / 4) + 4 j + lr % 4 of the wave's: a lane's sums over all j are 4 NT consecutive n
-      const int r = wn * NT * 16 + (lr >> 2) * 4 * NT + 4 * j + (lr & 3);
-      wf[j] = fragment(ws, r, (r & 3) | (r / (4 * NT) & 1) << 2);
+      // Lane row lr of tile j is row 32 (j / 2) + 8 (lr / 4) + 4 (j % 2) + lr % 4 of the wave's: a lane's sums of two tiles are eight
+      // consecutive n, and those of the four lanes of a row 32.
+      const int r = wn * NT * 16 + (j >> 1) * 32 + (lr >> 2) * 8 + (j & 1) * 4 + (lr & 3);
+      wf[j] = fragment(ws, r, w_key(r));
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const int r = (wm * MT + i) * 16 + lr;
-      const i32x8 xf = fragment(xs, r, r & 7);
+      xf[i] = fragment(xs, r, r & 7);
+    }
 #pragma unroll
-      for (int j = 0; j < NT; ++j) acc[i][j] = mfma8(wf[j], xf, acc[i][j]);
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j] = mfma8(wf[j], xf[i], acc[i][j]);
+    // a row of products while the next one's operand is read
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * NT + 2, 0);
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      if (i + 1 < MT) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, NT, 0);
     }
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no copy into LDS outlives the workgroup
+  const int lm = wm * MT * 16 + lr, ln = wn * NT * 16 + lq * 8;
+  if (p.splits > 1) {   // linear_finish_kernel adds the slices' sums
+    float* part = p.part + blockIdx.y * p.M * p.N;
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    float v[4 * NT];
+    for (int h = 0; h < NT / 2; ++h)
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+      for (int i = 0; i < MT; ++i) {
+        const int64_t m = m0 + lm + i * 16, n = n0 + ln + h * 32;
+        if (m >= p.M) continue;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[4 * j + r] = acc[i][j][r];
-    finish<T, 4 * NT>(p, m0 + (wm * MT + i) * 16 + lr, n0 + wn * NT * 16 + lq * 4 * NT, v);
+        for (int q = 0; q < 2; ++q) {
+          float* to = part + m * p.N + n + 4 * q;
+          const f32x4 v = acc[i][2 * h + q];
+          if (n + 4 * q + 4 <= p.N) {
+            *(f32x4_any*)to = v;
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (n + 4 * q + r < p.N) to[r] = v[r];
+          }
+        }
+      }
+    return;
   }
+  auto epilogue = [&](auto act, auto full) {
+    float sx[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sx[i] = sxs[lm + i * 16];
+#pragma unroll
+    for (int h = 0; h < NT / 2; ++h) {
+      float sw[8], bias[8];
+      load_some<float, 8, true>(sws + ln + h * 32, 8, sw);
+      load_some<float, 8, true>(bs + ln + h * 32, 8, bias);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        float v[8];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = acc[i][2 * h][r], v[4 + r] = acc[i][2 * h + 1][r];
+        finish<T, 8, decltype(act)::value, decltype(full)::value>(p, m0 + lm + i * 16, n0 + ln + h * 32, v, sx[i], sw, bias);
+      }
+    }
+  };
+  with_activation(p.act, [&](auto act) {
+    if (p.wide && n0 + BN <= p.N) epilogue(act, Const<true>());
+    else epilogue(act, Const<false>());
+  });
 }
 
 // ------------------------------------------------------------------------------------------------ few rows
@@ -196,25 +271,33 @@ __global__ __launch_bounds__(WAVES * 64) void linear_rows_kernel(LinearParams p)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lq = lane >> 4;
   const int64_t n0 = (int64_t)blockIdx.x * 16;
   const int64_t n = n0 + lr < p.N ? n0 + lr : p.N - 1;
-  const uint8_t* wr = p.w + n * p.K + lq * 32;
+  const uint8_t* wr = p.w + n * p.K + lq * 16;
   const uint8_t* xr[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const int64_t m = i * 16 + lr < p.M ? i * 16 + lr : p.M - 1;
-    xr[i] = p.x + m * p.K + lq * 32;
+    xr[i] = p.x + m * p.K + lq * 16;
   }
+  float sw[4], bias[4], sx[MT];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t c = n0 + lq * 4 + i;
+    sw[i] = c < p.N ? p.sw[c] : 0.f;
+    bias[i] = bias_of<T>(p, c);
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) sx[i] = i * 16 + lr < p.M ? p.sx[i * 16 + lr] : 0.f;
   f32x4 acc[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int64_t slices = (p.K + 127) / 128, per = (slices + p.splits - 1) / p.splits;
-  const int64_t first = blockIdx.y * per, end = first + per < slices ? first + per : slices;
+  const int64_t slices = (p.K + 127) / 128;
   auto load = [&](const uint8_t* r, int64_t k) {
-    // K in multiples of 16: a lane's 32 bytes end in the middle at most
+    // K in multiples of 16
     const i32x4 zero = {0, 0, 0, 0};
-    const i32x4 a = k + lq * 32 < p.K ? *(const i32x4*)(r + k) : zero, b = k + lq * 32 + 16 < p.K ? *(const i32x4*)(r + k + 16) : zero;
+    const i32x4 a = k + lq * 16 < p.K ? *(const i32x4*)(r + k) : zero, b = k + lq * 16 + 64 < p.K ? *(const i32x4*)(r + k + 64) : zero;
     return i32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   };
-  for (int64_t s = first + wave; s < end; s += WAVES) {
+  for (int64_t s = wave; s < slices; s += WAVES) {
     const i32x8 wf = load(wr, s * 128);
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[i] = mfma8(wf, load(xr[i], s * 128), acc[i]);
@@ -222,59 +305,141 @@ __global__ __launch_bounds__(WAVES * 64) void linear_rows_kernel(LinearParams p)
 #pragma unroll
   for (int i = 0; i < MT; ++i) sums[wave][i][lane] = acc[i];
   __syncthreads();
-  for (int i = wave; i < MT; i += WAVES) {
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    if (i % WAVES != wave) continue;
     f32x4 t = sums[0][i][lane];
 #pragma unroll
     for (int w = 1; w < WAVES; ++w) t += sums[w][i][lane];
     const float v[4] = {t[0], t[1], t[2], t[3]};
-    finish<T, 4>(p, i * 16 + lr, n0 + lq * 4, v);
+    with_activation(p.act, [&](auto act) {
+      constexpr int A = decltype(act)::value;
+      if (p.wide && n0 + 16 <= p.N) finish<T, 4, A, true>(p, i * 16 + lr, n0 + lq * 4, v, sx[i], sw, bias);
+      else finish<T, 4, A, false>(p, i * 16 + lr, n0 + lq * 4, v, sx[i], sw, bias);
+    });
   }
 }
 
-template <typename T, int BM, int BN, int WM, int WN>
+// y from the sums of slices of K, added in their order: four columns a thread
+template <typename T>
+__global__ __launch_bounds__(256) void linear_finish_kernel(LinearParams p) {
+  const int64_t per = (p.N + 3) / 4, id = (int64_t)blockIdx.x * 256 + threadIdx.x, m = id / per, n = id % per * 4;
+  if (m >= p.M) return;
+  const int valid = p.N - n < 4 ? (int)(p.N - n) : 4;
+  float v[4] = {0.f, 0.f, 0.f, 0.f}, sw[4], bias[4];
+  for (int s = 0; s < p.splits; ++s) {
+    const float* from = p.part + (s * p.M + m) * p.N + n;
+    float t[4];
+    if (valid == 4) load_some<float, 4, true>(from, 4, t);
+    else load_some<float, 4, false>(from, valid, t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] += t[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    sw[i] = i < valid ? p.sw[n + i] : 0.f;
+    bias[i] = bias_of<T>(p, n + i);
+  }
+  const float sx = p.sx[m];
+  with_activation(p.act, [&](auto act) {
+    if (p.wide) finish<T, 4, decltype(act)::value, true>(p, m, n, v, sx, sw, bias);
+    else finish<T, 4, decltype(act)::value, false>(p, m, n, v, sx, sw, bias);
+  });
+}
+
+template <typename T, int BM, int BN, int WM, int WN, int PER_SIMD>
 int launch_tiles(const LinearParams& p, hipStream_t st) {
   const int64_t total = fla_cdiv(p.M, BM) * fla_cdiv(p.N, BN);
   FLA_REQUIRE(total <= 0x7fffffff, FLA_E_UNSUPPORTED);
-  hipLaunchKernelGGL((linear_tile_kernel<T, BM, BN, WM, WN>), dim3((unsigned)total), dim3(WM * WN * 64), 0, st, p);
+  hipLaunchKernelGGL((linear_tile_kernel<T, BM, BN, WM, WN, PER_SIMD>), dim3((unsigned)total, p.splits), dim3(WM * WN * 64), 0, st, p);
   FLA_CHECK_LAUNCH();
+  if (p.splits > 1) {
+    hipLaunchKernelGGL((linear_finish_kernel<T>), dim3((unsigned)fla_cdiv(p.M * fla_cdiv(p.N, 4), 256)), dim3(256), 0, st, p);
+    FLA_CHECK_LAUNCH();
+  }
   return FLA_OK;
 }
 template <typename T, int MT>
 int launch_rows(const LinearParams& p, hipStream_t st) {
-  hipLaunchKernelGGL((linear_rows_kernel<T, MT, 8>), dim3((unsigned)fla_cdiv(p.N, 16), 1), dim3(512), 0, st, p);
+  hipLaunchKernelGGL((linear_rows_kernel<T, MT, 8>), dim3((unsigned)fla_cdiv(p.N, 16)), dim3(512), 0, st, p);
   FLA_CHECK_LAUNCH();
   return FLA_OK;
 }
+// Which kernel, and how many slices of K: by an estimate in us of each.  Measured (us; M x N x K):
+//                     rows   64 x 64 in 1, 2, 4, 8 slices    128 x 64   128 x 128   256 x 256
+//   16 x 2048 x 8192    9.6  24.4  16.6  12.0  10.8             32.9
+//   48 x 2048 x 8192   16.5  24.5  16.9  12.5  11.6             33.2
+//   48 x 8192 x 2048    9.8   8.5   8.9   9.3  10.8             11.2
+//   48 x 2048 x 2048    6.0   8.5   8.7   8.6   9.5             10.9
+//   32 x 4096 x 4096    8.0  13.9  11.6  10.1  11.0             18.3
+//   64 x 16384 x 8192  73.5  37.2  28.9  29.5  34.6             42.1
+//   100 x 2048 x 8192        24.6  17.5  13.5  14.1             33.4
+//   256 x 4096 x 4096        14.7  19.6  20.9  25.4             19.1        24        51
+//   1000 x 4096 x 4096       28.7  44.0                         25.9        29.7      57
+//   8191 x 8192 x 2048      226.8                              176.3       168.9     161.6
+enum LinearKind { kRows, kTile64, kTile128x64, kTile256 };
+struct LinearPlan {
+  LinearKind kind;
+  int splits;
+};
+LinearPlan plan_linear(int64_t M, int64_t N, int64_t K) {
+  // tiles of 256 x 256 need the fewest bytes, tiles of 128 x 64 a quarter of the rows and columns to fill the chip
+  if (fla_cdiv(M, 256) * fla_cdiv(N, 256) >= 192) return {kTile256, 1};
+  if (fla_cdiv(M, 128) * fla_cdiv(N, 64) >= 256) return {kTile128x64, 1};
+  const int64_t tiles = fla_cdiv(M, 64) * fla_cdiv(N, 64), slices = fla_cdiv(K, 128);
+  LinearPlan best{kTile64, 1};
+  double time = 0;
+  for (int splits = 1; splits <= 16; splits *= 2) {
+    if (splits > 1 && (tiles * splits > 1024 || slices < 4 * splits)) break;
+    // a slice takes 0.37 us; the second launch 4 us, and its sums go out and in
+    const double t = 2.5 + 0.37 * (double)fla_cdiv(slices, splits) + (splits > 1 ? 4 + 8e-6 / 4 * splits * (double)(M * N) : 0);
+    if (splits == 1 || t < time) best.splits = splits, time = t;
+  }
+  best.splits = (int)fla_cdiv(slices, fla_cdiv(slices, best.splits));   // none of them empty
+  // a workgroup reads 16 rows of w and all of x, 38 bytes a ns
+  if (M <= 64 && 3 + (double)fla_cdiv(fla_cdiv(N, 16), 256) * (double)((16 + M) * K) / 38000 < time) return {kRows, 1};
+  return best;
+}
+
 template <typename T>
-int launch_linear(const LinearParams& p, hipStream_t st) {
+int launch_linear(const LinearParams& p, LinearKind kind, hipStream_t st) {
+  switch (kind) {
+    case kTile256: return launch_tiles<T, 256, 256, 2, 4, 2>(p, st);
+    case kTile128x64: return launch_tiles<T, 128, 64, 2, 2, 3>(p, st);
+    case kTile64: return launch_tiles<T, 64, 64, 2, 2, 4>(p, st);
+    default: break;
+  }
   if (p.M <= 16) return launch_rows<T, 1>(p, st);
   if (p.M <= 32) return launch_rows<T, 2>(p, st);
   if (p.M <= 48) return launch_rows<T, 3>(p, st);
-  if (p.M <= 64) return launch_rows<T, 4>(p, st);
-  const int64_t big = fla_cdiv(p.M, 256) * fla_cdiv(p.N, 256), mid = fla_cdiv(p.M, 128) * fla_cdiv(p.N, 128);
-  if (big >= 192) return launch_tiles<T, 256, 256, 2, 4>(p, st);
-  if (mid >= 128) return launch_tiles<T, 128, 128, 2, 2>(p, st);
-  return launch_tiles<T, 64, 64, 2, 2>(p, st);
+  return launch_rows<T, 4>(p, st);
 }
 
 }  // namespace
 
+extern "C" int fla_quant_linear_splits(int64_t M, int64_t N, int64_t K) {
+  return M <= 0 || N <= 0 || K <= 0 ? 1 : plan_linear(M, N, K).splits;
+}
+
 extern "C" int fla_quant_linear(const void* x, const float* x_scale, const void* weight, const float* weight_scale, const void* bias,
                                 int bias_dtype, const void* residual, int residual_dtype, void* y, int64_t M, int64_t N, int64_t K,
-                                int activation, int dtype, fla_stream_t stream) {
+                                int activation, int dtype, float* workspace, fla_stream_t stream) {
   FLA_REQUIRE(x && x_scale && weight && weight_scale && y && M >= 0 && N > 0 && K > 0, FLA_E_INVALID);
   FLA_REQUIRE(activation >= FLA_ACT_NONE && activation <= FLA_ACT_RELU, FLA_E_INVALID);
   FLA_REQUIRE(dtype == FLA_BF16 || dtype == FLA_F16, FLA_E_UNSUPPORTED);
   FLA_REQUIRE(!bias || bias_dtype == dtype || bias_dtype == FLA_F32, FLA_E_UNSUPPORTED);
   FLA_REQUIRE(!residual || residual_dtype == dtype || residual_dtype == FLA_F32, FLA_E_UNSUPPORTED);
-  FLA_REQUIRE(K % 16 == 0 && N <= 0x7fffffff && M <= 0x7fffffff, FLA_E_UNSUPPORTED);
+  FLA_REQUIRE(K % 16 == 0 && K <= 1 << 23 && N <= 0x7fffffff && M <= 0x7fffffff, FLA_E_UNSUPPORTED);
   FLA_REQUIRE((((uintptr_t)x) | ((uintptr_t)weight)) % 16 == 0, FLA_E_ALIGNMENT);
   if (M == 0) return FLA_OK;
   LinearParams p{};
   p.x = (const uint8_t*)x, p.sx = x_scale, p.w = (const uint8_t*)weight, p.sw = weight_scale, p.bias = bias, p.res = residual, p.y = y;
-  p.M = M, p.N = N, p.K = K, p.act = activation, p.splits = 1;
+  p.M = M, p.N = N, p.K = K, p.act = activation;
+  const LinearPlan plan = plan_linear(M, N, K);
+  FLA_REQUIRE(plan.splits == 1 || workspace, FLA_E_INVALID);
+  p.splits = plan.splits, p.part = workspace;
   p.bias_f32 = bias_dtype == FLA_F32, p.res_f32 = residual_dtype == FLA_F32;
   p.wide = N % 8 == 0 && (((uintptr_t)residual) | ((uintptr_t)y)) % 16 == 0;
   hipStream_t st = (hipStream_t)stream;
-  return dtype == FLA_BF16 ? launch_linear<bf16>(p, st) : launch_linear<f16>(p, st);
+  return dtype == FLA_BF16 ? launch_linear<bf16>(p, plan.kind, st) : launch_linear<f16>(p, plan.kind, st);
 }

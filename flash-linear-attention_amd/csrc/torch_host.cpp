@@ -1280,8 +1280,10 @@ PyObject* py_quant_linear(PyObject*, PyObject* const* p, Py_ssize_t n) {
   if (bias.defined()) bias = (bias.scalar_type() == type ? bias : f32(bias)).contiguous();
   if (res.defined()) res = res.contiguous();
   const int64_t M = x.numel() / K;
+  const int splits = fla_quant_linear_splits(M, N, K);
+  const Tensor sums = splits > 1 ? fresh({splits, M, N}, x, at::kFloat) : Tensor();
   check(fla_quant_linear(ptr(x), fptr(sx), ptr(w), fptr(sw), ptr(bias), bias.defined() ? dt(bias) : FLA_F32, ptr(res),
-                         res.defined() ? dt(res) : FLA_F32, ptr(y), M, N, K, (int)act, dt(y), stream_of(x)),
+                         res.defined() ? dt(res) : FLA_F32, ptr(y), M, N, K, (int)act, dt(y), fptr(sums), stream_of(x)),
         "fla_quant_linear");
   return THPVariable_Wrap(y);
   END_HANDLE_TH_ERRORS

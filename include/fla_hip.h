@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define FLA_ABI_VERSION 21
+#define FLA_ABI_VERSION 22
 
 enum fla_dtype { FLA_F32 = 0, FLA_BF16 = 1, FLA_F16 = 2 };
 
@@ -850,11 +850,13 @@ int fla_rms_norm_bwd(const void* dy, const void* kept, int kept_dtype, const voi
  * torch.nn.Linear and whose 8-bit rows, fla/modules/fused_bitlinear.py, are multiplied in 16 bits):
  *   y[m,n] = act(x_scale[m] weight_scale[n] sum_k x[m,k] weight[n,k] + bias[n]) + residual[m,n].
  * x [M,K], weight [N,K] e4m3, K % 16 == 0, 16-byte addresses; scales fp32; y in `dtype`, bf16 or fp16; bias [N] and residual
- * [M,N] in `dtype` or fp32, or NULL.  gelu is the one of the error function. */
+ * [M,N] in `dtype` or fp32, or NULL.  gelu is the one of the error function.  A product of few tiles and a long K is summed in slices of
+ * K: fla_quant_linear_splits gives their number, and where it is more than one `workspace` is fp32 [splits, M, N]. */
 enum fla_activation { FLA_ACT_NONE = 0, FLA_ACT_SILU = 1, FLA_ACT_GELU = 2, FLA_ACT_RELU = 3 };
+int fla_quant_linear_splits(int64_t M, int64_t N, int64_t K);
 int fla_quant_linear(const void* x, const float* x_scale, const void* weight, const float* weight_scale, const void* bias,
                      int bias_dtype, const void* residual, int residual_dtype, void* y, int64_t M, int64_t N, int64_t K,
-                     int activation, int dtype, fla_stream_t stream);
+                     int activation, int dtype, float* workspace, fla_stream_t stream);
 
 /* Diagnostics: C[M,N] (fp32) = A[M,Kd] * B[N,Kd]^T with bf16 operands, computed
  * with the same MFMA fragment helpers the kernels use (mode 0: 32x32x16 tiles,

@@ -61,7 +61,8 @@ CASES = [  # M, N, K, type, bias, activation, residual
     (16, 64, 128, HF, None, "relu", HF), (17, 72, 272, BF, BF, None, BF), (33, 48, 1040, BF, FL, "silu", FL), (48, 200, 4096, HF, HF, None, HF),
     (64, 17, 240, BF, BF, "gelu", BF), (65, 64, 128, BF, None, None, None), (65, 70, 144, HF, HF, "silu", FL), (100, 129, 656, BF, BF, None, BF),
     (250, 1000, 528, BF, BF, "gelu", BF), (1400, 1411, 272, HF, FL, "relu", HF), (3500, 4000, 384, BF, BF, "silu", BF), (3601, 3333, 208, HF, None, None, FL),
-    (130, 65, 16, BF, None, None, None), (2000, 2040, 128, BF, BF, None, None),
+    (130, 65, 16, BF, None, None, None), (70, 130, 4112, BF, BF, "silu", FL), (60, 258, 6400, HF, None, "gelu", HF), (300, 2050, 400, BF, FL, None, BF),
+    (2000, 2040, 128, BF, BF, None, None),
 ]
 
 

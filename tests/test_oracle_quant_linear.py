@@ -49,7 +49,11 @@ def test_library_arguments():
     lib = be.lib()
     buf = torch.zeros(64)
     p, odd = ctypes.c_void_p(buf.data_ptr()), ctypes.c_void_p(buf.data_ptr() + 4)
-    call = lambda x=p, K=16, act=0, dtype=1, res=None, rt=0, N=4: lib.fla_quant_linear(x, p, p, p, None, 0, res, rt, p, 1, N, K, act, dtype, None)
+    call = lambda x=p, K=16, act=0, dtype=1, res=None, rt=0, N=4: lib.fla_quant_linear(x, p, p, p, None, 0, res, rt, p, 1, N, K, act, dtype, None, None)
     assert call(x=None) == -1 and call(K=0) == -1 and call(act=4) == -1 and call(N=0) == -1
     assert call(K=24) == -2 and call(dtype=0) == -2 and call(res=p, rt=2) == -2
     assert call(x=odd) == -3
+    # few tiles and a long K: in slices, which need a workspace; single rows and large products are not cut
+    splits = lib.fla_quant_linear_splits
+    assert splits(48, 2048, 8192) > 1 and splits(1, 4096, 2048) == 1 and splits(8191, 8192, 2048) == 1 and splits(0, 1, 1) == 1
+    assert lib.fla_quant_linear(p, p, p, p, None, 0, None, 0, p, 48, 2048, 8192, 0, 1, None, None) == -1
