@@ -10,43 +10,40 @@
 namespace {
 
 // OUT: writes the gradients; otherwise the map of the segment.
-template <typename T, typename GT, bool GATES, bool WIDE, bool OUT>
+template <typename T, typename GT, int GATES, bool WIDE, bool OUT>
 __global__ __launch_bounds__(kWaves * 64) void hgrn_bwd_kernel(HgrnParams p) {
+  constexpr int R = 2, kSpan = kGroups * R, kTile = kWaves * kSpan;   // rows of a lane, a wave, the workgroup
   __shared__ __attribute__((aligned(16))) TileShare sh;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 3;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = lane >> 3;
   const int cb = blockIdx.x % p.ncb, D = p.D;
   bool exists;
   const Segment s = find_segment(p, blockIdx.x / p.ncb, &exists);
   if (!exists) return;
+  if (!OUT && s.c == 0) return;               // nothing is ahead of the first segment of a sequence
   const int ch = cb * kCh + lane;
   const int col = cb * kCh + (lane & 7) * VEC, valid = D - col;
-  if (!OUT && s.c == 0) return;               // nothing is ahead of the first segment of a sequence
-  float lb[VEC], dlb[VEC];
+  const bool whole_block = cb * kCh + kCh <= D;
+  if (GATES == kBoundedGates) keep_bounds(sh, p.lb, cb * kCh, D);
+  float dlb[VEC];
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    lb[i] = GATES && p.lb && i < valid ? p.lb[col + i] : 0.f;
-    dlb[i] = 0.f;
-  }
+  for (int i = 0; i < VEC; ++i) dlb[i] = 0.f;
 
-  constexpr int kRows = kBwdRows, kSpan = kGroups * kRows, kTile = kWaves * kSpan;
-  typename Row8<T>::raw nx[kRows], nd[kRows];
-  typename Row8<GT>::raw ng[kRows];
-  float nh[VEC];
+  const int64_t row0 = s.begin + wave * kSpan;
+  const T* xr = (const T*)p.x + row0 * p.ldx + cb * kCh;
+  const GT* gr = (const GT*)p.g + row0 * p.ldg + cb * kCh;
+  const int64_t out0 = row0 * D + cb * kCh;
+  const uint32_t ax = lane_at<R>(lane, p.ldx), ag = lane_at<R>(lane, p.ldg), ao = lane_at<R>(lane, D);
+  const float* st0 = p.states + (state_slot(s) + s.c * p.segment / kSpan + wave) * D + col;
+  const int64_t left = s.len - wave * kSpan;
+  typename Row8<T>::raw nx[R], nd[R];
+  typename Row8<GT>::raw ng[R];
+  typename Row8<float>::raw nh;
   auto fetch = [&](int64_t t0) {
-    const int64_t w0 = t0 + wave * kSpan;
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      const int64_t t = w0 + group * kRows + r, row = s.begin + t;
-      const int v = t >= 0 && t < s.len ? valid : 0;
-      if (OUT) nx[r] = load_raw8<T, WIDE>((const T*)p.x + row * p.ldx + col, v);
-      ng[r] = load_raw8<GT, WIDE>((const GT*)p.g + row * p.ldg + col, v);
-      nd[r] = load_raw8<T, WIDE>((const T*)p.dout + row * D + col, p.dout ? v : 0);
-    }
-    if (OUT) {
-      const bool v = t0 >= 0 && w0 < s.len;
-      const float* st = p.states + (state_slot(s) + (s.c * p.segment + w0) / kKept) * D + col;
-      Row8<float>::unpack(load_raw8<float, WIDE>(st, v ? valid : 0), nh);
-    }
+    const int n = t0 < 0 ? 0 : (int)(left - t0 < kSpan ? left - t0 : kSpan);
+    if (OUT) fetch_rows<T, WIDE>(nx, xr + t0 * p.ldx, p.ldx, ax, n, group, valid, whole_block, 0.f);
+    fetch_rows<GT, WIDE>(ng, gr + t0 * p.ldg, p.ldg, ag, n, group, valid, whole_block, GATES ? __builtin_inff() : 0.f);
+    fetch_rows<T, WIDE>(nd, (const T*)p.dout + out0 + t0 * D, D, ao, p.dout ? n : 0, group, valid, whole_block, 0.f);
+    if (OUT) nh = load_raw8<float, WIDE>(st0 + t0 / kSpan * D, n > 0 ? valid : 0);
   };
   const int64_t last = s.len > 0 ? (s.len - 1) / kTile * kTile : -1;
   fetch(last);
@@ -54,111 +51,91 @@ __global__ __launch_bounds__(kWaves * 64) void hgrn_bwd_kernel(HgrnParams p) {
   if (OUT && ch < D) {
     if (p.dht) carry = p.dht[s.n * D + ch];
     const float* m = p.maps + s.first * 2 * D + ch;
-#pragma unroll 8
+#pragma unroll 4
     for (int64_t k = s.count - 1; k > s.c; --k) carry = onto(m[2 * k * D], m[(2 * k + 1) * D], carry);
   }
   int buf = 0;
   for (int64_t t0 = last; t0 >= 0; t0 -= kTile, buf ^= 1) {
-    float a[kRows][VEC], d[kRows][VEC], before[kRows][VEC], hs[VEC];
-    typename Row8<T>::raw rx[kRows];
-    typename Row8<GT>::raw rg[kRows];
+    // Held for the second half: x itself, sigmoid(x), both sides of the forget gate's sigmoid (or the decay), do and the state ahead
+    float x[R][VEC], si[R][VEC], sf[R][VEC], rest[R][VEC], d[R][VEC], before[R][VEC];
+    float A[VEC], M[VEC], hs[VEC];
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      rx[r] = nx[r];
-      rg[r] = ng[r];
+    for (int r = 0; r < R; ++r) {
+      if (OUT) Row8<T>::unpack(nx[r], x[r]);
+      Row8<GT>::unpack(ng[r], sf[r]);
       Row8<T>::unpack(nd[r], d[r]);
     }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) hs[i] = nh[i];
+    if (OUT) Row8<float>::unpack(nh, hs);
     fetch(t0 - kTile);
-
-    float A[VEC], M[VEC];
-    {
-      // the lane's rows as a map of the state (H) and, from the right, of the gradient (M); before: u until the states are known
-      float H[VEC];
+    float lb[VEC];
+    if (GATES == kBoundedGates) bounds_of(sh, lane, lb);
+    auto decay = [&](int r, int i) { return GATES == kBoundedGates ? fmaf(1.f - lb[i], sf[r][i], lb[i]) : sf[r][i]; };
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) A[i] = 1.f, H[i] = 0.f, M[i] = 0.f;
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const bool in = t0 + wave * kSpan + group * kRows + r < s.len;
-        float x[VEC], g[VEC];
-        if (OUT) Row8<T>::unpack(rx[r], x);
-        Row8<GT>::unpack(rg[r], g);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          float keep;
-          const float dec = decay_of<GATES>(g[i], lb[i], &keep);
-          a[r][i] = in ? dec : 1.f;
-          if (OUT) {
-            const float v = GATES ? keep * (x[i] * sigmoidf(x[i])) : x[i];
-            before[r][i] = in ? v : 0.f;
-            H[i] = fmaf(a[r][i], H[i], before[r][i]);
-          }
-          A[i] *= a[r][i];
+      for (int i = 0; i < VEC; ++i) {
+        if (GATES) {
+          sigmoid_both(sf[r][i], &sf[r][i], &rest[r][i]);
+          if (OUT) si[r][i] = sigmoidf(x[r][i]);
+        } else {
+          sf[r][i] = __expf(sf[r][i]);
         }
       }
+    auto weight = [&](int r, int i) { return GATES == kBoundedGates ? (1.f - lb[i]) * rest[r][i] : rest[r][i]; };   // 1 - a
+    auto input = [&](int r, int i) { return GATES ? weight(r, i) * (x[r][i] * si[r][i]) : x[r][i]; };
 #pragma unroll
-      for (int r = kRows - 1; r >= 0; --r)
+    for (int i = 0; i < VEC; ++i) {
+      const float a0 = decay(0, i), a1 = decay(1, i);
+      A[i] = a0 * a1;
+      M[i] = a0 * (d[0][i] + a1 * d[1][i]);
+    }
+    if (OUT) {
+      float P[VEC], H[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) M[i] = a[r][i] * (d[r][i] + M[i]);
-      if (OUT) {
-        float P[VEC];
+      for (int i = 0; i < VEC; ++i) {
+        P[i] = A[i];
+        H[i] = fmaf(decay(1, i), input(0, i), input(1, i));
+      }
+      join_groups<true>(P, H, group);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) P[i] = A[i];
-        join_groups<true>(P, H, group);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          const float ea = __shfl_up(P[i], 8, 64), eh = __shfl_up(H[i], 8, 64);
-          float h = group > 0 ? onto(ea, eh, hs[i]) : hs[i];
-#pragma unroll
-          for (int r = 0; r < kRows; ++r) {
-            const float u = before[r][i];
-            before[r][i] = h;
-            h = fmaf(a[r][i], h, u);
-          }
-        }
+      for (int i = 0; i < VEC; ++i) {
+        const float ahead = __shfl_up(onto(P[i], H[i], hs[i]), 8, 64);
+        before[0][i] = group > 0 ? ahead : hs[i];
+        before[1][i] = fmaf(decay(0, i), before[0][i], input(0, i));
       }
     }
     join_groups<false>(A, M, group);
     const float mine = join_waves<false>(sh, buf, A, M, group == 0, wave, lane, &carry, &all);
     if (!OUT) continue;
+    const int n = (int)(left - t0 < kSpan ? left - t0 : kSpan);
+    if (n <= 0) continue;
     float m[VEC];
     spread(sh, mine, wave, lane, m);
+    if (GATES == kBoundedGates) bounds_of(sh, lane, lb);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const float ea = __shfl_down(A[i], 8, 64), em = __shfl_down(M[i], 8, 64);
-      if (group + 1 < kGroups) m[i] = onto(ea, em, m[i]);
+      const float behind = __shfl_down(onto(A[i], M[i], m[i]), 8, 64);
+      m[i] = group + 1 < kGroups ? behind : m[i];
     }
 #pragma unroll
-    for (int r = kRows - 1; r >= 0; --r) {
-      const int64_t t = t0 + wave * kSpan + group * kRows + r, row = s.begin + t;
-      const int v = t < s.len ? valid : 0;
-      float x[VEC], g[VEC];
-      if (GATES) {
-        forget(rx[r]);
-        forget(rg[r]);
-      }
-      Row8<T>::unpack(rx[r], x);
-      Row8<GT>::unpack(rg[r], g);
+    for (int r = R - 1; r >= 0; --r) {
+      float dx[VEC], dg[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         const float l = d[r][i] + m[i];
-        m[i] = a[r][i] * l;
+        m[i] = decay(r, i) * l;
         if (GATES) {
-          float sf, rest;
-          sigmoid_both(g[i], &sf, &rest);
-          const float si = sigmoidf(x[i]), z = x[i] * si;
-          const float da = l * (before[r][i] - z);
-          x[i] = l * (1.f - lb[i]) * rest * fmaf(z, 1.f - si, si);
-          g[i] = da * (1.f - lb[i]) * sf * rest;
-          dlb[i] += v > i ? da * rest : 0.f;
+          const float z = x[r][i] * si[r][i], da = l * (before[r][i] - z);
+          dx[i] = l * weight(r, i) * fmaf(z, 1.f - si[r][i], si[r][i]);
+          dg[i] = da * weight(r, i) * sf[r][i];
+          if (GATES == kBoundedGates) dlb[i] = fmaf(da, rest[r][i], dlb[i]);
         } else {
-          x[i] = l;
-          g[i] = m[i] * before[r][i];
+          dx[i] = l;
+          dg[i] = m[i] * before[r][i];
         }
       }
-      store8<T, WIDE>((T*)p.dx + row * D + col, x, v);
-      store8<GT, WIDE>((GT*)p.dg + row * D + col, g, v);
+      store_row<T, WIDE, R>((T*)p.dx + out0 + t0 * D, D, ao, r, dx, n, group, valid, whole_block);
+      store_row<GT, WIDE, R>((GT*)p.dg + out0 + t0 * D, D, ao, r, dg, n, group, valid, whole_block);
     }
   }
   if (wave == 0 && ch < D) {
@@ -170,11 +147,12 @@ __global__ __launch_bounds__(kWaves * 64) void hgrn_bwd_kernel(HgrnParams p) {
       p.dh0[s.n * D + ch] = carry;
     }
   }
-  if (OUT && p.dlb && s.len > 0) {   // the segment's column sums: the groups of a wave, then the waves in order
+  if (OUT && GATES == kBoundedGates && p.dlb && s.len > 0) {   // the segment's column sums: the groups of a wave, then the waves in order
 #pragma unroll
-    for (int i = 0; i < VEC; ++i)
+    for (int i = 0; i < VEC; ++i) {
 #pragma unroll
       for (int k = 8; k < 64; k *= 2) dlb[i] += __shfl_xor(dlb[i], k, 64);
+    }
     __syncthreads();
     if (group == 0)
 #pragma unroll
@@ -189,7 +167,7 @@ __global__ __launch_bounds__(kWaves * 64) void hgrn_bwd_kernel(HgrnParams p) {
   }
 }
 
-template <typename T, typename GT, bool GATES, bool WIDE>
+template <typename T, typename GT, int GATES, bool WIDE>
 int launch_bwd(const HgrnParams& p, int64_t segments, int64_t empty, hipStream_t st) {
   if (p.maps) {
     hipLaunchKernelGGL((hgrn_bwd_kernel<T, GT, GATES, WIDE, false>), dim3((unsigned)(segments * p.ncb)), dim3(kWaves * 64), 0, st, p);
@@ -211,7 +189,7 @@ extern "C" int fla_hgrn_bwd(const void* x, const void* g, const float* lower_bou
   FLA_REQUIRE(offsets ? B == 1 && (indices || NT == 0) && chunk_offsets : N == B, FLA_E_INVALID);
   const int64_t nseg = fla_cdiv(T, segment), cbs = fla_cdiv(D, kCh), segments = offsets ? NT : B * nseg;
   FLA_REQUIRE(maps || offsets || nseg == 1, FLA_E_INVALID);
-  FLA_REQUIRE(D <= 0x3fffffff && (segments + N) <= 0x7fffffff / cbs, FLA_E_UNSUPPORTED);
+  FLA_REQUIRE(ldx <= FLA_HGRN_MAX_PITCH && ldg <= FLA_HGRN_MAX_PITCH && (segments + N) <= 0x7fffffff / cbs, FLA_E_UNSUPPORTED);
   HgrnParams p{};
   p.x = x, p.g = g, p.lb = lower_bound, p.states = const_cast<float*>(states), p.maps = maps;
   p.dout = dout, p.dht = dht, p.dx = dx, p.dg = dg, p.dh0 = dh0, p.dlb = dlb_partials;
@@ -221,11 +199,13 @@ extern "C" int fla_hgrn_bwd(const void* x, const void* g, const float* lower_bou
   const bool wide = wide_rows(x, ldx, D, x_dtype) && wide_rows(g, ldg, D, g_dtype) && wide_rows(dout, D, D, x_dtype) &&
                     wide_rows(dx, D, D, x_dtype) && wide_rows(dg, D, D, g_dtype);
   const int64_t empty = offsets ? N : 0;
+  const int kind = !gates ? kLogDecays : lower_bound ? kBoundedGates : kGates;
   hipStream_t st = (hipStream_t)stream;
 #define D_(XE, XT, GE, GT)                                                                                       \
   if (x_dtype == XE && g_dtype == GE) {                                                                          \
-    if (gates) return wide ? launch_bwd<XT, GT, true, true>(p, segments, empty, st) : launch_bwd<XT, GT, true, false>(p, segments, empty, st); \
-    return wide ? launch_bwd<XT, GT, false, true>(p, segments, empty, st) : launch_bwd<XT, GT, false, false>(p, segments, empty, st);         \
+    if (kind == kLogDecays) return wide ? launch_bwd<XT, GT, 0, true>(p, segments, empty, st) : launch_bwd<XT, GT, 0, false>(p, segments, empty, st); \
+    if (kind == kGates) return wide ? launch_bwd<XT, GT, 1, true>(p, segments, empty, st) : launch_bwd<XT, GT, 1, false>(p, segments, empty, st); \
+    return wide ? launch_bwd<XT, GT, 2, true>(p, segments, empty, st) : launch_bwd<XT, GT, 2, false>(p, segments, empty, st); \
   }
   HGRN_TYPES(D_)
 #undef D_

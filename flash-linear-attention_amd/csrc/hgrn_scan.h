@@ -1,10 +1,11 @@
 // The elementwise gated recurrence h_t = a_t h_{t-1} + u_t, what its forward and backward launches share.
 //
 // A step is an affine map of the state, so a run of steps is one too: (A, H) with h -> A h + H, joined in order.  A workgroup
-// owns 64 channels of a segment of a sequence and goes through it in tiles of 256 tokens (backward: 128): eight waves of 32 rows, a lane
-// four (two) rows of eight channels (16 bytes a load in 16 bits, a wave's load covers eight whole 128-byte rows).  A tile is joined in
-// three levels: the lane's rows in registers, the eight row groups of a wave by shuffles, the eight waves through LDS (one
-// barrier a tile).  Between tiles the state stays in a register of the lane with that channel's number.
+// owns 64 channels of a segment of a sequence and goes through it in tiles: eight waves of 8 R rows, a lane R = 2 or 4 rows of eight
+// channels (16 bytes a load in 16 bits, a wave's load covers eight whole 128-byte rows).  A tile is joined in
+// three levels: the lane's rows in registers, the eight row groups of a wave by shuffles, the waves through LDS (one
+// barrier a tile).  Between tiles the state stays in a register of the lane with that channel's number.  Rows past the end of a segment are
+// read as steps that change nothing: a log decay of 0, a forget gate of plus infinity, an input and a gradient of 0.
 //
 // Sequences are cut into segments where (sequence, 64 channels) pairs would leave CUs idle; a first launch then forms each
 // segment's map, and every workgroup of the second joins the maps of the segments ahead of its own (a fixed order, no atomics,
@@ -16,11 +17,12 @@
 namespace {
 
 constexpr int kCh = 64;                           // channels of a workgroup
-constexpr int kWaves = 8, kGroups = 8;            // waves, row groups of a wave
-constexpr int kFwdRows = 4, kBwdRows = 2;         // rows of a lane: what fits its registers
+constexpr int kWaves = 8, kGroups = 8;            // waves of a workgroup, row groups of a wave
 constexpr int kKept = FLA_HGRN_STATE_ROWS;        // rows from one kept state to the next
-static_assert(kKept == kGroups * kBwdRows, "a wave of the backward starts from a kept state");
-static_assert(FLA_HGRN_TILE == kWaves * kGroups * kFwdRows, "segments are whole tiles");
+static_assert(kKept == kGroups * 2, "a wave of the backward (R = 2) starts from a kept state");
+static_assert(FLA_HGRN_TILE == kWaves * kGroups * 4, "a segment is whole tiles of either kind");
+// what the operands hold
+enum Gates { kLogDecays = 0, kGates = 1, kBoundedGates = 2 };
 
 struct HgrnParams {
   const void* x;        // u, or the pre-activations i  [B,T,D], rows ldx apart
@@ -93,17 +95,26 @@ FLA_DEVICE void sigmoid_both(float x, float* s, float* rest) {
   *rest = x >= 0.f ? small : r;
 }
 
-// The decay of a step, and with GATES the weight 1 - a of its input
-template <bool GATES>
-FLA_DEVICE float decay_of(float g, float lb, float* keep) {
-  if (!GATES) {
-    *keep = 1.f;
-    return __expf(g);
+// Element offset of the lane's piece of its first row within the wave's rows; rows of at most 2^24 elements keep it in 32 bits
+template <int R>
+FLA_DEVICE uint32_t lane_at(int lane, int64_t ld) { return (uint32_t)(lane >> 3) * R * (uint32_t)ld + (lane & 7) * VEC; }
+
+// The lane's rows of a tile: `rows` is the wave's first row (64 channels from `cb` on), of which `left` exist
+template <typename T, bool WIDE, int R>
+FLA_DEVICE void fetch_rows(typename Row8<T>::raw (&r)[R], const T* rows, int64_t ld, uint32_t at, int left, int group, int valid,
+                           bool whole_block, float fill) {
+  if (WIDE && whole_block && left >= kGroups * R) {   // (uniform)
+#pragma unroll
+    for (int i = 0; i < R; ++i) r[i] = Row8<T>::load_raw(rows + i * ld + at);
+  } else {
+#pragma unroll
+    for (int i = 0; i < R; ++i) r[i] = load_raw8<T, WIDE>(rows + i * ld + at, group * R + i < left ? valid : 0, fill);
   }
-  float s, rest;
-  sigmoid_both(g, &s, &rest);
-  *keep = (1.f - lb) * rest;
-  return fmaf(1.f - lb, s, lb);
+}
+template <typename T, bool WIDE, int R>
+FLA_DEVICE void store_row(T* rows, int64_t ld, uint32_t at, int i, const float* v, int left, int group, int valid, bool whole_block) {
+  if (WIDE && whole_block && left >= kGroups * R) Row8<T>::store(rows + i * ld + at, v);
+  else store8<T, WIDE>(rows + i * ld + at, v, group * R + i < left ? valid : 0);
 }
 
 // A map on its way through the eight row groups of a wave: joined with those of lower (UP) or higher groups, own group included
@@ -112,12 +123,18 @@ FLA_DEVICE void join_groups(float A[VEC], float H[VEC], int group) {
 #pragma unroll
   for (int d = 1; d < kGroups; d *= 2) {
     const bool has = UP ? group >= d : group + d < kGroups;
+    float a[VEC], h[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const float a = UP ? __shfl_up(A[i], 8 * d, 64) : __shfl_down(A[i], 8 * d, 64);
-      const float h = UP ? __shfl_up(H[i], 8 * d, 64) : __shfl_down(H[i], 8 * d, 64);
-      H[i] = has ? fmaf(A[i], h, H[i]) : H[i];
-      A[i] = has ? A[i] * a : A[i];
+      a[i] = UP ? __shfl_up(A[i], 8 * d, 64) : __shfl_down(A[i], 8 * d, 64);
+      h[i] = UP ? __shfl_up(H[i], 8 * d, 64) : __shfl_down(H[i], 8 * d, 64);
+    }
+    if (has) {   // (a branch: selects would cost as much as the arithmetic)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        H[i] = fmaf(A[i], h[i], H[i]);
+        A[i] *= a[i];
+      }
     }
   }
 }
@@ -126,13 +143,28 @@ FLA_DEVICE void join_groups(float A[VEC], float H[VEC], int group) {
 struct TileShare {
   float A[2][kWaves][kCh], H[2][kWaves][kCh];
   float in[kWaves][kCh];
+  float lb[kCh];       // the lower bounds: read again for every tile, eight registers less
 };
+// The lower bounds of the workgroup's channels into LDS (channels that are not there: 0)
+FLA_DEVICE void keep_bounds(TileShare& sh, const float* lb, int first, int D) {
+  if (threadIdx.x < kCh) sh.lb[threadIdx.x] = first + (int)threadIdx.x < D ? lb[first + threadIdx.x] : 0.f;
+  __syncthreads();
+}
+FLA_DEVICE void bounds_of(const TileShare& sh, int lane, float o[VEC]) {
+  const int c = (lane & 7) * VEC;
+  const f32x4 a = *(const f32x4*)&sh.lb[c], b = *(const f32x4*)&sh.lb[c + 4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    o[i] = a[i];
+    o[4 + i] = b[i];
+  }
+}
 // Leaves a wave's map, whose eight channels the lanes of one group hold, and returns the state that enters this wave; `carry`,
 // the state that enters the tile, becomes the one that leaves it (both for the channel with the lane's number), and `all` the
 // product of the decays.  UP: waves in ascending order.
 template <bool UP>
-FLA_DEVICE float join_waves(TileShare& sh, int buf, const float A[VEC], const float H[VEC], bool holds, int wave, int lane, float* carry,
-                            float* all) {
+FLA_DEVICE float join_waves(TileShare& sh, int buf, const float A[VEC], const float H[VEC], bool holds, int wave, int lane,
+                            float* carry, float* all) {
   if (holds) {
     const int c = (lane & 7) * VEC;
     *(f32x4*)&sh.A[buf][wave][c] = f32x4{A[0], A[1], A[2], A[3]};
@@ -142,7 +174,7 @@ FLA_DEVICE float join_waves(TileShare& sh, int buf, const float A[VEC], const fl
   }
   lds_barrier();
   float c = *carry, mine = c, prod = *all;
-#pragma unroll
+#pragma unroll 4
   for (int k = 0; k < kWaves; ++k) {
     const int w = UP ? k : kWaves - 1 - k;
     if (w == wave) mine = c;

@@ -21,7 +21,7 @@ struct RmsParams {
   float* scale;         // [M], 8-bit rows only
   void* res_out;        // [M,N] or NULL
   float* rstd;          // [M] or NULL; backward: read
-  // backward: x is what the forward normalised, in the type of `kept_f32`
+  // backward: x is what the forward normalised
   const void* dy;
   const void* dres;     // [M,N] in the kept type, or NULL
   void* dx;
@@ -31,7 +31,7 @@ struct RmsParams {
   int64_t M;
   int N;
   float eps;
-  int res_f32, res_out_f32, w_f32, kept_f32, plain;   // plain: rows are not normalised (8-bit rows of x itself)
+  int res_f32, res_out_f32, w_f32, plain;   // plain: rows are not normalised (8-bit rows of x itself)
 };
 
 template <typename T, bool WIDE>
@@ -143,8 +143,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_fwd_kernel(RmsParam
   }
 }
 
-// Rows are walked so that the column sums of the weight gradients stay in registers and leave once per workgroup.
-template <typename T, int TPR, int NP, bool WIDE>
+// Rows are walked so that the column sums of the weight gradients stay in registers and leave once per workgroup.  The operands of the next
+// row are on their way while one is worked on.
+template <typename T, typename KT, int TPR, int NP, bool WIDE, bool BIAS>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_bwd_kernel(RmsParams p) {
   constexpr int BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR;
   __shared__ float lds[2][TPR > 64 ? TPR / 64 : 1];
@@ -156,19 +157,36 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_bwd_kernel(RmsParam
 #pragma unroll
     for (int i = 0; i < VEC; ++i) dw[q][i] = db[q][i] = 0.f;
   int turn = 0;
+  const float inv = 1.f / (float)N;
   const int64_t step = (int64_t)gridDim.x * RPB;
-  // every thread makes as many rounds: rows of several waves exchange through a barrier
-  for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < p.M; row0 += step, turn ^= 1) {
-    const int64_t row = row0 + rl;
+  typename Row8<KT>::raw ns[NP], nr[NP];
+  typename Row8<T>::raw nd[NP];
+  float nrstd;
+  auto fetch = [&](int64_t row) {
     const bool in = row < p.M;
-    float s[NP][VEC], d[NP][VEC];
-    const float rstd = in ? p.rstd[row] : 0.f;
+    nrstd = in ? p.rstd[row] : 0.f;
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
       const int col = (q * TPR + sub) * VEC, valid = in ? N - col : 0;
-      load8_of<T, WIDE>(p.x, p.kept_f32, row * N + col, valid, s[q]);
-      load8_of<T, WIDE>(p.dy, 0, row * N + col, valid, d[q]);
+      ns[q] = load_raw8<KT, WIDE>((const KT*)p.x + row * N + col, valid);
+      nd[q] = load_raw8<T, WIDE>((const T*)p.dy + row * N + col, valid);
+      if (p.dres) nr[q] = load_raw8<KT, WIDE>((const KT*)p.dres + row * N + col, valid);
     }
+  };
+  fetch((int64_t)blockIdx.x * RPB + rl);
+  // every thread makes as many rounds: rows of several waves exchange through a barrier
+  for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < p.M; row0 += step, turn ^= 1) {
+    const int64_t row = row0 + rl;
+    float s[NP][VEC], d[NP][VEC];
+    typename Row8<KT>::raw r8[NP];
+    const float rstd = nrstd;
+#pragma unroll
+    for (int q = 0; q < NP; ++q) {
+      Row8<KT>::unpack(ns[q], s[q]);
+      Row8<T>::unpack(nd[q], d[q]);
+      r8[q] = nr[q];
+    }
+    fetch(row + step);
     float c = 0.f;
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
@@ -179,27 +197,27 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_bwd_kernel(RmsParam
       for (int i = 0; i < VEC; ++i) {
         s[q][i] *= rstd;
         dw[q][i] = fmaf(d[q][i], s[q][i], dw[q][i]);
-        db[q][i] += d[q][i];
+        if (BIAS) db[q][i] += d[q][i];
         if (p.w) d[q][i] *= w[i];
         c = fmaf(d[q][i], s[q][i], c);
       }
     }
-    c = row_reduce<TPR, false>(c, lds, turn) / (float)N;
+    c = row_reduce<TPR, false>(c, lds, turn) * inv;
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
-      const int col = (q * TPR + sub) * VEC, valid = in ? N - col : 0;
+      const int col = (q * TPR + sub) * VEC, valid = row < p.M ? N - col : 0;
       float r[VEC];
-      if (p.dres) load8_of<T, WIDE>(p.dres, p.kept_f32, row * N + col, valid, r);
+      if (p.dres) Row8<KT>::unpack(r8[q], r);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         d[q][i] = (d[q][i] - s[q][i] * c) * rstd;
         if (p.dres) d[q][i] += r[i];
       }
       store8<T, WIDE>((T*)p.dx + row * N + col, d[q], valid);
-      if (p.dres_in) store8_of<T, WIDE>(p.dres_in, p.kept_f32, row * N + col, valid, d[q]);
+      if (p.dres_in) store8<KT, WIDE>((KT*)p.dres_in + row * N + col, d[q], valid);
     }
   }
-  for (int which = 0; which < 2; ++which) {
+  for (int which = 0; which < (BIAS ? 2 : 1); ++which) {
     float* part = which ? p.db_part : p.dw_part;
     if (!part) continue;   // uniform
     part += (int64_t)blockIdx.x * N;
@@ -208,9 +226,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_bwd_kernel(RmsParam
       const float* mine = which ? db[q] : dw[q];
       const int col = (q * TPR + sub) * VEC;
       if (RPB == 1) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          if (col + i < N) part[col + i] = mine[i];
+        store8<float, WIDE>(part + col, mine, N - col);
       } else {
         __syncthreads();
 #pragma unroll
@@ -227,39 +243,59 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_bwd_kernel(RmsParam
   }
 }
 
-// (threads to a row, passes) by the row's length
-#define RMS_SHAPES(CALL)               \
-  if (N <= 64) CALL(8, 1)              \
-  else if (N <= 128) CALL(16, 1)       \
-  else if (N <= 256) CALL(32, 1)       \
-  else if (N <= 512) CALL(64, 1)       \
-  else if (N <= 1024) CALL(64, 2)      \
-  else if (N <= 2048) CALL(64, 4)      \
-  else if (N <= 4096) CALL(256, 2)     \
-  else if (N <= 8192) CALL(256, 4)     \
+// (threads to a row, passes) by the row's length.  Forward: a wave to a row up to 2048 elements (16384 rows in 54 us, 4.95 TB/s), but four
+// waves where there are few rows (32 rows of 2048 to 8 bits: 4.1 us, with one wave 5.5).  Backward: rows of one pass as long as there are
+// threads, since the column sums and the next row's operands take registers (16384 rows of 2048: 54 us; with four passes of a wave 75 us,
+// 80 with the next row's operands in flight).
+#define RMS_FWD_SHAPES(CALL)                       \
+  if (N <= 64) CALL(8, 1)                          \
+  else if (N <= 128) CALL(16, 1)                   \
+  else if (N <= 256) CALL(32, 1)                   \
+  else if (N <= 512) CALL(64, 1)                   \
+  else if (N <= 2048 && p.M <= kFewRows) CALL(256, 1) \
+  else if (N <= 1024) CALL(64, 2)                  \
+  else if (N <= 2048) CALL(64, 4)                  \
+  else if (N <= 4096) CALL(256, 2)                 \
+  else if (N <= 8192) CALL(256, 4)                 \
+  else CALL(512, 4)
+#define RMS_BWD_SHAPES(CALL)      \
+  if (N <= 64) CALL(8, 1)         \
+  else if (N <= 128) CALL(16, 1)  \
+  else if (N <= 256) CALL(32, 1)  \
+  else if (N <= 512) CALL(64, 1)  \
+  else if (N <= 2048) CALL(256, 1) \
+  else if (N <= 4096) CALL(512, 1) \
+  else if (N <= 8192) CALL(512, 2) \
   else CALL(512, 4)
 
-int rows_per_block(int64_t N) {
-  const int threads = N <= 64 ? 8 : N <= 128 ? 16 : N <= 256 ? 32 : N <= 2048 ? 64 : 256;
-  return 256 / threads;
-}
+constexpr int64_t kFewRows = 1024;
 constexpr int64_t kMaxN = 512 * 4 * VEC;
+constexpr int64_t kBwdWorkgroups = 1024;
+int bwd_rows_per_block(int64_t N) { return N <= 64 ? 32 : N <= 128 ? 16 : N <= 256 ? 8 : N <= 512 ? 4 : 1; }
 
 template <typename T, bool WIDE, bool QUANT>
 int launch_fwd(const RmsParams& p, hipStream_t st) {
   const int N = p.N;
-  const dim3 grid((unsigned)fla_cdiv(p.M, rows_per_block(N)));
-#define CALL(TPR, NP) hipLaunchKernelGGL((rms_fwd_kernel<T, TPR, NP, WIDE, QUANT>), grid, dim3(TPR > 256 ? TPR : 256), 0, st, p);
-  RMS_SHAPES(CALL)
+#define CALL(TPR, NP)                                                                                                             \
+  {                                                                                                                               \
+    constexpr int block = TPR > 256 ? TPR : 256;                                                                                  \
+    hipLaunchKernelGGL((rms_fwd_kernel<T, TPR, NP, WIDE, QUANT>), dim3((unsigned)fla_cdiv(p.M, block / TPR)), dim3(block), 0, st, p); \
+  }
+  RMS_FWD_SHAPES(CALL)
 #undef CALL
   FLA_CHECK_LAUNCH();
   return FLA_OK;
 }
-template <typename T, bool WIDE>
+template <typename T, typename KT, bool WIDE>
 int launch_bwd(const RmsParams& p, int grid, hipStream_t st) {
   const int N = p.N;
-#define CALL(TPR, NP) hipLaunchKernelGGL((rms_bwd_kernel<T, TPR, NP, WIDE>), dim3(grid), dim3(TPR > 256 ? TPR : 256), 0, st, p);
-  RMS_SHAPES(CALL)
+#define CALL(TPR, NP)                                                                                                                       \
+  {                                                                                                                                         \
+    constexpr int block = TPR > 256 ? TPR : 256;                                                                                            \
+    if (p.db_part) hipLaunchKernelGGL((rms_bwd_kernel<T, KT, TPR, NP, WIDE, true>), dim3(grid), dim3(block), 0, st, p);                     \
+    else hipLaunchKernelGGL((rms_bwd_kernel<T, KT, TPR, NP, WIDE, false>), dim3(grid), dim3(block), 0, st, p);                              \
+  }
+  RMS_BWD_SHAPES(CALL)
 #undef CALL
   FLA_CHECK_LAUNCH();
   return FLA_OK;
@@ -304,8 +340,8 @@ extern "C" int fla_rms_norm_fwd(const void* x, const void* residual, int residua
 
 extern "C" int fla_rms_norm_workgroups(int64_t M, int64_t N) {
   if (M <= 0 || N <= 0) return 1;
-  const int64_t g = fla_cdiv(M, rows_per_block(N));
-  return (int)(g < 1024 ? g : 1024);
+  const int64_t g = fla_cdiv(M, bwd_rows_per_block(N));
+  return (int)(g < kBwdWorkgroups ? g : kBwdWorkgroups);
 }
 
 extern "C" int fla_rms_norm_bwd(const void* dy, const void* kept, int kept_dtype, const void* weight, int weight_dtype, const float* rstd,
@@ -318,12 +354,13 @@ extern "C" int fla_rms_norm_bwd(const void* dy, const void* kept, int kept_dtype
   RmsParams p{};
   p.x = kept, p.w = weight, p.rstd = (float*)rstd, p.dy = dy, p.dres = dresidual, p.dx = dx, p.dres_in = dresidual_in;
   p.dw_part = dw_partial, p.db_part = db_partial, p.M = M, p.N = (int)N;
-  p.kept_f32 = kept_dtype == FLA_F32, p.w_f32 = weight_dtype == FLA_F32;
+  p.w_f32 = weight_dtype == FLA_F32;
   const bool w = wide(N, {dy, kept, weight, dresidual, dx, dresidual_in});
   const int grid = fla_rms_norm_workgroups(M, N);
   hipStream_t st = (hipStream_t)stream;
-#define D_(E, T) \
-  if (dtype == E) return w ? launch_bwd<T, true>(p, grid, st) : launch_bwd<T, false>(p, grid, st);
+#define D_(E, T)                                                                                                  \
+  if (dtype == E && kept_dtype == E) return w ? launch_bwd<T, T, true>(p, grid, st) : launch_bwd<T, T, false>(p, grid, st); \
+  if (dtype == E) return w ? launch_bwd<T, float, true>(p, grid, st) : launch_bwd<T, float, false>(p, grid, st);
   D_(FLA_BF16, bf16)
   D_(FLA_F16, f16)
   D_(FLA_F32, float)

@@ -75,19 +75,21 @@ struct Row8<f16> {
   }
 };
 
-// Eight elements at p of which the first `valid` exist (<= 0: none, zeros come back and p is not read).  WIDE: p is aligned to
-// 16 bytes and valid is 8 or more, or not positive; otherwise any element address goes, one element at a time.
+// Eight elements at p of which the first `valid` exist, the others as `fill` (<= 0: none, p is not read).  WIDE: p is aligned to 16 bytes
+// and valid is 8 or more, or not positive; otherwise any element address goes, whole pieces in one load all the same.
 template <typename T, bool WIDE>
-FLA_DEVICE typename Row8<T>::raw load_raw8(const T* p, int valid) {
+FLA_DEVICE typename Row8<T>::raw load_raw8(const T* p, int valid, float fill = 0.f) {
   typename Row8<T>::raw r;
-  if (WIDE) {
-    if (valid > 0) return Row8<T>::load_raw(p);
-    __builtin_memset(&r, 0, sizeof r);
+  if (WIDE && valid > 0) return Row8<T>::load_raw(p);
+  if (!WIDE && valid >= VEC) {
+    typedef T any8 __attribute__((ext_vector_type(8), aligned(alignof(T))));
+    const any8 v = *(const any8*)p;
+    __builtin_memcpy(&r, &v, sizeof r);
     return r;
   }
   T e[VEC];
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) e[i] = i < valid ? p[i] : (T)0.f;
+  for (int i = 0; i < VEC; ++i) e[i] = !WIDE && i < valid ? p[i] : (T)fill;
   __builtin_memcpy(&r, e, sizeof r);
   return r;
 }
@@ -95,22 +97,17 @@ template <typename T, bool WIDE>
 FLA_DEVICE void store8(T* p, const float* v, int valid) {
   if (WIDE) {
     if (valid > 0) Row8<T>::store(p, v);
-    return;
+  } else if (valid >= VEC) {
+    typedef T any8 __attribute__((ext_vector_type(8), aligned(alignof(T))));
+    any8 o;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) o[i] = (T)v[i];
+    *(any8*)p = o;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (i < valid) p[i] = (T)v[i];
   }
-#pragma unroll
-  for (int i = 0; i < VEC; ++i)
-    if (i < valid) p[i] = (T)v[i];
-}
-
-// The same registers, and nothing the compiler knows about them: what was computed from r before is computed again after, instead of
-// being held (sixteen or more values a lane in the kernels that ask for it).
-template <typename R>
-FLA_DEVICE void forget(R& r) {
-  int w[sizeof(R) / 4];
-  __builtin_memcpy(w, &r, sizeof r);
-#pragma unroll
-  for (unsigned i = 0; i < sizeof(R) / 4; ++i) asm volatile("" : "+v"(w[i]));
-  __builtin_memcpy(&r, w, sizeof r);
 }
 
 // sum over the LPR lanes of a group (LPR a power of two <= 64), result in every lane

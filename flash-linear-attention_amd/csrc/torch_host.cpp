@@ -640,7 +640,7 @@ struct NormGateNode : torch::autograd::Function<NormGateNode> {
 Tensor pitched(const Tensor& x, int64_t* ld) {
   const int64_t B = x.size(0), T = x.size(1), D = x.size(2);
   const int64_t pitch = T > 1 ? x.stride(1) : B > 1 ? x.stride(0) : D;
-  const bool fits = (D == 1 || x.stride(2) == 1) && pitch >= D && (T == 1 || B == 1 || x.stride(0) == T * x.stride(1));
+  const bool fits = (D == 1 || x.stride(2) == 1) && pitch >= D && pitch <= FLA_HGRN_MAX_PITCH && (T == 1 || B == 1 || x.stride(0) == T * x.stride(1));
   *ld = fits ? pitch : D;
   return fits ? x : x.contiguous();
 }

@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define FLA_ABI_VERSION 22
+#define FLA_ABI_VERSION 23
 
 enum fla_dtype { FLA_F32 = 0, FLA_BF16 = 1, FLA_F16 = 2 };
 
@@ -814,6 +814,7 @@ int fla_gdn_gate_bwd(const void* a, const void* b, const float* A_log, const flo
  * fla_hgrn_step: one token for each of N sequences, x, g, o [N, D]; ht may be h0. */
 #define FLA_HGRN_TILE 256
 #define FLA_HGRN_STATE_ROWS 16
+#define FLA_HGRN_MAX_PITCH (1 << 24) /* elements from one row to the next */
 int64_t fla_hgrn_segment(int64_t n_seqs, int64_t tokens, int64_t longest, int64_t D);
 int fla_hgrn_fwd(const void* x, const void* g, const float* lower_bound, const float* h0, void* o, float* ht, float* states,
                  float* maps, const int64_t* offsets, const int64_t* indices, const int64_t* chunk_offsets, int64_t NT,

@@ -33,7 +33,7 @@ def test_library_exports_every_declared_symbol():
 # What a binding relies on, by version: a digest of the C declarations and of the names and argument counts of the host
 # extension's entries (15: without the names).
 INTERFACES = {15: "b7a4f7cfed6a371e", 16: "ecb9b6be8de7c997", 17: "8d259aba7a1ce02b", 18: "d280e32277841484",
-              19: "ffed6d79950c4a2c", 20: "7277003d13de7e6d", 21: "88fd3932e6552668", 22: "491ca6ca57f1a4d8"}
+              19: "ffed6d79950c4a2c", 20: "7277003d13de7e6d", 21: "88fd3932e6552668", 22: "491ca6ca57f1a4d8", 23: "6120caa44fecd8de"}
 
 
 def _interface():
