@@ -22,7 +22,6 @@ __global__ __launch_bounds__(kWaves * 64) void hgrn_bwd_kernel(HgrnParams p) {
   if (!OUT && s.c == 0) return;               // nothing is ahead of the first segment of a sequence
   const int ch = cb * kCh + lane;
   const int col = cb * kCh + (lane & 7) * VEC, valid = D - col;
-  const bool whole_block = cb * kCh + kCh <= D;
   if (GATES == kBoundedGates) keep_bounds(sh, p.lb, cb * kCh, D);
   float dlb[VEC];
 #pragma unroll
@@ -38,15 +37,20 @@ __global__ __launch_bounds__(kWaves * 64) void hgrn_bwd_kernel(HgrnParams p) {
   typename Row8<T>::raw nx[R], nd[R];
   typename Row8<GT>::raw ng[R];
   typename Row8<float>::raw nh;
-  auto fetch = [&](int64_t t0) {
-    const int n = t0 < 0 ? 0 : (int)(left - t0 < kSpan ? left - t0 : kSpan);
-    if (OUT) fetch_rows<T, WIDE>(nx, xr + t0 * p.ldx, p.ldx, ax, n, group, valid, whole_block, 0.f);
-    fetch_rows<GT, WIDE>(ng, gr + t0 * p.ldg, p.ldg, ag, n, group, valid, whole_block, GATES ? __builtin_inff() : 0.f);
-    fetch_rows<T, WIDE>(nd, (const T*)p.dout + out0 + t0 * D, D, ao, p.dout ? n : 0, group, valid, whole_block, 0.f);
-    if (OUT) nh = load_raw8<float, WIDE>(st0 + t0 / kSpan * D, n > 0 ? valid : 0);
+  auto fetch = [&](int64_t t0, auto full) {
+    constexpr bool F = decltype(full)::value;
+    const int64_t n = t0 < 0 ? 0 : left - t0;
+    if (OUT) fetch_rows<T, WIDE, R, F>(nx, xr + t0 * p.ldx, p.ldx, ax, n, group, valid, 0.f);
+    fetch_rows<GT, WIDE, R, F>(ng, gr + t0 * p.ldg, p.ldg, ag, n, group, valid, GATES ? __builtin_inff() : 0.f);
+    fetch_rows<T, WIDE, R, F>(nd, (const T*)p.dout + out0 + t0 * D, D, ao, p.dout ? n : 0, group, valid, 0.f);
+    if (OUT && F) nh = Row8<float>::load_raw(st0 + t0 / kKept * D);
+    else if (OUT) nh = load_raw8<float, WIDE>(st0 + t0 / kKept * D, n > 0 ? valid : 0);
   };
+  // tiles of which all rows and channels exist
+  const int64_t whole = WIDE && cb * kCh + kCh <= D && p.dout ? s.len / kTile * kTile : 0;
   const int64_t last = s.len > 0 ? (s.len - 1) / kTile * kTile : -1;
-  fetch(last);
+  if (last >= 0 && last < whole) fetch(last, Full<true>());
+  else fetch(last, Full<false>());
   float carry = 0.f, all = 1.f;
   if (OUT && ch < D) {
     if (p.dht) carry = p.dht[s.n * D + ch];
@@ -55,7 +59,7 @@ __global__ __launch_bounds__(kWaves * 64) void hgrn_bwd_kernel(HgrnParams p) {
     for (int64_t k = s.count - 1; k > s.c; --k) carry = onto(m[2 * k * D], m[(2 * k + 1) * D], carry);
   }
   int buf = 0;
-  for (int64_t t0 = last; t0 >= 0; t0 -= kTile, buf ^= 1) {
+  auto tile = [&](int64_t t0, auto full, auto full_next) {
     // Held for the second half: x itself, sigmoid(x), both sides of the forget gate's sigmoid (or the decay), do and the state ahead
     float x[R][VEC], si[R][VEC], sf[R][VEC], rest[R][VEC], d[R][VEC], before[R][VEC];
     float A[VEC], M[VEC], hs[VEC];
@@ -66,7 +70,7 @@ __global__ __launch_bounds__(kWaves * 64) void hgrn_bwd_kernel(HgrnParams p) {
       Row8<T>::unpack(nd[r], d[r]);
     }
     if (OUT) Row8<float>::unpack(nh, hs);
-    fetch(t0 - kTile);
+    fetch(t0 - kTile, full_next);
     float lb[VEC];
     if (GATES == kBoundedGates) bounds_of(sh, lane, lb);
     auto decay = [&](int r, int i) { return GATES == kBoundedGates ? fmaf(1.f - lb[i], sf[r][i], lb[i]) : sf[r][i]; };
@@ -106,9 +110,10 @@ __global__ __launch_bounds__(kWaves * 64) void hgrn_bwd_kernel(HgrnParams p) {
     }
     join_groups<false>(A, M, group);
     const float mine = join_waves<false>(sh, buf, A, M, group == 0, wave, lane, &carry, &all);
-    if (!OUT) continue;
-    const int n = (int)(left - t0 < kSpan ? left - t0 : kSpan);
-    if (n <= 0) continue;
+    buf ^= 1;
+    if (!OUT) return;
+    const int64_t n = left - t0;
+    if (!decltype(full)::value && n <= 0) return;   // (uniform, and no barrier behind it)
     float m[VEC];
     spread(sh, mine, wave, lane, m);
     if (GATES == kBoundedGates) bounds_of(sh, lane, lb);
@@ -134,10 +139,18 @@ __global__ __launch_bounds__(kWaves * 64) void hgrn_bwd_kernel(HgrnParams p) {
           dg[i] = m[i] * before[r][i];
         }
       }
-      store_row<T, WIDE, R>((T*)p.dx + out0 + t0 * D, D, ao, r, dx, n, group, valid, whole_block);
-      store_row<GT, WIDE, R>((GT*)p.dg + out0 + t0 * D, D, ao, r, dg, n, group, valid, whole_block);
+      store_row<T, WIDE, R, decltype(full)::value>((T*)p.dx + out0 + t0 * D, D, ao, r, dx, n, group, valid);
+      store_row<GT, WIDE, R, decltype(full)::value>((GT*)p.dg + out0 + t0 * D, D, ao, r, dg, n, group, valid);
     }
+  };
+  int64_t t0 = last;
+  if (t0 >= whole && t0 >= 0) {   // the ragged end (or no tile is whole)
+    if (whole > 0) tile(t0, Full<false>(), Full<true>()), t0 -= kTile;
+    else
+      for (; t0 >= 0; t0 -= kTile) tile(t0, Full<false>(), Full<false>());
   }
+  for (; t0 > 0; t0 -= kTile) tile(t0, Full<true>(), Full<true>());
+  if (t0 == 0) tile(t0, Full<true>(), Full<false>());
   if (wave == 0 && ch < D) {
     if (!OUT) {
       float* q = p.maps + s.id * 2 * D + ch;

@@ -16,7 +16,6 @@ __global__ __launch_bounds__(kWaves * 64) void hgrn_fwd_kernel(HgrnParams p) {
   if (!OUT && s.c + 1 == s.count) return;     // nothing follows the last segment of a sequence
   const int ch = cb * kCh + lane;             // the channel this lane carries between tiles
   const int col = cb * kCh + (lane & 7) * VEC, valid = D - col;   // the eight it scans
-  const bool whole_block = cb * kCh + kCh <= D;
   if (GATES == kBoundedGates) keep_bounds(sh, p.lb, cb * kCh, D);
 
   // the wave's rows of the tile that is fetched
@@ -25,15 +24,18 @@ __global__ __launch_bounds__(kWaves * 64) void hgrn_fwd_kernel(HgrnParams p) {
   const GT* gr = (const GT*)p.g + row0 * p.ldg + cb * kCh;
   T* orow = (T*)p.o + row0 * D + cb * kCh;
   const uint32_t ax = lane_at<R>(lane, p.ldx), ag = lane_at<R>(lane, p.ldg), ao = lane_at<R>(lane, D);
-  int64_t left = s.len - wave * kSpan;
+  const int64_t left = s.len - wave * kSpan;
   typename Row8<T>::raw nx[R];
   typename Row8<GT>::raw ng[R];
-  auto fetch = [&](int64_t t0) {
-    const int n = (int)(left - t0 < kSpan ? left - t0 : kSpan);
-    fetch_rows<T, WIDE>(nx, xr + t0 * p.ldx, p.ldx, ax, n, group, valid, whole_block, 0.f);
-    fetch_rows<GT, WIDE>(ng, gr + t0 * p.ldg, p.ldg, ag, n, group, valid, whole_block, GATES ? __builtin_inff() : 0.f);
+  auto fetch = [&](int64_t t0, auto full) {
+    constexpr bool F = decltype(full)::value;
+    fetch_rows<T, WIDE, R, F>(nx, xr + t0 * p.ldx, p.ldx, ax, left - t0, group, valid, 0.f);
+    fetch_rows<GT, WIDE, R, F>(ng, gr + t0 * p.ldg, p.ldg, ag, left - t0, group, valid, GATES ? __builtin_inff() : 0.f);
   };
-  fetch(0);
+  // tiles of which all rows and channels exist
+  const int64_t whole = WIDE && cb * kCh + kCh <= D ? s.len / kTile * kTile : 0;
+  if (whole > 0) fetch(0, Full<true>());
+  else fetch(0, Full<false>());
   float carry = 0.f, all = 1.f;
   if (OUT && ch < D) {
     if (p.h0) carry = p.h0[s.n * D + ch];
@@ -42,14 +44,14 @@ __global__ __launch_bounds__(kWaves * 64) void hgrn_fwd_kernel(HgrnParams p) {
     for (int64_t k = 0; k < s.c; ++k) carry = onto(m[2 * k * D], m[(2 * k + 1) * D], carry);
   }
   int buf = 0;
-  for (int64_t t0 = 0; t0 < s.len; t0 += kTile, buf ^= 1) {
+  auto tile = [&](int64_t t0, auto full, auto full_next) {
     float a[R][VEC], u[R][VEC], A[VEC], H[VEC];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       Row8<T>::unpack(nx[r], u[r]);
       Row8<GT>::unpack(ng[r], a[r]);
     }
-    fetch(t0 + kTile);
+    fetch(t0 + kTile, full_next);
     float lb[VEC];
     if (GATES == kBoundedGates) bounds_of(sh, lane, lb);
 #pragma unroll
@@ -76,9 +78,10 @@ __global__ __launch_bounds__(kWaves * 64) void hgrn_fwd_kernel(HgrnParams p) {
     }
     join_groups<true>(A, H, group);
     const float mine = join_waves<true>(sh, buf, A, H, group == kGroups - 1, wave, lane, &carry, &all);
-    if (!OUT) continue;
-    const int n = (int)(left - t0 < kSpan ? left - t0 : kSpan);
-    if (n <= 0) continue;   // (uniform, and no barrier behind it)
+    buf ^= 1;
+    if (!OUT) return;
+    const int64_t n = left - t0;
+    if (!decltype(full)::value && n <= 0) return;   // (uniform, and no barrier behind it)
     float h[VEC];
     spread(sh, mine, wave, lane, h);
     // the state behind the groups ahead: that of the neighbour's last row
@@ -95,9 +98,13 @@ __global__ __launch_bounds__(kWaves * 64) void hgrn_fwd_kernel(HgrnParams p) {
     for (int r = 0; r < R; ++r) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) h[i] = fmaf(a[r][i], h[i], u[r][i]);
-      store_row<T, WIDE, R>(orow + t0 * D, D, ao, r, h, n, group, valid, whole_block);
+      store_row<T, WIDE, R, decltype(full)::value>(orow + t0 * D, D, ao, r, h, n, group, valid);
     }
-  }
+  };
+  int64_t t0 = 0;
+  for (; t0 + kTile < whole; t0 += kTile) tile(t0, Full<true>(), Full<true>());
+  if (t0 < whole) tile(t0, Full<true>(), Full<false>()), t0 += kTile;
+  for (; t0 < s.len; t0 += kTile) tile(t0, Full<false>(), Full<false>());
   if (wave == 0 && ch < D) {
     if (!OUT) {
       float* m = p.maps + s.id * 2 * D + ch;

@@ -99,21 +99,24 @@ FLA_DEVICE void sigmoid_both(float x, float* s, float* rest) {
 template <int R>
 FLA_DEVICE uint32_t lane_at(int lane, int64_t ld) { return (uint32_t)(lane >> 3) * R * (uint32_t)ld + (lane & 7) * VEC; }
 
-// The lane's rows of a tile: `rows` is the wave's first row (64 channels from `cb` on), of which `left` exist
-template <typename T, bool WIDE, int R>
-FLA_DEVICE void fetch_rows(typename Row8<T>::raw (&r)[R], const T* rows, int64_t ld, uint32_t at, int left, int group, int valid,
-                           bool whole_block, float fill) {
-  if (WIDE && whole_block && left >= kGroups * R) {   // (uniform)
+template <bool V>
+struct Full {
+  static constexpr bool value = V;
+};
+// The lane's rows of a tile: `rows` is the wave's first row (64 channels from `cb` on), of which `left` exist.  FULL: all of the wave's rows and
+// channels exist, and no branch stands around the loads: the compiler counts what is in flight behind a load, and where a branch may have
+// skipped some of it, waits for all of it instead, the stores of the tile before included.
+template <typename T, bool WIDE, int R, bool FULL>
+FLA_DEVICE void fetch_rows(typename Row8<T>::raw (&r)[R], const T* rows, int64_t ld, uint32_t at, int64_t left, int group, int valid, float fill) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) r[i] = Row8<T>::load_raw(rows + i * ld + at);
-  } else {
-#pragma unroll
-    for (int i = 0; i < R; ++i) r[i] = load_raw8<T, WIDE>(rows + i * ld + at, group * R + i < left ? valid : 0, fill);
+  for (int i = 0; i < R; ++i) {
+    if (FULL) r[i] = Row8<T>::load_raw(rows + i * ld + at);
+    else r[i] = load_raw8<T, WIDE>(rows + i * ld + at, group * R + i < left ? valid : 0, fill);
   }
 }
-template <typename T, bool WIDE, int R>
-FLA_DEVICE void store_row(T* rows, int64_t ld, uint32_t at, int i, const float* v, int left, int group, int valid, bool whole_block) {
-  if (WIDE && whole_block && left >= kGroups * R) Row8<T>::store(rows + i * ld + at, v);
+template <typename T, bool WIDE, int R, bool FULL>
+FLA_DEVICE void store_row(T* rows, int64_t ld, uint32_t at, int i, const float* v, int64_t left, int group, int valid) {
+  if (FULL) Row8<T>::store(rows + i * ld + at, v);
   else store8<T, WIDE>(rows + i * ld + at, v, group * R + i < left ? valid : 0);
 }
 
