@@ -63,6 +63,9 @@ CASES = [  # M, N, K, type, bias, activation, residual
     (250, 1000, 528, BF, BF, "gelu", BF), (1400, 1411, 272, HF, FL, "relu", HF), (3500, 4000, 384, BF, BF, "silu", BF), (3601, 3333, 208, HF, None, None, FL),
     (130, 65, 16, BF, None, None, None), (70, 130, 4112, BF, BF, "silu", FL), (60, 258, 6400, HF, None, "gelu", HF), (300, 2050, 400, BF, FL, None, BF),
     (2000, 2040, 128, BF, BF, None, None),
+    # panels of four waves, tiles for few rows, slices of K, tiles of three slices and more
+    (5, 4100, 1040, BF, BF, "silu", BF), (20, 4112, 272, HF, None, None, FL), (45, 4200, 144, BF, FL, "relu", None), (64, 4099, 1168, BF, BF, None, BF),
+    (64, 12300, 1040, BF, None, None, BF), (100, 256, 6288, HF, HF, "silu", HF), (1100, 2100, 400, BF, BF, "gelu", BF),
 ]
 
 

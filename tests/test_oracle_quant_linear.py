@@ -55,5 +55,5 @@ def test_library_arguments():
     assert call(x=odd) == -3
     # few tiles and a long K: in slices, which need a workspace; single rows and large products are not cut
     splits = lib.fla_quant_linear_splits
-    assert splits(48, 2048, 8192) > 1 and splits(1, 4096, 2048) == 1 and splits(8191, 8192, 2048) == 1 and splits(0, 1, 1) == 1
-    assert lib.fla_quant_linear(p, p, p, p, None, 0, None, 0, p, 48, 2048, 8192, 0, 1, None, None) == -1
+    assert splits(100, 2048, 8192) > 1 and splits(48, 2048, 8192) == 1 and splits(1, 4096, 2048) == 1 and splits(8191, 8192, 2048) == 1 and splits(0, 1, 1) == 1
+    assert lib.fla_quant_linear(p, p, p, p, None, 0, None, 0, p, 100, 2048, 8192, 0, 1, None, None) == -1
