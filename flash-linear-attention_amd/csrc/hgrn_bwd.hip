@@ -202,7 +202,7 @@ extern "C" int fla_hgrn_bwd(const void* x, const void* g, const float* lower_bou
   FLA_REQUIRE(offsets ? B == 1 && (indices || NT == 0) && chunk_offsets : N == B, FLA_E_INVALID);
   const int64_t nseg = fla_cdiv(T, segment), cbs = fla_cdiv(D, kCh), segments = offsets ? NT : B * nseg;
   FLA_REQUIRE(maps || offsets || nseg == 1, FLA_E_INVALID);
-  FLA_REQUIRE(ldx <= FLA_HGRN_MAX_PITCH && ldg <= FLA_HGRN_MAX_PITCH && (segments + N) <= 0x7fffffff / cbs, FLA_E_UNSUPPORTED);
+  FLA_REQUIRE(ldx <= FLA_HGRN_MAX_PITCH && ldg <= FLA_HGRN_MAX_PITCH && segments + N <= kMostWorkgroups / cbs, FLA_E_UNSUPPORTED);
   HgrnParams p{};
   p.x = x, p.g = g, p.lb = lower_bound, p.states = const_cast<float*>(states), p.maps = maps;
   p.dout = dout, p.dht = dht, p.dx = dx, p.dg = dg, p.dh0 = dh0, p.dlb = dlb_partials;

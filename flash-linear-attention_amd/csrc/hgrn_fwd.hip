@@ -207,7 +207,7 @@ extern "C" int fla_hgrn_fwd(const void* x, const void* g, const float* lower_bou
   FLA_REQUIRE(offsets ? B == 1 && (indices || NT == 0) && chunk_offsets : N == B, FLA_E_INVALID);
   const int64_t nseg = fla_cdiv(T, segment), cbs = fla_cdiv(D, kCh), segments = offsets ? NT : B * nseg;
   FLA_REQUIRE(maps || offsets || nseg == 1, FLA_E_INVALID);
-  FLA_REQUIRE(ldx <= FLA_HGRN_MAX_PITCH && ldg <= FLA_HGRN_MAX_PITCH && (segments + N) <= 0x7fffffff / cbs, FLA_E_UNSUPPORTED);
+  FLA_REQUIRE(ldx <= FLA_HGRN_MAX_PITCH && ldg <= FLA_HGRN_MAX_PITCH && segments + N <= kMostWorkgroups / cbs, FLA_E_UNSUPPORTED);
   HgrnParams p{};
   p.x = x, p.g = g, p.lb = lower_bound, p.h0 = h0, p.o = o, p.ht = ht, p.states = states, p.maps = maps;
   p.offsets = offsets, p.indices = indices, p.chunk_offsets = chunk_offsets;
@@ -231,7 +231,7 @@ extern "C" int fla_hgrn_fwd(const void* x, const void* g, const float* lower_bou
 extern "C" int fla_hgrn_step(const void* x, const void* g, const float* lower_bound, const float* h0, void* o, float* ht, int gates,
                              int x_dtype, int g_dtype, int64_t N, int64_t D, int64_t ldx, int64_t ldg, fla_stream_t stream) {
   FLA_REQUIRE(x && g && o && N > 0 && D > 0 && ldx >= D && ldg >= D && (!lower_bound || gates), FLA_E_INVALID);
-  FLA_REQUIRE(ldx <= FLA_HGRN_MAX_PITCH && ldg <= FLA_HGRN_MAX_PITCH && N <= 0x7fffffff / fla_cdiv(D, VEC) , FLA_E_UNSUPPORTED);
+  FLA_REQUIRE(ldx <= FLA_HGRN_MAX_PITCH && ldg <= FLA_HGRN_MAX_PITCH && N <= 0x7fffffff / fla_cdiv(D, VEC), FLA_E_UNSUPPORTED);
   const StepParams p{x, g, lower_bound, h0, o, ht, N, ldx, ldg, (int)D};
   const bool wide = wide_rows(x, ldx, D, x_dtype) && wide_rows(g, ldg, D, g_dtype) && wide_rows(o, D, D, x_dtype);
   const int kind = !gates ? kLogDecays : lower_bound ? kBoundedGates : kGates;

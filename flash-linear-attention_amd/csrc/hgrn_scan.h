@@ -210,6 +210,7 @@ FLA_DEVICE float onto(float A, float H, float h) { return fmaf(A, h, H); }
   D(FLA_BF16, bf16, FLA_BF16, bf16) D(FLA_BF16, bf16, FLA_F32, float) D(FLA_F16, f16, FLA_F16, f16) \
   D(FLA_F16, f16, FLA_F32, float) D(FLA_F32, float, FLA_F32, float)
 
+constexpr int64_t kMostWorkgroups = 0xffffffff / (kWaves * 64);   // (a launch is less than 2^32 threads)
 // whether rows ld apart can be read 16 bytes at a time
 inline bool wide_rows(const void* p, int64_t ld, int64_t D, int type) {
   const int64_t e = type == FLA_F32 ? 4 : 2;

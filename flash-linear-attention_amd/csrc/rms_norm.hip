@@ -252,7 +252,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_bwd_kernel(RmsParam
   else if (N <= 128) CALL(16, 1)                   \
   else if (N <= 256) CALL(32, 1)                   \
   else if (N <= 512) CALL(64, 1)                   \
-  else if (N <= 2048 && p.M <= kFewRows) CALL(256, 1) \
+  else if (N <= 2048 && all.M <= kFewRows) CALL(256, 1) \
   else if (N <= 1024) CALL(64, 2)                  \
   else if (N <= 2048) CALL(64, 4)                  \
   else if (N <= 4096) CALL(256, 2)                 \
@@ -273,17 +273,36 @@ constexpr int64_t kMaxN = 512 * 4 * VEC;
 constexpr int64_t kBwdWorkgroups = 1024;
 int bwd_rows_per_block(int64_t N) { return N <= 64 ? 32 : N <= 128 ? 16 : N <= 256 ? 8 : N <= 512 ? 4 : 1; }
 
+constexpr int64_t kLaunchRows = 1 << 22;   // of a forward launch: one is less than 2^32 threads
+
+// the `rows` rows from number `row` on
+template <typename T, bool QUANT>
+RmsParams rows_from(const RmsParams& all, int64_t row, int64_t rows) {
+  RmsParams p = all;
+  const int64_t at = row * p.N;
+  p.x = (const T*)p.x + at;
+  if (p.res) p.res = (const char*)p.res + at * (p.res_f32 ? 4 : sizeof(T));
+  if (p.res_out) p.res_out = (char*)p.res_out + at * (p.res_out_f32 ? 4 : sizeof(T));
+  p.y = (char*)p.y + at * (QUANT ? 1 : sizeof(T));
+  if (p.scale) p.scale += row;
+  if (p.rstd) p.rstd += row;
+  p.M = rows;
+  return p;
+}
 template <typename T, bool WIDE, bool QUANT>
-int launch_fwd(const RmsParams& p, hipStream_t st) {
-  const int N = p.N;
+int launch_fwd(const RmsParams& all, hipStream_t st) {
+  const int N = all.N;
+  for (int64_t row = 0; row < all.M; row += kLaunchRows) {
+    const RmsParams p = rows_from<T, QUANT>(all, row, all.M - row < kLaunchRows ? all.M - row : kLaunchRows);
 #define CALL(TPR, NP)                                                                                                             \
   {                                                                                                                               \
     constexpr int block = TPR > 256 ? TPR : 256;                                                                                  \
     hipLaunchKernelGGL((rms_fwd_kernel<T, TPR, NP, WIDE, QUANT>), dim3((unsigned)fla_cdiv(p.M, block / TPR)), dim3(block), 0, st, p); \
   }
-  RMS_FWD_SHAPES(CALL)
+    RMS_FWD_SHAPES(CALL)
 #undef CALL
-  FLA_CHECK_LAUNCH();
+    FLA_CHECK_LAUNCH();
+  }
   return FLA_OK;
 }
 template <typename T, typename KT, bool WIDE>

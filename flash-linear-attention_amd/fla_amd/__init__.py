@@ -26,9 +26,9 @@ def install() -> list:
         'l2_norm', 'l2norm_fwd', 'l2norm_bwd', 'L2NormFunction', 'FusedRMSNormSwishGate', 'FusedLayerNormSwishGate',
         'rms_norm_swish_gate_fn', 'layer_norm_swish_gate_fn', 'LayerNormSwishGateFn', 'ShortConvolution')})
     targets = ['fla.ops.gla', 'fla.ops.gated_delta_rule', 'fla.ops.delta_rule', 'fla.ops.simple_gla', 'fla.ops.hgrn',
-               'fla.ops.utils', 'fla.ops', 'fla.layers.gla', 'fla.layers.gated_deltanet', 'fla.layers.hgrn', 'fla.layers.hgrn2', 'fla.layers.delta_net',
-               'fla.layers.simple_gla', 'fla.modules', 'fla.modules.l2norm', 'fla.modules.fused_norm_gate',
-               'fla.modules.convolution']
+               'fla.ops.utils', 'fla.ops', 'fla.layers.gla', 'fla.layers.gated_deltanet', 'fla.layers.hgrn', 'fla.layers.hgrn2',
+               'fla.layers.delta_net', 'fla.layers.simple_gla', 'fla.modules', 'fla.modules.l2norm',
+               'fla.modules.fused_norm_gate', 'fla.modules.convolution']
     for modname in targets:
         try:
             mod = importlib.import_module(modname)

@@ -55,6 +55,16 @@ class QuantLinear(nn.Module):
             new.bias = linear.bias.detach().clone()
         return new
 
+    def _apply(self, fn, recurse=True):
+        # module.to(dtype) and its like are for the bias; rows in 8 bits and their scales follow to another device, never into another type
+        rows = self.weight, self.weight_scale
+        super()._apply(fn, recurse)
+        if self.weight.dtype != rows[0].dtype:
+            self.weight = rows[0].to(self.weight.device)
+        if self.weight_scale.dtype != rows[1].dtype:
+            self.weight_scale = rows[1].to(self.weight_scale.device)
+        return self
+
     def extra_repr(self) -> str:
         return f"{self.in_features}, {self.out_features}, bias={self.bias is not None}, activation={self.activation}"
 

@@ -246,6 +246,10 @@ def test_no_tokens(device):
     assert torch.equal(torch.autograd.grad(ht.sum(), h0)[0], torch.ones_like(h0))
     o, ht = chunk_hgrn(x, x, output_final_state=True)
     assert not ht.any() and ht.shape == (2, 16)
+    x, g = x.clone().requires_grad_(), x.bfloat16().requires_grad_()
+    o, _ = chunk_hgrn(x, g)
+    o.sum().backward()
+    assert o.dtype == x.dtype and x.grad.shape == x.shape and g.grad.shape == x.shape
 
 
 def test_only_some_gradients_arrive(device):

@@ -172,3 +172,15 @@ def test_captured_and_two_streams(device):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, want) and torch.equal(other, want), (M, k)
+
+
+def test_module_in_another_type(device):
+    """module.to(dtype) is for the bias alone"""
+    from fla_amd.modules import QuantLinear
+    layer = QuantLinear.from_linear(torch.nn.Linear(64, 48).to(device))
+    weight, scale = layer.weight.clone(), layer.weight_scale.clone()
+    layer = torch.nn.Sequential(layer).half()[0]
+    assert layer.bias.dtype == HF and layer.weight.dtype == F8 and layer.weight_scale.dtype == FL
+    assert torch.equal(layer.weight.view(torch.uint8), weight.view(torch.uint8)) and torch.equal(layer.weight_scale, scale)
+    assert layer(torch.randn(3, 64, device=device)).shape == (3, 48)
+    assert layer.cpu().weight.device.type == "cpu" and layer.weight.dtype == F8

@@ -200,3 +200,38 @@ def test_captured_and_other_streams(device):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(want, out)), k
+
+
+def test_more_rows_than_a_launch_takes(device):
+    from fla_amd.modules import rms_norm
+    M, N = (1 << 22) + 5, 8
+    gen = torch.Generator(device=device).manual_seed(1)
+    x, r = torch.randn(M, N, generator=gen, device=device).bfloat16(), torch.randn(M, N, generator=gen, device=device)
+    w = torch.randn(N, generator=gen, device=device)
+    with torch.no_grad():
+        (q, scale), s = rms_norm(x, w, None, r, prenorm=True, quantize=True)
+        y, _ = rms_norm(x, w, None, r, prenorm=True)
+        for rows in (slice(0, 40), slice(M - 45, M)):
+            (q1, scale1), s1 = rms_norm(x[rows], w, None, r[rows], prenorm=True, quantize=True)
+            assert torch.equal(q[rows].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(scale[rows], scale1) and torch.equal(s[rows], s1)
+            assert torch.equal(y[rows], rms_norm(x[rows], w, None, r[rows]))
+    x, r = x.requires_grad_(), r.requires_grad_()
+    dy = torch.randn(M, N, generator=gen, device=device).bfloat16()
+    dx, dr = torch.autograd.grad(rms_norm(x, w, None, r), (x, r), dy)
+    rows = slice(M - 45, M)
+    a, b = x[rows].detach().requires_grad_(), r[rows].detach().requires_grad_()
+    da, db = torch.autograd.grad(rms_norm(a, w, None, b), (a, b), dy[rows])
+    assert torch.equal(dx[rows], da) and torch.equal(dr[rows], db)
+
+
+def test_one_tensor_twice(device):
+    from fla_amd.modules import rms_norm
+    x = torch.randn(7, 264, generator=torch.Generator().manual_seed(2)).to(device).requires_grad_()
+    y, s = rms_norm(x, None, None, x, prenorm=True)
+    got, = torch.autograd.grad((y.square().sum() + s.sum()), x)
+    z = x.detach().double().requires_grad_()
+    t = 2 * z
+    want, = torch.autograd.grad((t * torch.rsqrt(t.square().mean(-1, keepdim=True) + 1e-6)).square().sum() + t.sum(), z)
+    # The sum of y^2 is N up to eps, so its gradient (dy - y mean(dy y)) rstd is a difference of two equal terms of at most 2 * 5 * 0.6.  Each is off by
+    # less than 16 roundings of fp32 (the mean's sum in 3 + 6 levels, rstd, products), both twice (x and residual): 4 * 6 * 16 * 2^-24.  The rest is 2.
+    assert (got.double() - want).abs().max() <= 4 * 6 * 16 * 2.0 ** -24 + 2.0 ** -22

@@ -92,6 +92,7 @@ def test_library_arguments():
     assert fwd(T=300) == -1                                   # cut, and no workspace
     assert fwd(N=2) == -1 and fwd(ldx=4) == -1 and fwd(T=0) == -1 and fwd(lb=p) == -1
     assert fwd(types=(1, 2)) == -2
+    assert fwd(B=1 << 23, N=1 << 23, T=1) == -2               # more workgroups than a launch takes
     bwd = lambda states, dlb=None: lib.fla_hgrn_bwd(p, p, None, states, None, None, p, p, None, dlb, None, None, None, None, 0, 256, 0, 0, 0,
                                                     1, 8, 8, 1, 8, 8, None)
     assert bwd(None) == -1 and bwd(p, p) == -1
