@@ -404,6 +404,7 @@ int launch_panel(const LinearParams& p, hipStream_t st) {
 //   200 x 16384 x 2048    7.8           21.2  34    45                  16.2        30
 //   256 x 4096 x 4096     3.9           14.6  18.3  20.8  24.7          18.5        50
 //   1000 x 4096 x 4096    5.6           32    43    62                  24.1        51
+//   8191 x 8192 x 2048   32.5 (115 at the rate of 8192^3)               176         149 (1.84 PFLOP/s; 8192^3: 2.45)
 enum LinearKind { kPanel, kTile64, kTile128x64, kTile256 };
 struct LinearPlan {
   LinearKind kind;
