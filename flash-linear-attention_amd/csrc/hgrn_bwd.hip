@@ -10,7 +10,8 @@
 namespace {
 
 // OUT: writes the gradients; otherwise the map of the segment.  A lane holds six values an element for the second half of a tile, 2 x 8 elements take
-// all 256 registers: R = 4 does not fit.
+// all 256 registers: R = 4 does not fit, and joining both directions side by side, which hides one's shuffles behind the other's, spills (227 us
+// instead of 188; in 206 registers, with log decays, it takes as long as one after the other).
 template <typename T, typename GT, int GATES, bool WIDE, bool OUT>
 __global__ __launch_bounds__(kWaves * 64) void hgrn_bwd_kernel(HgrnParams p) {
   constexpr int R = 2, kSpan = kGroups * R, kTile = kWaves * kSpan;   // rows of a lane, a wave, the workgroup
