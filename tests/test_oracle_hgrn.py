@@ -98,3 +98,23 @@ def test_library_arguments():
     assert bwd(None) == -1 and bwd(p, p) == -1
     assert lib.fla_hgrn_step(p, p, None, None, p, None, 0, 1, 2, 1, 8, 8, 8, None) == -2
     assert lib.fla_hgrn_step(p, p, None, None, p, None, 0, 0, 0, 1, 8, 4, 8, None) == -1
+
+
+def test_install_rebinds_the_recurrence(monkeypatch):
+    """``fla_amd.install()`` on stub modules: the package's names and those that the layer bound at import."""
+    import sys
+    import types
+    import fla_amd
+    from fla_amd.ops import hgrn
+    names = ("chunk_hgrn", "fused_recurrent_hgrn")
+    mods = {}
+    for name in ("fla", "fla.ops", "fla.ops.hgrn", "fla.layers", "fla.layers.hgrn"):
+        mods[name] = types.ModuleType(name)
+        mods[name].__path__ = []
+        monkeypatch.setitem(sys.modules, name, mods[name])
+    for name in ("fla.ops.hgrn", "fla.layers.hgrn"):
+        for n in names:
+            setattr(mods[name], n, object())
+    patched = fla_amd.install()
+    assert {f"{m}.{n}" for m in ("fla.ops.hgrn", "fla.layers.hgrn") for n in names} == set(patched)
+    assert all(getattr(mods[m], n) is getattr(hgrn, n) for m in ("fla.ops.hgrn", "fla.layers.hgrn") for n in names)
