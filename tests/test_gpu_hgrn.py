@@ -338,3 +338,31 @@ def test_long_rows_pass_32_bits(device):
         o, _ = chunk_hgrn(wide[..., :D], wide[..., :D], use_gate_in_kernel=True)
     ho, _, eo, _ = oracle.forward(x, x, gates=True)
     _check("o", o, ho, eo)
+
+
+def test_packed_batch_captured(device):
+    """A packed training step, cut into segments, as a graph: the tables of its offsets are there since an eager step."""
+    from fla_amd.ops.hgrn import chunk_hgrn
+    ends = [0, 1, 701, 701, 2201, 2264]
+    x, g, h0, lb, offs, do, dht = [t.to(device) for t in _inputs(1, ends[-1], 40, HF, FL, True, True, True, ends)]
+    leaves = [t.requires_grad_() for t in (x, g, h0, lb)]
+
+    def train():
+        o, ht = chunk_hgrn(leaves[0], leaves[1], leaves[2], True, cu_seqlens=offs, use_gate_in_kernel=True, lower_bound=leaves[3])
+        return [o.detach(), ht.detach(), *torch.autograd.grad((o, ht), leaves, (do, dht))]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        train()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = train()
+    for k in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn(x.shape, generator=torch.Generator().manual_seed(k)))
+        want = train()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, out)), k

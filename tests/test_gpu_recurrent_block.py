@@ -159,3 +159,19 @@ def test_a_training_step_in_a_graph(device):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(want, out)), k
+
+
+def test_tangents_are_refused(device):
+    """None of the three has a forward-mode derivative: an operand with a tangent raises, also where no gradient is asked for."""
+    import torch.autograd.forward_ad as fwd
+    from fla_amd.modules import quant_linear, quantize_rows, rms_norm
+    from fla_amd.ops.hgrn import chunk_hgrn, fused_recurrent_hgrn
+    x = torch.randn(1, 6, 32, device=device)
+    w = quantize_rows(x[0])
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad), fwd.dual_level():
+            dual = fwd.make_dual(x, torch.ones_like(x))
+            for call in (lambda: chunk_hgrn(dual, x), lambda: fused_recurrent_hgrn(x[:, :1], dual[:, :1]), lambda: rms_norm(dual, None),
+                         lambda: quantize_rows(dual), lambda: quant_linear(w, w, residual=dual[0, :, :6])):
+                with pytest.raises(RuntimeError):
+                    call()
