@@ -56,7 +56,7 @@ FLA_DEVICE float row_reduce(float v, float (*lds)[TPR > 64 ? TPR / 64 : 1], int 
     v = MAX ? fmaxf(v, o) : v + o;
   }
   if (TPR > 64) {
-    if ((threadIdx.x & 63) == 0) lds[turn][threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) lds[turn][threadIdx.x % TPR >> 6] = v;
     lds_barrier();
     v = lds[turn][0];
 #pragma unroll
@@ -143,12 +143,16 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_fwd_kernel(RmsParam
   }
 }
 
+// Threads of a backward's workgroup: four rows of 256 threads or two of 512, so that their column sums meet in LDS and a quarter of the partial
+// sums is left for the launch that adds them (16384 x 2048: 4 us instead of 8.4); several passes of 512 threads need the registers of two workgroups.
+constexpr int bwd_block(int tpr, int passes) { return tpr <= 64 ? 256 : passes > 1 ? tpr : 1024; }
+
 // Rows are walked so that the column sums of the weight gradients stay in registers and leave once per workgroup.  The operands of the next
 // row are on their way while one is worked on.
 template <typename T, typename KT, int TPR, int NP, bool WIDE, bool BIAS>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_bwd_kernel(RmsParams p) {
-  constexpr int BLOCK = TPR > 256 ? TPR : 256, RPB = BLOCK / TPR;
-  __shared__ float lds[2][TPR > 64 ? TPR / 64 : 1];
+__global__ __launch_bounds__(bwd_block(TPR, NP)) void rms_bwd_kernel(RmsParams p) {
+  constexpr int BLOCK = bwd_block(TPR, NP), RPB = BLOCK / TPR;
+  __shared__ float lds[RPB][2][TPR > 64 ? TPR / 64 : 1];
   __shared__ float sum[RPB > 1 ? RPB : 1][RPB > 1 ? TPR * VEC : 1];
   const int sub = threadIdx.x % TPR, rl = threadIdx.x / TPR, N = p.N;
   float dw[NP][VEC], db[NP][VEC];
@@ -202,7 +206,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_bwd_kernel(RmsParam
         c = fmaf(d[q][i], s[q][i], c);
       }
     }
-    c = row_reduce<TPR, false>(c, lds, turn) * inv;
+    c = row_reduce<TPR, false>(c, lds[rl], turn) * inv;
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
       const int col = (q * TPR + sub) * VEC, valid = row < p.M ? N - col : 0;
@@ -270,8 +274,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_bwd_kernel(RmsParam
 
 constexpr int64_t kFewRows = 1024;
 constexpr int64_t kMaxN = 512 * 4 * VEC;
-constexpr int64_t kBwdWorkgroups = 1024;
-int bwd_rows_per_block(int64_t N) { return N <= 64 ? 32 : N <= 128 ? 16 : N <= 256 ? 8 : N <= 512 ? 4 : 1; }
+int bwd_rows_per_block(int64_t N) { return N <= 64 ? 32 : N <= 128 ? 16 : N <= 256 ? 8 : N <= 2048 ? 4 : N <= 4096 ? 2 : 1; }
+// as many workgroups as are on the chip at once: 16 waves a CU
+int64_t bwd_workgroups(int64_t N) { return N <= 512 ? 1024 : N <= 4096 ? 256 : 1024; }
 
 constexpr int64_t kLaunchRows = 1 << 22;   // of a forward launch: one is less than 2^32 threads
 
@@ -310,7 +315,7 @@ int launch_bwd(const RmsParams& p, int grid, hipStream_t st) {
   const int N = p.N;
 #define CALL(TPR, NP)                                                                                                                       \
   {                                                                                                                                         \
-    constexpr int block = TPR > 256 ? TPR : 256;                                                                                            \
+    constexpr int block = bwd_block(TPR, NP);                                                                                               \
     if (p.db_part) hipLaunchKernelGGL((rms_bwd_kernel<T, KT, TPR, NP, WIDE, true>), dim3(grid), dim3(block), 0, st, p);                     \
     else hipLaunchKernelGGL((rms_bwd_kernel<T, KT, TPR, NP, WIDE, false>), dim3(grid), dim3(block), 0, st, p);                              \
   }
@@ -360,7 +365,8 @@ extern "C" int fla_rms_norm_fwd(const void* x, const void* residual, int residua
 extern "C" int fla_rms_norm_workgroups(int64_t M, int64_t N) {
   if (M <= 0 || N <= 0) return 1;
   const int64_t g = fla_cdiv(M, bwd_rows_per_block(N));
-  return (int)(g < kBwdWorkgroups ? g : kBwdWorkgroups);
+  const int64_t most = bwd_workgroups(N);
+  return (int)(g < most ? g : most);
 }
 
 extern "C" int fla_rms_norm_bwd(const void* dy, const void* kept, int kept_dtype, const void* weight, int weight_dtype, const float* rstd,
