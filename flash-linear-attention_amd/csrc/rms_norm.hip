@@ -143,15 +143,15 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_fwd_kernel(RmsParam
   }
 }
 
-// Threads of a backward's workgroup: four rows of 256 threads or two of 512, so that their column sums meet in LDS and a quarter of the partial
-// sums is left for the launch that adds them (16384 x 2048: 4 us instead of 8.4); several passes of 512 threads need the registers of two workgroups.
-constexpr int bwd_block(int tpr, int passes) { return tpr <= 64 ? 256 : passes > 1 ? tpr : 1024; }
+// Threads of a backward's workgroup: as many rows as 1024 threads hold where a row has waves of its own, so that their column sums meet in LDS and
+// few partial sums are left for the launch that adds them (16384 x 2048: 4 us instead of 8.4 from workgroups of one row).
+constexpr int bwd_block(int tpr) { return tpr <= 64 ? 256 : 1024; }
 
 // Rows are walked so that the column sums of the weight gradients stay in registers and leave once per workgroup.  The operands of the next
 // row are on their way while one is worked on.
 template <typename T, typename KT, int TPR, int NP, bool WIDE, bool BIAS>
-__global__ __launch_bounds__(bwd_block(TPR, NP)) void rms_bwd_kernel(RmsParams p) {
-  constexpr int BLOCK = bwd_block(TPR, NP), RPB = BLOCK / TPR;
+__global__ __launch_bounds__(bwd_block(TPR)) void rms_bwd_kernel(RmsParams p) {
+  constexpr int BLOCK = bwd_block(TPR), RPB = BLOCK / TPR;
   __shared__ float lds[RPB][2][TPR > 64 ? TPR / 64 : 1];
   __shared__ float sum[RPB > 1 ? RPB : 1][RPB > 1 ? TPR * VEC : 1];
   const int sub = threadIdx.x % TPR, rl = threadIdx.x / TPR, N = p.N;
@@ -177,10 +177,12 @@ __global__ __launch_bounds__(bwd_block(TPR, NP)) void rms_bwd_kernel(RmsParams p
       if (p.dres) nr[q] = load_raw8<KT, WIDE>((const KT*)p.dres + row * N + col, valid);
     }
   };
-  fetch((int64_t)blockIdx.x * RPB + rl);
+  constexpr bool AHEAD = NP == 1;   // (the registers of two passes do not hold a second row)
+  if (AHEAD) fetch((int64_t)blockIdx.x * RPB + rl);
   // every thread makes as many rounds: rows of several waves exchange through a barrier
   for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < p.M; row0 += step, turn ^= 1) {
     const int64_t row = row0 + rl;
+    if (!AHEAD) fetch(row);
     float s[NP][VEC], d[NP][VEC];
     typename Row8<KT>::raw r8[NP];
     const float rstd = nrstd;
@@ -190,7 +192,7 @@ __global__ __launch_bounds__(bwd_block(TPR, NP)) void rms_bwd_kernel(RmsParams p
       Row8<T>::unpack(nd[q], d[q]);
       r8[q] = nr[q];
     }
-    fetch(row + step);
+    if (AHEAD) fetch(row + step);
     float c = 0.f;
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
@@ -248,9 +250,10 @@ __global__ __launch_bounds__(bwd_block(TPR, NP)) void rms_bwd_kernel(RmsParams p
 }
 
 // (threads to a row, passes) by the row's length.  Forward: a wave to a row up to 2048 elements (16384 rows in 54 us, 4.95 TB/s), but four
-// waves where there are few rows (32 rows of 2048 to 8 bits: 4.1 us, with one wave 5.5).  Backward: rows of one pass as long as there are
+// waves where there are few rows (32 rows of 2048 to 8 bits: 4.0 us, with one wave 5.5).  Backward: rows of one pass as long as there are
 // threads, since the column sums and the next row's operands take registers (16384 rows of 2048: 54 us; with four passes of a wave 75 us,
-// 80 with the next row's operands in flight).
+// 80 with the next row's operands in flight), and the least threads that hold them: 2^25 elements with the weight's gradient take 51 - 55 us (the bytes: 52)
+// in rows of 64 to 16384, up to 63 where a quarter of the threads is idle (1024 in 256 threads: 67; 8192 in two passes of 512: 74, 16384 in four: 112).
 #define RMS_FWD_SHAPES(CALL)                       \
   if (N <= 64) CALL(8, 1)                          \
   else if (N <= 128) CALL(16, 1)                   \
@@ -262,21 +265,24 @@ __global__ __launch_bounds__(bwd_block(TPR, NP)) void rms_bwd_kernel(RmsParams p
   else if (N <= 4096) CALL(256, 2)                 \
   else if (N <= 8192) CALL(256, 4)                 \
   else CALL(512, 4)
-#define RMS_BWD_SHAPES(CALL)      \
-  if (N <= 64) CALL(8, 1)         \
-  else if (N <= 128) CALL(16, 1)  \
-  else if (N <= 256) CALL(32, 1)  \
-  else if (N <= 512) CALL(64, 1)  \
+#define RMS_BWD_SHAPES(CALL)       \
+  if (N <= 64) CALL(8, 1)          \
+  else if (N <= 128) CALL(16, 1)   \
+  else if (N <= 256) CALL(32, 1)   \
+  else if (N <= 512) CALL(64, 1)   \
+  else if (N <= 1024) CALL(128, 1) \
   else if (N <= 2048) CALL(256, 1) \
   else if (N <= 4096) CALL(512, 1) \
-  else if (N <= 8192) CALL(512, 2) \
-  else CALL(512, 4)
+  else if (N <= 8192) CALL(1024, 1) \
+  else CALL(1024, 2)
 
 constexpr int64_t kFewRows = 1024;
 constexpr int64_t kMaxN = 512 * 4 * VEC;
-int bwd_rows_per_block(int64_t N) { return N <= 64 ? 32 : N <= 128 ? 16 : N <= 256 ? 8 : N <= 2048 ? 4 : N <= 4096 ? 2 : 1; }
+int bwd_rows_per_block(int64_t N) {
+  return N <= 64 ? 32 : N <= 128 ? 16 : N <= 256 ? 8 : N <= 512 ? 4 : N <= 1024 ? 8 : N <= 2048 ? 4 : N <= 4096 ? 2 : 1;
+}
 // as many workgroups as are on the chip at once: 16 waves a CU
-int64_t bwd_workgroups(int64_t N) { return N <= 512 ? 1024 : N <= 4096 ? 256 : 1024; }
+int64_t bwd_workgroups(int64_t N) { return N <= 512 ? 1024 : 256; }
 
 constexpr int64_t kLaunchRows = 1 << 22;   // of a forward launch: one is less than 2^32 threads
 
@@ -315,7 +321,7 @@ int launch_bwd(const RmsParams& p, int grid, hipStream_t st) {
   const int N = p.N;
 #define CALL(TPR, NP)                                                                                                                       \
   {                                                                                                                                         \
-    constexpr int block = bwd_block(TPR, NP);                                                                                               \
+    constexpr int block = bwd_block(TPR);                                                                                               \
     if (p.db_part) hipLaunchKernelGGL((rms_bwd_kernel<T, KT, TPR, NP, WIDE, true>), dim3(grid), dim3(block), 0, st, p);                     \
     else hipLaunchKernelGGL((rms_bwd_kernel<T, KT, TPR, NP, WIDE, false>), dim3(grid), dim3(block), 0, st, p);                              \
   }

@@ -32,7 +32,7 @@ CASES = [  # M, N, type, residual, weight, bias
     (3, 65, FL, FL, FL, True), (100, 200, BF, FL, BF, False), (9, 512, HF, HF, HF, False), (1027, 1000, BF, BF, BF, False),
     (10, 1001, HF, FL, HF, True), (4100, 2048, BF, BF, BF, False), (6, 2050, BF, BF, None, False), (2, 4096, FL, None, FL, False),
     (1030, 4104, BF, FL, FL, True), (3, 8192, BF, None, BF, True), (1100, 1800, HF, HF, HF, True), (7, 777, BF, FL, BF, False), (5, 3001, FL, FL, None, False), (2, 8193, HF, HF, FL, False), (1025, 16384, BF, BF, BF, False),
-    (3, 16383, FL, FL, FL, True),
+    (3, 16383, FL, FL, FL, True), (1100, 3000, BF, FL, BF, True),
 ]
 
 
