@@ -3,8 +3,8 @@
 
 namespace {
 
-// OUT: writes o (and ht, states); otherwise the map of the segment.  R = 4 rows a lane where every CU has one workgroup all the same, R = 2 in cut
-// sequences, whose workgroups share CUs (107 registers instead of 161 - 203).  Whole tiles have no branch around their loads and stores: a
+// OUT: writes o (and ht, states); otherwise the map of the segment.  R = 4 rows a lane in long whole sequences, R = 2 in cut and short ones, whose
+// workgroups share CUs (107 registers instead of 161 - 203).  Whole tiles have no branch around their loads and stores: a
 // training step of 8 x 4096 x 2048 takes 262 us instead of 312.
 template <typename T, typename GT, int GATES, bool WIDE, bool OUT, int R>
 __global__ __launch_bounds__(kWaves * 64) void hgrn_fwd_kernel(HgrnParams p) {
@@ -173,7 +173,13 @@ int launch_fwd(const HgrnParams& p, int64_t segments, int64_t empty, hipStream_t
     FLA_CHECK_LAUNCH();
     return FLA_OK;
   }
-  hipLaunchKernelGGL((hgrn_fwd_kernel<T, GT, GATES, WIDE, true, 4>), dim3((unsigned)((segments + empty) * p.ncb)), dim3(kWaves * 64), 0, st, p);
+  // Uncut.  Short sequences leave less of a tile of 128 rows empty than of one of 256, and two workgroups share a CU if there are that many (us, 2048
+  // channels, R = 2 and 4): 256 x 128 tokens 96 and 185, 64 x 300 58 and 89, 64 x 512 87 and 97; 6 x 4096 87 and 77, 16 x 2048 102 and 96.
+  const int64_t grid = (segments + empty) * p.ncb;
+  if (p.segment <= 1024 && grid > 256)
+    hipLaunchKernelGGL((hgrn_fwd_kernel<T, GT, GATES, WIDE, true, 2>), dim3((unsigned)grid), dim3(kWaves * 64), 0, st, p);
+  else
+    hipLaunchKernelGGL((hgrn_fwd_kernel<T, GT, GATES, WIDE, true, 4>), dim3((unsigned)grid), dim3(kWaves * 64), 0, st, p);
   FLA_CHECK_LAUNCH();
   return FLA_OK;
 }
@@ -190,10 +196,11 @@ int launch_step(const StepParams& p, hipStream_t st) {
 extern "C" int64_t fla_hgrn_segment(int64_t n_seqs, int64_t tokens, int64_t longest, int64_t D) {
   if (n_seqs <= 0 || tokens <= 0 || longest <= 0 || D <= 0) return FLA_HGRN_TILE;
   const int64_t cbs = fla_cdiv(D, kCh), whole = fla_cdiv(longest, FLA_HGRN_TILE) * FLA_HGRN_TILE;
-  // Whole sequences where they give every CU work of about the same length; otherwise four workgroups a CU, at most 64 segments to a
+  // Whole sequences where all of them are as much work as 144 chains of the longest side by side (us forward / backward, 4096 tokens of 2048 channels, whole
+  // and cut: 4 sequences, 128 chains, 70 / 147 and 79 / 125; 5: 69 / 149 and 105 / 161); otherwise four workgroups a CU, at most 64 segments to a
   // sequence (a workgroup joins the maps of all segments ahead of its own).  8191 tokens of 2048 channels: 47 us from 512 workgroups on,
   // 55 with 256; 12 sequences of 16384 tokens in all, 1000 channels, both ways: 151, 144, 144 us with 512, 1024, 2048.
-  if (n_seqs * cbs >= 192 && longest * n_seqs <= 2 * tokens) return whole;
+  if (tokens * cbs >= 144 * longest) return whole;
   int64_t seg = fla_cdiv(fla_cdiv(tokens * cbs, 1024), FLA_HGRN_TILE) * FLA_HGRN_TILE;
   const int64_t least = fla_cdiv(fla_cdiv(longest, 64), FLA_HGRN_TILE) * FLA_HGRN_TILE;
   if (seg < least) seg = least;

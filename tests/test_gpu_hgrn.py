@@ -75,6 +75,7 @@ CASES = [
     (1, 1030, 67, FL, FL, True, True, True, None),        # five segments, odd channels
     (1, 770, 128, HF, FL, True, True, True, None),
     (200, 300, 64, BF, BF, True, True, True, None),       # a workgroup for every CU: whole sequences, two tiles each
+    (260, 130, 72, HF, FL, True, True, True, None),       # short sequences that share CUs
     (1, 600, 96, BF, BF, True, True, True, [0, 1, 1, 300, 317, 600]),          # an empty sequence, one of a single token
     (1, 900, 30, HF, FL, False, False, True, [5, 40, 40, 40, 850]),            # rows outside, empty ones, segments
     (1, 64, 64, FL, FL, False, False, True, [0, 0, 0]),                        # no sequence has a token
