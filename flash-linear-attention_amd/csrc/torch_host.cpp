@@ -214,6 +214,7 @@ bool chunk_operands(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
   if (v.size(0) != d->B || v.size(1) != d->T || v.size(2) != d->H) return false;
   if ((d->K != 64 && d->K != 128) || (d->V != 64 && d->V != 128)) return false;
   if (plan && d->B != 1) return false;
+  TORCH_CHECK_VALUE(!plan || plan->offsets.device() == q.device(), "fla_amd: offsets on ", plan->offsets.device(), ", the operands on ", q.device());
   d->N = plan ? plan->N : d->B;
   const int64_t per = (d->T + BT - 1) / BT;
   d->NT = plan ? plan->NT : 0;
@@ -1142,6 +1143,8 @@ PyObject* py_hgrn(PyObject*, PyObject* const* p, Py_ssize_t n) {
                     a.D, "]");
   TORCH_CHECK_VALUE(!a.plan || (a.plan->host.front() >= 0 && a.plan->host.back() <= a.T), "fla_amd hgrn: offsets leave the ", a.T, " rows");
   need_gpu({&x, &g, &lb, &h0});
+  TORCH_CHECK_VALUE(!a.plan || a.plan->offsets.device() == x.device(), "fla_amd: offsets on ", a.plan->offsets.device(),
+                    ", the operands on ", x.device());
   const bool grad = wants_grad({&x, &g, &lb, &h0});
   if (inplace) {
     TORCH_CHECK_VALUE(h0.defined() && a.want_ht && h0.scalar_type() == at::kFloat && h0.is_contiguous(),

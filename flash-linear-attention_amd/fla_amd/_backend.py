@@ -157,9 +157,11 @@ def dt(t: torch.Tensor) -> int:
 
 
 def ptr(t: Optional[torch.Tensor]):
-    """Device (or host) address of a contiguous tensor, or NULL."""
+    """Device address of a contiguous tensor, or NULL.  A host address would fault in the kernel: it is refused here."""
     if t is None:
         return None
+    if not t.is_cuda:
+        raise RuntimeError("fla_amd: the HIP kernels need tensors on a GPU device; there is no CPU fallback")
     assert t.is_contiguous(), "fla_amd: tensors crossing the C ABI must be contiguous"
     return c_void_p(t.data_ptr())
 

@@ -6,7 +6,7 @@ from typing import Optional
 import torch
 
 from ... import _backend as be
-from ...utils import VarlenPlan
+from ...utils import VarlenPlan, check_offsets_device
 
 
 def chunk_local_cumsum(
@@ -24,6 +24,7 @@ def chunk_local_cumsum(
                          f"which should be (B, H, T, dim) if `head_first=True` "
                          f"or (batch_size, num_heads, seq_len) otherwise")
     assert chunk_size == 2 ** (chunk_size.bit_length() - 1), "chunk_size must be a power of 2"
+    check_offsets_device(g, offsets)
     be.require_gpu(g)
     if head_first:
         # the kernels are seq-first; head-first is served by a transpose
@@ -58,6 +59,7 @@ def chunk_local_cumsum_inverse(
     """The raw values whose ``chunk_local_cumsum`` is ``g_cumsum`` (fp32): differences of consecutive rows
     inside every chunk (``fla_chunk_local_cumsum_inverse``).  No counterpart in the reference, whose internal
     entry points take the cumulative gates as they are; the kernels here start from the raw gates."""
+    check_offsets_device(g_cumsum, offsets)
     be.require_gpu(g_cumsum)
     if head_first:
         out = chunk_local_cumsum_inverse(g_cumsum.transpose(1, 2), chunk_size, reverse, offsets, indices, head_first=False)
@@ -95,6 +97,7 @@ def chunk_global_cumsum(
         raise ValueError(f"Unsupported input shape {s.shape}. "
                          f"which should be [B, H, T]/[B, H, T, D] if `head_first=True` "
                          f"or [B, T, H]/[B, T, H, D] otherwise")
+    check_offsets_device(s, offsets)
     be.require_gpu(s)
     if head_first:
         out = chunk_global_cumsum(s.transpose(1, 2), dtype, reverse, offsets, head_first=False)

@@ -155,6 +155,13 @@ def resolve_offsets(offsets: Optional[torch.Tensor], cu_seqlens: Optional[torch.
     return offsets if offsets is not None else cu_seqlens
 
 
+def check_offsets_device(x, offsets):
+    """Kernels read the boundaries and the tables made from them beside the operands: on another device (a ``cu_seqlens`` left on
+    the host) they would be addresses of that device."""
+    if isinstance(offsets, torch.Tensor) and offsets.device != x.device:
+        raise ValueError(f"fla_amd: offsets on {offsets.device}, the operands on {x.device}")
+
+
 def check_varlen_args(q, offsets, head_first, initial_state):
     """Error behaviour of the reference entry points
     (``fla/ops/gla/chunk.py:1483-1491`` and the identical blocks elsewhere)."""
@@ -167,6 +174,7 @@ def check_varlen_args(q, offsets, head_first, initial_state):
         if initial_state is not None and initial_state.shape[0] != len(offsets) - 1:
             raise ValueError(f"The number of initial states is expected to be equal to the number of input sequences, "
                              f"i.e., {len(offsets) - 1} rather than {initial_state.shape[0]}.")
+        check_offsets_device(q, offsets)
 
 
 def empty_batch_result(q, v, offsets, initial_state, output_final_state):
