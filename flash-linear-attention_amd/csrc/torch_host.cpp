@@ -125,9 +125,8 @@ struct SplitTables {
   fla_split ints{};
   Tensor tables;   // seg_table, sub_table and sub_base, one behind the other
 };
-// The device tables of a packed batch, made once per offsets tensor by fla_amd.utils.VarlenPlan.  `offsets` is the caller's
-// own tensor where it is int64: a node saves it, so that a backward after it has been written to is refused instead of
-// combining the other tables, made from the old boundaries, with the new ones.
+// The device tables of a packed batch, made once per offsets tensor by fla_amd.utils.VarlenPlan, `offsets` a copy among them.  (A node
+// saves the caller's own tensor beside them, so that a backward after it has been written to is refused.)
 struct Plan : torch::CustomClassHolder {
   Tensor offsets, indices, chunk_offsets, seq_order;
   std::vector<int64_t> host;
@@ -136,6 +135,13 @@ struct Plan : torch::CustomClassHolder {
   std::map<std::tuple<int64_t, int, bool, int>, SplitTables> splits;
 
   bool covers(int64_t begin, int64_t end) const { return !host.empty() && host.front() == begin && host.back() == end; }
+
+  // The boundaries and tables share one allocation; it belongs to the stream that uploaded it.  (Tensors of this build call
+  // their device CUDA.)
+  void used() const {
+    const auto stream = c10::hip::getCurrentHIPStream(offsets.device().index());
+    offsets.record_stream(c10::Stream(c10::Stream::UNSAFE, offsets.device(), stream.id()));
+  }
 
   // The tables of a cut are used by later calls on any stream.  A stream that is being captured takes no copy: a call whose
   // tables are not there yet runs uncut under it.
@@ -173,7 +179,12 @@ struct Plan : torch::CustomClassHolder {
 };
 using PlanPtr = c10::intrusive_ptr<Plan>;
 
-const int64_t* offs(const PlanPtr& p) { return p ? (const int64_t*)p->offsets.data_ptr() : nullptr; }
+// Every launch that reads a plan takes its boundaries from here: the plan may be dropped while this stream still reads it.
+const int64_t* offs(const PlanPtr& p) {
+  if (!p) return nullptr;
+  p->used();
+  return (const int64_t*)p->offsets.data_ptr();
+}
 const int64_t* idx(const PlanPtr& p) { return p ? (const int64_t*)p->indices.data_ptr() : nullptr; }
 const int64_t* coff(const PlanPtr& p) { return p ? (const int64_t*)p->chunk_offsets.data_ptr() : nullptr; }
 const int64_t* order(const PlanPtr& p) { return p ? (const int64_t*)p->seq_order.data_ptr() : nullptr; }

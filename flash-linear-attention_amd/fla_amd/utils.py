@@ -41,8 +41,15 @@ autocast_custom_bwd = functools.partial(torch.amp.custom_bwd, device_type="cuda"
 
 # Host copies of device-resident offsets, keyed by tensor identity: a model passes the same
 # cu_seqlens tensor to every layer, and reading it back costs a device synchronisation.
-# An entry is valid only for the very same, unmodified tensor object.
+# An entry is valid only for the very same, unmodified tensor object, and goes with it.
 _HOST_OFFSETS_CACHE = {}
+
+
+def _refuse_under_capture(offsets):
+    """A capture takes no copy in either direction, and one recorded into it would not have run when an eager call meets the tables."""
+    if offsets.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("fla_amd: the tables of these offsets are not on the device yet, and a stream that is being captured takes "
+                           "no copy: run the call once ahead of the capture")
 
 
 def _host_offsets(offsets) -> Tuple[int, ...]:
@@ -54,10 +61,9 @@ def _host_offsets(offsets) -> Tuple[int, ...]:
         ref, version, host = hit
         if ref() is offsets and version == offsets._version:
             return host
+    _refuse_under_capture(offsets)
     host = tuple(int(x) for x in offsets.detach().cpu().tolist())
-    if len(_HOST_OFFSETS_CACHE) > 256:
-        _HOST_OFFSETS_CACHE.clear()
-    _HOST_OFFSETS_CACHE[key] = (weakref.ref(offsets), offsets._version, host)
+    _HOST_OFFSETS_CACHE[key] = (weakref.ref(offsets, lambda _: _HOST_OFFSETS_CACHE.pop(key, None)), offsets._version, host)
     return host
 
 
@@ -95,10 +101,29 @@ def prepare_chunk_offsets(offsets, chunk_size: int, device=None) -> torch.Tensor
     return co.to(device) if device is not None else co.clone()
 
 
+_UPLOADS = {}    # a stream per device
+
+
+def _upload(tensor: torch.Tensor, device: torch.device) -> torch.Tensor:
+    """``tensor`` on ``device``, there for any stream from now on: copied on a stream of its own and waited for there, while the
+    streams that compute go on.  The memory belongs to that stream: readers call ``record_stream``."""
+    stream = _UPLOADS.get(device.index)
+    if stream is None:
+        stream = _UPLOADS.setdefault(device.index, torch.cuda.Stream(device))
+    pinned = tensor.pin_memory()
+    with torch.cuda.stream(stream):
+        out = pinned.to(device, non_blocking=True)
+    stream.synchronize()
+    return out
+
+
 class VarlenPlan:
     """Everything the kernels need to address a packed batch.  Plans are cached per offsets
     tensor (same object, unmodified), so the layers of a model that share one ``cu_seqlens``
-    build the device tables once."""
+    build the device tables once, and live as long as that tensor does.
+
+    The boundaries are copied with the tables: calls on any stream read both, complete before the plan is handed out, and each
+    use is recorded on its stream, so that a plan that is dropped does not give its memory away under a launch that reads it."""
 
     _cache = {}
 
@@ -111,35 +136,41 @@ class VarlenPlan:
                 return plan
         plan = super().__new__(cls)
         plan._build(offsets, chunk_size)
-        if len(cls._cache) > 256:
-            cls._cache.clear()
-        cls._cache[key] = (weakref.ref(offsets), offsets._version, plan)
+        cls._cache[key] = (weakref.ref(offsets, lambda _: cls._cache.pop(key, None)), offsets._version, plan)
         return plan
 
     def _build(self, offsets: torch.Tensor, chunk_size: int):
-        host = _host_offsets(offsets)
-        idx, co = _chunk_tables(host, int(chunk_size))
-        dev = offsets.device
-        self.offsets = offsets.to(torch.int64).contiguous()
-        self.indices = idx.to(dev, non_blocking=True)
-        self.chunk_offsets = co.to(dev, non_blocking=True)
-        self.N = len(host) - 1
-        self._host, self._native = host, None
-        self.NT = idx.shape[0]
+        _refuse_under_capture(offsets)
+        bounds = _host_offsets(offsets)
+        idx, co = _chunk_tables(bounds, int(chunk_size))
+        self.N, self.NT, self._host, self._native = len(bounds) - 1, idx.shape[0], bounds, None
         # sequence ids, longest first: the order in which the serial scan kernels start sequences
-        lens = [host[i + 1] - host[i] for i in range(self.N)]
-        order = sorted(range(self.N), key=lambda i: -lens[i])
-        self.seq_order = torch.tensor(order, dtype=torch.int64).to(dev, non_blocking=True)
+        order = sorted(range(self.N), key=lambda i: bounds[i] - bounds[i + 1])
+        tables = torch.cat([idx.flatten(), co, torch.tensor(order, dtype=torch.int64), torch.tensor(bounds, dtype=torch.int64)])
+        if offsets.is_cuda:
+            tables = _upload(tables, offsets.device)
+        idx, self._chunk_offsets, self._seq_order, self._offsets = tables.split([idx.numel(), self.N + 1, self.N, self.N + 1])
+        self._indices = idx.view(-1, 2)
+
+    def _used(self, table: torch.Tensor) -> torch.Tensor:
+        if table.is_cuda:
+            table.record_stream(torch.cuda.current_stream(table.device))
+        return table
+
+    offsets = property(lambda self: self._used(self._offsets))
+    indices = property(lambda self: self._used(self._indices))
+    chunk_offsets = property(lambda self: self._used(self._chunk_offsets))
+    seq_order = property(lambda self: self._used(self._seq_order))
 
     def covers(self, begin: int, end: int) -> bool:
         return self._host[0] == begin and self._host[-1] == end
 
     @property
     def native(self):
-        """The plan as the host extension takes it."""
+        """The plan as the host extension takes it (which records its uses itself)."""
         if self._native is None:
             from ._native import host
-            self._native = host().plan(self.offsets, self.indices, self.chunk_offsets, self.seq_order,
+            self._native = host().plan(self._offsets, self._indices, self._chunk_offsets, self._seq_order,
                                        torch.tensor(self._host, dtype=torch.int64))
         return self._native
 
