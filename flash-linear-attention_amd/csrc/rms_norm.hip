@@ -121,15 +121,15 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_fwd_kernel(RmsParam
   if (QUANT) {
     const float scale = fmaxf(row_reduce<TPR, true>(amax, lds, 1), kAmaxMin) / kE4M3Max;
     if (sub == 0) p.scale[row] = scale;
-    const float inv = 1.f / scale;
+    // (divided, as the scale is defined: a product with its rounded reciprocal moves values next to a border of the 8-bit type)
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
       const int col = (q * TPR + sub) * VEC, valid = N - col;
       int pk[2] = {0, 0};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        pk[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[q][4 * h] * inv, v[q][4 * h + 1] * inv, pk[h], false);
-        pk[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[q][4 * h + 2] * inv, v[q][4 * h + 3] * inv, pk[h], true);
+        pk[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[q][4 * h] / scale, v[q][4 * h + 1] / scale, pk[h], false);
+        pk[h] = __builtin_amdgcn_cvt_pk_fp8_f32(v[q][4 * h + 2] / scale, v[q][4 * h + 3] / scale, pk[h], true);
       }
       uint8_t* at = (uint8_t*)p.y + row * N + col;
       if (WIDE) {
