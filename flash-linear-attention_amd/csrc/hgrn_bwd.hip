@@ -202,6 +202,7 @@ extern "C" int fla_hgrn_bwd(const void* x, const void* g, const float* lower_bou
   FLA_REQUIRE(x && g && states && dx && dg && B > 0 && T > 0 && D > 0 && N > 0 && NT >= 0 && ldx >= D && ldg >= D, FLA_E_INVALID);
   FLA_REQUIRE(segment > 0 && segment % FLA_HGRN_TILE == 0 && (!lower_bound || gates) && (!dlb_partials || lower_bound), FLA_E_INVALID);
   FLA_REQUIRE(offsets ? B == 1 && (indices || NT == 0) && chunk_offsets : N == B, FLA_E_INVALID);
+  FLA_REQUIRE((uintptr_t)states % 16 == 0, FLA_E_ALIGNMENT);
   const int64_t nseg = fla_cdiv(T, segment), cbs = fla_cdiv(D, kCh), segments = offsets ? NT : B * nseg;
   FLA_REQUIRE(maps || offsets || nseg == 1, FLA_E_INVALID);
   FLA_REQUIRE(ldx <= FLA_HGRN_MAX_PITCH && ldg <= FLA_HGRN_MAX_PITCH && segments + N <= kMostWorkgroups / cbs, FLA_E_UNSUPPORTED);

@@ -381,6 +381,7 @@ extern "C" int fla_rms_norm_bwd(const void* dy, const void* kept, int kept_dtype
   FLA_REQUIRE(dy && kept && rstd && dx && M >= 0 && N > 0, FLA_E_INVALID);
   FLA_REQUIRE(N <= kMaxN && M <= 0x7fffffffLL && type_ok(kept_dtype, dtype), FLA_E_UNSUPPORTED);
   FLA_REQUIRE(!weight || type_ok(weight_dtype, dtype), FLA_E_UNSUPPORTED);
+  FLA_REQUIRE(((uintptr_t)dw_partial | (uintptr_t)db_partial) % 16 == 0, FLA_E_ALIGNMENT);
   if (M == 0) return FLA_OK;
   RmsParams p{};
   p.x = kept, p.w = weight, p.rstd = (float*)rstd, p.dy = dy, p.dres = dresidual, p.dx = dx, p.dres_in = dresidual_in;

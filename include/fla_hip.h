@@ -809,7 +809,7 @@ int fla_gdn_gate_bwd(const void* a, const void* b, const float* A_log, const flo
  * fla_hgrn_segment: tokens of a segment (a multiple of FLA_HGRN_TILE) for n_seqs sequences of `tokens` in all, the longest
  * `longest`; `longest` or more: sequences are not cut (host arithmetic).  Sequences of more than one segment need the workspace
  * maps, fp32 [segments, 2, D] (segments: NT, or B times those of a sequence).
- * states: fp32 [B*T / FLA_HGRN_STATE_ROWS + N + 1, D] or NULL, kept by a forward for its backward.
+ * states: fp32 [B*T / FLA_HGRN_STATE_ROWS + N + 1, D] at a 16-byte address or NULL, kept by a forward for its backward.
  * dlb_partials: fp32 [segments, D] or NULL, its column sums are the gradient of lb (segments: as above).
  * fla_hgrn_step: one token for each of N sequences, x, g, o [N, D]; ht may be h0. */
 #define FLA_HGRN_TILE 256
@@ -837,7 +837,8 @@ int fla_hgrn_step(const void* x, const void* g, const float* lower_bound, const 
  * normalise == 0: y = s (8-bit rows of s itself; no weight, bias or rstd).
  * Backward: kept is what the forward normalised (x, or residual_out) in kept_dtype; dresidual, the gradient that arrived for
  * residual_out (in kept_dtype, or NULL), is added to dx; dresidual_in (in kept_dtype, or NULL) receives a copy of dx.  dw_partial,
- * db_partial: fp32 [fla_rms_norm_workgroups(M, N), N] or NULL, their column sums are the gradients of weight and bias. */
+ * db_partial: fp32 [fla_rms_norm_workgroups(M, N), N] at 16-byte addresses or NULL, their column sums are the gradients of weight
+ * and bias. */
 int fla_rms_norm_workgroups(int64_t M, int64_t N);
 int fla_rms_norm_fwd(const void* x, const void* residual, int residual_dtype, const void* weight, const void* bias,
                      int weight_dtype, void* y, float* scale, void* residual_out, int residual_out_dtype, float* rstd, int64_t M,
