@@ -1204,8 +1204,9 @@ PyObject* py_rms_norm(PyObject*, PyObject* const* p, Py_ssize_t n) {
   const bool prenorm = arg_bool(p[5]), in_f32 = arg_bool(p[6]);
   a.quantize = arg_bool(p[7]);
   a.normalise = arg_bool(p[8]);
-  TORCH_CHECK_VALUE(x.defined() && x.dim() >= 1 && x.size(-1) > 0, "fla_amd rms_norm: x is [..., N], N at least 1");
-  TORCH_CHECK_TYPE(floating(x), "fla_amd rms_norm: x in bf16, fp16 or fp32, not ", x.scalar_type());
+  const char* who = a.normalise ? "fla_amd rms_norm" : "fla_amd quantize_rows";
+  TORCH_CHECK_VALUE(x.defined() && x.dim() >= 1 && x.size(-1) > 0, who, ": x is [..., N], N at least 1");
+  TORCH_CHECK_TYPE(floating(x), who, ": x in bf16, fp16 or fp32, not ", x.scalar_type());
   const int64_t N = x.size(-1);
   for (const Tensor* t : {&w, &b}) {
     if (!t->defined()) continue;
@@ -1217,7 +1218,8 @@ PyObject* py_rms_norm(PyObject*, PyObject* const* p, Py_ssize_t n) {
     TORCH_CHECK_TYPE(res.scalar_type() == x.scalar_type() || res.scalar_type() == at::kFloat,
                      "fla_amd rms_norm: the residual is in x's type or in fp32");
   }
-  TORCH_CHECK_NOT_IMPLEMENTED(N <= 16384, "fla_amd rms_norm: rows of at most 16384 elements, not ", N);
+  const int64_t most = a.normalise ? 16384 : 1 << 23;
+  TORCH_CHECK_NOT_IMPLEMENTED(N <= most, who, ": rows of at most ", most, " elements, not ", N);
   need_gpu({&x, &w, &b, &res});
   const bool grad = wants_grad({&x, &w, &b, &res});
   TORCH_CHECK(!(grad && a.quantize), "fla_amd: rows in 8 bits have no gradient; call it under torch.no_grad()");
@@ -1267,7 +1269,8 @@ PyObject* py_quant_linear(PyObject*, PyObject* const* p, Py_ssize_t n) {
   const int64_t K = x.size(-1), N = w.size(0);
   TORCH_CHECK_VALUE(sx.sizes() == x.sizes().slice(0, x.dim() - 1) && sw.dim() == 1 && sw.size(0) == N,
                     "fla_amd quant_linear: one scale for every row of x and of weight");
-  TORCH_CHECK_NOT_IMPLEMENTED(K > 0 && K % 16 == 0, "fla_amd quant_linear: rows of a multiple of 16 elements, not ", K);
+  TORCH_CHECK_NOT_IMPLEMENTED(K > 0 && K % 16 == 0 && K <= 1 << 23,
+                              "fla_amd quant_linear: rows of a multiple of 16 elements, at most 2^23, not ", K);
   if (bias.defined()) {
     TORCH_CHECK_VALUE(bias.dim() == 1 && bias.size(0) == N, "fla_amd quant_linear: bias holds ", N, " values");
     TORCH_CHECK_TYPE(bias.is_floating_point(), "fla_amd quant_linear: bias in a floating type");

@@ -20,7 +20,8 @@ def rms_norm(x, weight, bias=None, residual=None, prenorm=False, residual_in_fp3
 
 
 def quantize_rows(x):
-    """``(q, scale)`` of the rows of ``x``: ``q`` in ``torch.float8_e4m3fn``, ``scale = max(max|x|, 1e-30) / 448`` in fp32 for each row."""
+    """``(q, scale)`` of the rows of ``x``: ``q`` in ``torch.float8_e4m3fn``, ``scale = max(max|x|, 1e-30) / 448`` in fp32 for each row.
+    Rows of at most 2^23 elements, as many as :func:`quant_linear` takes."""
     return host().rms_norm(x, None, None, None, 0.0, False, False, True, False)
 
 

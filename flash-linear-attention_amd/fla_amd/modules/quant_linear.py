@@ -21,7 +21,7 @@ def quant_linear(x: Rows, weight: Rows, bias: Optional[torch.Tensor] = None, act
 
     ``activation``: ``None``, ``"silu"`` (``"swish"``), ``"gelu"`` (of the error function) or ``"relu"``; ``residual`` ``[..., N]`` and ``bias`` in the
     output's type or in fp32; ``output_dtype`` bf16 or fp16 (the matrix instruction's sums of 8-bit products hold about 16 bits, fp32
-    results are refused).  ``K`` in multiples of 16.  Sums in fp32; one launch.  There is no gradient, and a call that wants one is refused."""
+    results are refused).  ``K`` in multiples of 16, at most 2^23.  Sums in fp32; one launch.  There is no gradient, and a call that wants one is refused."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"fla_amd quant_linear: unknown activation {activation!r}")
     if output_dtype not in (torch.bfloat16, torch.float16):
@@ -31,13 +31,15 @@ def quant_linear(x: Rows, weight: Rows, bias: Optional[torch.Tensor] = None, act
 
 class QuantLinear(nn.Module):
     """A ``torch.nn.Linear`` for serving with its weight in 8 bits: ``forward(x, residual=None)`` takes 16-bit or fp32 rows, which it quantises first,
-    or the pair that a norm with ``quantize=True`` returned."""
+    or the pair that a norm with ``quantize=True`` returned.  ``in_features`` in multiples of 16, at most 2^23."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, activation: Optional[str] = None,
                  output_dtype: torch.dtype = torch.bfloat16, device=None):
         super().__init__()
         if activation not in _ACTIVATIONS:
             raise ValueError(f"fla_amd quant_linear: unknown activation {activation!r}")
+        if in_features <= 0 or in_features % 16 or in_features > 1 << 23:
+            raise NotImplementedError(f"fla_amd quant_linear: rows of a multiple of 16 elements, at most 2^23, not {in_features}")
         self.in_features, self.out_features, self.activation, self.output_dtype = in_features, out_features, activation, output_dtype
         self.register_buffer("weight", torch.zeros(out_features, in_features, device=device).to(torch.float8_e4m3fn))
         self.register_buffer("weight_scale", torch.zeros(out_features, device=device))

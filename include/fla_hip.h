@@ -834,7 +834,7 @@ int fla_hgrn_step(const void* x, const void* g, const float* lower_bound, const 
  * residual_out, kept, dresidual, dresidual_in [M,N] in `dtype` or fp32; weight, bias [N] in `dtype` or fp32 (one type for both).
  * residual, weight, bias, residual_out (receives s), rstd (fp32 [M], for the backward) may be NULL.
  * scale (fp32 [M]) not NULL: y receives rows in 8 bits, e4m3 (finite up to 448): scale = max(max|y|, 1e-30) / 448, y / scale.
- * normalise == 0: y = s (8-bit rows of s itself; no weight, bias or rstd).
+ * normalise == 0: y = s (8-bit rows of s itself; no weight, bias or rstd); without residual and residual_out N <= 2^23.
  * Backward: kept is what the forward normalised (x, or residual_out) in kept_dtype; dresidual, the gradient that arrived for
  * residual_out (in kept_dtype, or NULL), is added to dx; dresidual_in (in kept_dtype, or NULL) receives a copy of dx.  dw_partial,
  * db_partial: fp32 [fla_rms_norm_workgroups(M, N), N] at 16-byte addresses or NULL, their column sums are the gradients of weight
