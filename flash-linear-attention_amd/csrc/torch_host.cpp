@@ -77,6 +77,9 @@ bool on_gpu(std::initializer_list<const Tensor*> ts) {
 // grads in the dtype of the operand they belong to
 Tensor as(const Tensor& g, at::ScalarType type) { return g.scalar_type() == type ? g : g.to(type); }
 
+// Whether an operand of a node has a gradient: those of frozen weights are not formed
+bool asks(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
 // An operand that may be absent, as a node takes it
 using Maybe = std::optional<Tensor>;
 Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
@@ -696,7 +699,7 @@ Tensor hgrn_forward(const Tensor& x_, const Tensor& g_, const Tensor& lb, const 
 struct HgrnNode : torch::autograd::Function<HgrnNode> {
   struct Rest {
     HgrnArgs a;
-    bool has_h0;
+    bool lb, h0;     // whether they have a gradient
   };
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& g, const Maybe& lb_, const Maybe& h0_,
                                const Maybe& offsets, const HgrnArgs& a) {
@@ -706,7 +709,7 @@ struct HgrnNode : torch::autograd::Function<HgrnNode> {
     Tensor o = hgrn_forward(x, g, lb, h0, a, &ht, &states);
     ctx->save_for_backward({x, g, lb, states, given(offsets)});
     ctx->set_materialize_grads(false);
-    hold(ctx, Rest{a, h0.defined()});
+    hold(ctx, Rest{a, asks(lb), asks(h0)});
     return a.want_ht ? variable_list{o, ht} : variable_list{o};
   }
 
@@ -722,16 +725,16 @@ struct HgrnNode : torch::autograd::Function<HgrnNode> {
     const Tensor dout = grads[0].defined() ? as(grads[0], x.scalar_type()).contiguous() : Tensor();
     const Tensor dht = a.want_ht ? f32(grads[1]) : Tensor();
     Tensor dx = a.rows(x), dg = a.rows(g), maps = a.maps(x);
-    Tensor dh0 = r.has_h0 ? fresh({a.N, a.D}, x, at::kFloat) : Tensor();
+    Tensor dh0 = r.h0 ? fresh({a.N, a.D}, x, at::kFloat) : Tensor();
     const int64_t segments = a.segments();
-    Tensor part = lb.defined() && segments > 0 ? fresh({segments, a.D}, x, at::kFloat) : Tensor();
+    Tensor part = r.lb && segments > 0 ? fresh({segments, a.D}, x, at::kFloat) : Tensor();
     check(fla_hgrn_bwd(ptr(x), ptr(g), fptr(lb), fptr(states), ptr(dout), fptr(dht), ptr(dx), ptr(dg), fptr(dh0), fptr(part), fptr(maps),
                        offs(a.plan), idx(a.plan), coff(a.plan), a.plan ? a.plan->NT : 0, a.segment, a.gates, dt(x), dt(g), a.B, a.T, a.D,
                        a.N, ldx, ldg, stream_of(x)),
           "fla_hgrn_bwd");
     Tensor dlb;
     if (part.defined()) dlb = sum_partials(part, {a.D}, at::kFloat);
-    else if (lb.defined()) dlb = at::zeros({a.D}, x.options().dtype(at::kFloat));
+    else if (r.lb) dlb = at::zeros({a.D}, x.options().dtype(at::kFloat));
     return {dx, dg, dlb, dh0, Tensor(), Tensor()};
   }
 };
@@ -764,7 +767,7 @@ RmsOut rms_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tens
 
 struct RmsNode : torch::autograd::Function<RmsNode> {
   struct Rest {
-    bool w, b, res;
+    bool w, b, res;  // whether they have a gradient
     at::ScalarType type;
   };
   static variable_list forward(AutogradContext* ctx, const Tensor& x_, const Maybe& w_, const Maybe& b_, const Maybe& res_, const RmsArgs& a) {
@@ -773,7 +776,7 @@ struct RmsNode : torch::autograd::Function<RmsNode> {
     RmsOut o = rms_forward(x, w, b, res, a, true);
     ctx->save_for_backward({o.kept.defined() ? o.kept : x, w, b, o.rstd});
     ctx->set_materialize_grads(false);
-    hold(ctx, Rest{w.defined(), b.defined(), res.defined(), x.scalar_type()});
+    hold(ctx, Rest{asks(w), asks(b), res_ && asks(*res_), x.scalar_type()});
     return o.kept.defined() ? variable_list{o.y, o.kept} : variable_list{o.y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
