@@ -1192,6 +1192,8 @@ PyObject* py_hgrn(PyObject*, PyObject* const* p, Py_ssize_t n) {
   if (direct) ht = h0;
   Tensor o = hgrn_forward(x, g, lb, h0, a, &ht, nullptr);
   if (inplace && !direct) ht = h0.copy_(ht);
+  // written to: a node that saved the state before refuses its backward (inference tensors have no version)
+  if (inplace && !h0.is_inference()) h0.unsafeGetTensorImpl()->bump_version();
   return pair(o, ht);
   END_HANDLE_TH_ERRORS
 }
