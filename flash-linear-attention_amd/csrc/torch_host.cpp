@@ -1170,7 +1170,8 @@ PyObject* py_hgrn(PyObject*, PyObject* const* p, Py_ssize_t n) {
   if (lb.defined()) lb = f32(lb).reshape({a.D});
   if (h0.defined()) h0 = f32(h0);
   if (x.numel() == 0 || a.N == 0) {   // no token: the states stay
-    Tensor o = grad && x.numel() == 0 ? (x * g).to(x.scalar_type()) : at::zeros(x.sizes(), x.options());   // (empty, of their graph)
+    Tensor o = grad && x.numel() == 0 ? (lb.defined() ? x * g * lb : x * g).to(x.scalar_type())   // (empty, of their graph)
+                                      : at::zeros(x.sizes(), x.options());
     Tensor ht;
     if (a.want_ht) ht = inplace ? h0 : h0.defined() ? h0.clone() : at::zeros({a.N, a.D}, x.options().dtype(at::kFloat));
     return pair(o, ht);
