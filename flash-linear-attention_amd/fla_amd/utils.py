@@ -52,6 +52,13 @@ def _refuse_under_capture(offsets):
                            "no copy: run the call once ahead of the capture")
 
 
+def _remember(cache, key, offsets, value):
+    """Keeps what was made from ``offsets`` until that tensor goes.  One made in inference mode has no version that would show a
+    change: what was made from it is made again by every call."""
+    if not offsets.is_inference():
+        cache[key] = (weakref.ref(offsets, lambda _, cache=cache, key=key: cache.pop(key, None)), offsets._version, value)
+
+
 def _host_offsets(offsets) -> Tuple[int, ...]:
     if not isinstance(offsets, torch.Tensor):
         return tuple(int(x) for x in offsets)
@@ -63,7 +70,7 @@ def _host_offsets(offsets) -> Tuple[int, ...]:
             return host
     _refuse_under_capture(offsets)
     host = tuple(int(x) for x in offsets.detach().cpu().tolist())
-    _HOST_OFFSETS_CACHE[key] = (weakref.ref(offsets, lambda _: _HOST_OFFSETS_CACHE.pop(key, None)), offsets._version, host)
+    _remember(_HOST_OFFSETS_CACHE, key, offsets, host)
     return host
 
 
@@ -136,7 +143,7 @@ class VarlenPlan:
                 return plan
         plan = super().__new__(cls)
         plan._build(offsets, chunk_size)
-        cls._cache[key] = (weakref.ref(offsets, lambda _: cls._cache.pop(key, None)), offsets._version, plan)
+        _remember(cls._cache, key, offsets, plan)
         return plan
 
     def _build(self, offsets: torch.Tensor, chunk_size: int):

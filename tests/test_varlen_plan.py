@@ -37,6 +37,35 @@ def test_tables():
     assert VarlenPlan(offs, 64).indices.tolist() == [[0, 0], [1, 0], [1, 1], [2, 0], [2, 1]]
 
 
+def test_offsets_made_in_inference_mode():
+    """They have no version that would show a change: their tables are made by every call."""
+    with torch.inference_mode():
+        offs = torch.tensor([0, 5, 9])
+        assert VarlenPlan(offs, 64).offsets.tolist() == [0, 5, 9]
+        offs[1] = 7
+        assert VarlenPlan(offs, 64).offsets.tolist() == [0, 7, 9]
+    assert (id(offs), 64) not in VarlenPlan._cache
+
+
+@pytest.mark.gpu
+def test_a_packed_call_in_inference_mode(device):
+    from fla_amd.ops.gla import chunk_gla
+    from fla_amd.ops.hgrn import chunk_hgrn
+    x = torch.randn(1, 600, 64, device=device).bfloat16()
+    q = x.view(1, 600, 1, 64)
+    gk = torch.nn.functional.logsigmoid(q.float())
+    bounds = [0, 300, 417, 600]
+    outside = torch.tensor(bounds, device=device)
+    want, ht = chunk_hgrn(x, x, output_final_state=True, cu_seqlens=outside, use_gate_in_kernel=True)
+    o, _ = chunk_gla(q, q, q, gk, cu_seqlens=outside, head_first=False)
+    with torch.inference_mode():
+        inside = torch.tensor(bounds, device=device)
+        for offs in (inside, outside):
+            got, gt = chunk_hgrn(x, x, output_final_state=True, cu_seqlens=offs, use_gate_in_kernel=True)
+            assert torch.equal(got, want) and torch.equal(gt, ht)
+            assert torch.equal(chunk_gla(q, q, q, gk, cu_seqlens=offs, head_first=False)[0], o)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("index_type", [torch.int64, torch.int32])
 def test_two_streams_share_the_tables(device, index_type):
