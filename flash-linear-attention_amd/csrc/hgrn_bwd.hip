@@ -10,8 +10,11 @@
 namespace {
 
 // OUT: writes the gradients; otherwise the map of the segment.  A lane holds six values an element for the second half of a tile, 2 x 8 elements take
-// all 256 registers: R = 4 does not fit, and joining both directions side by side, which hides one's shuffles behind the other's, spills (227 us
-// instead of 188; in 206 registers, with log decays, it takes as long as one after the other).
+// all 256 registers: R = 4 does not fit.  On wide rows with gates the results' launch spills in eight instances (registers, bytes of scratch a
+// lane): with a lower bound 14 (52) in 16 bits, 39 and 47 (136) with the gates in fp32, 119 (304) all in fp32; without one 1 (8) with the gates in
+// fp32, 71 (192) all in fp32.  Its time on 8 x 4096 x 2048 (us; bf16, fp16, bf16 with fp32 gates, fp32; the bytes 133, 133, 185, 263): with a bound 190, 168, 212,
+// 305; without 169, 162, 210, 278; log decays, which spill nowhere, 165, 156, 208, 280.  Joining both directions side by side, which hides one's shuffles
+// behind the other's, spills more (227 instead of 188 with a bound in bf16; in 206 registers, with log decays, it takes as long as one after the other).
 template <typename T, typename GT, int GATES, bool WIDE, bool OUT>
 __global__ __launch_bounds__(kWaves * 64) void hgrn_bwd_kernel(HgrnParams p) {
   constexpr int R = 2, kSpan = kGroups * R, kTile = kWaves * kSpan;   // rows of a lane, a wave, the workgroup

@@ -8,7 +8,7 @@
 // read as steps that change nothing: a log decay of 0, a forget gate of plus infinity, an input and a gradient of 0.
 //
 // Bounds and figures (bf16, us): 8 x 4096 x 2048 runs uncut, one workgroup a CU.  Log decays in fp32, forward: 114, 4.7 TB/s.  From pre-activations
-// with a lower bound: forward 95 - 105 with the states for the backward (4.0 - 4.4 TB/s), backward 169 - 197 (3.5 - 4.1 TB/s; the vector units are busy for
+// with a lower bound: forward 95 - 105 with the states for the backward (4.0 - 4.4 TB/s), backward 169 - 204 (3.4 - 4.1 TB/s; the vector units are busy for
 // two thirds of it, 51 instructions an element, the rest is latency that two waves a SIMD do not cover).  With gates in fp32 119 and 215, all in
 // fp32 171 and 305: 1.1 times the time of a copy of as many bytes.  32 channels to a workgroup, which leave half of every
 // 128-byte line to another one: forward 135 instead of 117; sixteen waves of half the rows: 121.

@@ -269,7 +269,8 @@ __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(PE
 // ------------------------------------------------------------------------------------------------ few rows
 // At most MT x 16 rows of x against 16 rows of w: the bytes of w bound it, and those of x out of L2 from 32 rows on.  The waves take slices of 128 bytes
 // of K in turn, each through RING pieces of LDS of its own, waiting for nobody until the sums are added.  (Operands loaded straight into the instruction's
-// registers meet 16 rows with every 16 lanes and pass 17 bytes a clock and CU, whole 128-byte pieces 50: 48 x 2048 x 8192 took 16.6 us, with copies 8.3.)
+// registers meet 16 rows with every 16 lanes and pass 17 bytes a clock and CU, whole 128-byte pieces 50: 48 x 2048 x 8192 took 16.6 us, with copies 8.3, w in the
+// last-level cache; out of HBM 11.2.)
 template <typename T, int MT, int WAVES, int RING>
 __global__ __launch_bounds__(WAVES * 64) void linear_panel_kernel(LinearParams p) {
   constexpr int BK = 128, ROWS = (MT + 1) * 16, COPIES = ROWS / 8;   // rows of x, then those of w
@@ -389,7 +390,10 @@ int launch_panel(const LinearParams& p, hipStream_t st) {
   FLA_CHECK_LAUNCH();
   return FLA_OK;
 }
-// Which kernel, and how many slices of K.  Measured (us, w out of HBM; M x N x K; the floor is the bytes'):
+// Which kernel, and how many slices of K.  Measured (us, in a captured graph, twelve sets of w or 600 MB of them in turn; M x N x K; the floor is the
+// bytes').  Twelve sets of at most 21 MB stay in the last-level cache, so w comes out of HBM in the rows with more than that only; out of HBM what
+// plan_linear takes needs 4.2 for 1 x 4096 x 2048, 11.2 for 48 x 2048 x 8192, 5.1 for 48 x 2048 x 2048, 15.9 for 100 x 2048 x 8192, 16.1 for 256 x 4096 x 4096,
+// 20.2 for 500 x 4096 x 4096 and 27.6 for 1000 x 4096 x 4096.
 //                       floor  panels  64 x 64 in 1, 2, 4, 8 slices   128 x 64   256 x 256
 //   1 x 16384 x 2048      6.5     8.7   10.1                            11.8        26
 //   16 x 16384 x 2048     6.6     8.5   10.2  13.1  15                  11.9        26

@@ -285,7 +285,9 @@ __global__ __launch_bounds__(bwd_block(TPR)) void rms_bwd_kernel(RmsParams p) {
 // waves where there are few rows (32 rows of 2048 to 8 bits: 4.0 us, with one wave 5.5).  Backward: rows of one pass as long as there are
 // threads, since the column sums and the next row's operands take registers (16384 rows of 2048: 54 us; with four passes of a wave 75 us,
 // 80 with the next row's operands in flight), and the least threads that hold them: 2^25 elements with the weight's gradient take 51 - 55 us (the bytes: 52)
-// in rows of 64 to 16384, up to 63 where a quarter of the threads is idle (1024 in 256 threads: 67; 8192 in two passes of 512: 74, 16384 in four: 112).
+// in rows of 64 to 16384, up to 63 where a quarter of the threads is idle (1024 in 256 threads: 67; 8192 in two passes of 512: 74, 16384 in four: 112).  The workgroups
+// of 1024 threads have 128 registers: above 8192 elements with a bias 12 - 74 of them are spilled, with an fp32 stream alone 2 - 8, and with a bias and
+// an fp32 stream 2 - 5 in rows of one pass from 1025 elements on; the others spill none.
 #define RMS_FWD_SHAPES(CALL)                       \
   if (N <= 64) CALL(8, 1)                          \
   else if (N <= 128) CALL(16, 1)                   \

@@ -807,7 +807,7 @@ int fla_gdn_gate_bwd(const void* a, const void* b, const float* A_log, const flo
  * are not written.  Any D; D and the row pitches in multiples of 16 bytes take the wide loads.
  *
  * fla_hgrn_segment: tokens of a segment (a multiple of FLA_HGRN_TILE) for n_seqs sequences of `tokens` in all, the longest
- * `longest`; `longest` or more: sequences are not cut (host arithmetic).  Sequences of more than one segment need the workspace
+ * `longest`; `longest` or more: sequences are not cut (host arithmetic; of n_seqs only whether it is positive counts).  Sequences of more than one segment need the workspace
  * maps, fp32 [segments, 2, D] (segments: NT, or B times those of a sequence).
  * states: fp32 [B*T / FLA_HGRN_STATE_ROWS + N + 1, D] at a 16-byte address or NULL, kept by a forward for its backward.
  * dlb_partials: fp32 [segments, D] or NULL, its column sums are the gradient of lb (segments: as above).
