@@ -385,6 +385,7 @@ int launch_tiles(const LinearParams& p, hipStream_t st) {
 template <typename T, int MT>
 int launch_panel(const LinearParams& p, hipStream_t st) {
   const int64_t grid = fla_cdiv(p.N, 16);
+  FLA_REQUIRE(grid < (int64_t)1 << 32 >> 8, FLA_E_UNSUPPORTED);   // (a launch is less than 2^32 threads)
   if (grid < 256) hipLaunchKernelGGL((linear_panel_kernel<T, MT, 8, 2>), dim3((unsigned)grid), dim3(512), 0, st, p);
   else hipLaunchKernelGGL((linear_panel_kernel<T, MT, 4, 2>), dim3((unsigned)grid), dim3(256), 0, st, p);
   FLA_CHECK_LAUNCH();
