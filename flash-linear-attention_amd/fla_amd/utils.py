@@ -130,19 +130,26 @@ class VarlenPlan:
     build the device tables once, and live as long as that tensor does.
 
     The boundaries are copied with the tables: calls on any stream read both, complete before the plan is handed out, and each
-    use is recorded on its stream, so that a plan that is dropped does not give its memory away under a launch that reads it."""
+    use is recorded on its stream, so that a plan that is dropped does not give its memory away under a launch that reads it.  A
+    plan that a capture has met stays for its replays (with the boundaries it was captured with) also where the offsets are
+    written to, as long as their tensor lives."""
 
     _cache = {}
 
     def __new__(cls, offsets: torch.Tensor, chunk_size: int):
         key = (id(offsets), int(chunk_size))
         hit = cls._cache.get(key)
+        before = None
         if hit is not None:
             ref, version, plan = hit
-            if ref() is offsets and version == offsets._version:
-                return plan
+            if ref() is offsets:
+                if version == offsets._version:
+                    plan._captured = plan._captured or (offsets.is_cuda and torch.cuda.is_current_stream_capturing())
+                    return plan
+                before = plan if plan._captured else plan._before
         plan = super().__new__(cls)
         plan._build(offsets, chunk_size)
+        plan._captured, plan._before = False, before
         _remember(cls._cache, key, offsets, plan)
         return plan
 

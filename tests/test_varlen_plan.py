@@ -1,5 +1,6 @@
 """The tables of packed batches: how long they live, and calls on several streams that share them."""
 import gc
+import weakref
 
 import pytest
 import torch
@@ -24,6 +25,23 @@ def test_a_plan_lives_as_long_as_its_offsets():
     del offs
     gc.collect()
     assert key not in VarlenPlan._cache and len(VarlenPlan._cache) == size - 1
+
+
+def test_a_captured_plan_outlives_a_change_of_its_offsets():
+    """Replays go on reading its tables; plans that no capture has met go with the boundaries they were made from."""
+    offs = torch.tensor([0, 5, 90])
+    plans = []
+    for captured in (False, True, False, True, False):
+        offs[1] += 1
+        plan = VarlenPlan(offs, 64)
+        plan._captured = captured           # (what a call under capture sets)
+        plans.append(weakref.ref(plan))
+    del plan
+    gc.collect()
+    assert [p() is not None for p in plans] == [False, True, False, True, True]
+    del offs
+    gc.collect()
+    assert not any(p() for p in plans)
 
 
 def test_tables():
@@ -133,3 +151,33 @@ def test_tables_first_met_under_capture_are_refused(device):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+def test_replays_behind_a_change_of_the_offsets(device):
+    """A graph goes on with the boundaries it was captured with; eager calls follow the offsets."""
+    from fla_amd.ops.hgrn import chunk_hgrn
+    x = torch.randn(1, 1500, 64, device=device).bfloat16()
+    bounds = [[0, 300, 1500], [0, 900, 1500]]
+    offs = torch.tensor(bounds[0], device=device)
+    call = lambda o: chunk_hgrn(x, x, cu_seqlens=o, use_gate_in_kernel=True)[0]
+    with torch.no_grad():
+        want = [call(torch.tensor(b, device=device)) for b in bounds]
+        assert not torch.equal(*want)
+        call(offs)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call(offs)
+        plans = [p for *_, p in VarlenPlan._cache.values() if p._captured]
+        assert len(plans) == 1
+        kept = weakref.ref(plans.pop())
+        for turn in range(3):
+            offs.copy_(torch.tensor(bounds[1 - turn % 2]))
+            gc.collect()
+            assert torch.equal(call(offs), want[1 - turn % 2]) and kept() is not None
+            others = [VarlenPlan(torch.tensor([0, n], device=device), 64).NT for n in (7, 70, 700)]
+            out.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert others == [1, 2, 11] and torch.equal(out, want[0])
