@@ -739,42 +739,54 @@ struct HgrnNode : torch::autograd::Function<HgrnNode> {
   }
 };
 
-// ---------------------------------------------------------------------------------------------------- RMS norm
-struct RmsArgs {
+// ---------------------------------------------------------------------------------------------------- RMS norm, layer norm
+enum NormKind { kRowsOnly, kRms, kLayer };
+struct NormArgs {
   double eps;
   std::optional<at::ScalarType> kept_type;   // of the sum x + residual; none: nothing is added and x itself is what is normalised
-  bool quantize, normalise;
+  long rows8;                                // FLA_ROWS_*
+  NormKind kind;
 };
-struct RmsOut {
-  Tensor y, scale, kept, rstd;
+struct NormOut {
+  Tensor y, scale, kept, mean, rstd;
 };
 // Any shape [..., N], contiguous operands
-RmsOut rms_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& res, const RmsArgs& a, bool want_rstd) {
+NormOut norm_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& res, const NormArgs& a, bool want_rstd) {
   const int64_t N = x.size(-1), M = x.numel() / N;
-  RmsOut o;
-  o.y = a.quantize ? fresh(x.sizes(), x, at::kFloat8_e4m3fn) : fresh_like(x);
-  if (a.quantize) o.scale = fresh(x.sizes().slice(0, x.dim() - 1), x, at::kFloat);
+  NormOut o;
+  o.y = a.rows8 ? fresh(x.sizes(), x, a.rows8 == FLA_ROWS_INT8 ? at::kChar : at::kFloat8_e4m3fn) : fresh_like(x);
+  if (a.rows8) o.scale = fresh(x.sizes().slice(0, x.dim() - 1), x, at::kFloat);
   if (a.kept_type) o.kept = fresh(x.sizes(), x, *a.kept_type);
   if (want_rstd) o.rstd = fresh({M}, x, at::kFloat);
+  if (want_rstd && a.kind == kLayer) o.mean = fresh({M}, x, at::kFloat);
   if (M == 0) return o;
   const Tensor& any_w = w.defined() ? w : b;
-  check(fla_rms_norm_fwd(ptr(x), ptr(res), res.defined() ? dt(res) : dt(x), ptr(w), ptr(b), any_w.defined() ? dt(any_w) : dt(x), ptr(o.y),
-                         fptr(o.scale), ptr(o.kept), o.kept.defined() ? dt(o.kept) : dt(x), fptr(o.rstd), M, N, (float)a.eps, a.normalise,
-                         dt(x), stream_of(x)),
-        "fla_rms_norm_fwd");
+  const int rt = res.defined() ? dt(res) : dt(x), wt = any_w.defined() ? dt(any_w) : dt(x), kt = o.kept.defined() ? dt(o.kept) : dt(x);
+  if (a.kind == kLayer)
+    check(fla_layer_norm_fwd(ptr(x), ptr(res), rt, ptr(w), ptr(b), wt, ptr(o.y), fptr(o.scale), ptr(o.kept), kt, fptr(o.mean), fptr(o.rstd), M,
+                             N, (float)a.eps, (int)a.rows8, dt(x), stream_of(x)),
+          "fla_layer_norm_fwd");
+  else if (a.rows8)
+    check(fla_rms_norm_rows8_fwd(ptr(x), ptr(res), rt, ptr(w), ptr(b), wt, ptr(o.y), fptr(o.scale), ptr(o.kept), kt, M, N, (float)a.eps,
+                                 a.kind == kRms, (int)a.rows8, dt(x), stream_of(x)),
+          "fla_rms_norm_rows8_fwd");
+  else
+    check(fla_rms_norm_fwd(ptr(x), ptr(res), rt, ptr(w), ptr(b), wt, ptr(o.y), nullptr, ptr(o.kept), kt, fptr(o.rstd), M, N, (float)a.eps, 1,
+                           dt(x), stream_of(x)),
+          "fla_rms_norm_fwd");
   return o;
 }
 
-struct RmsNode : torch::autograd::Function<RmsNode> {
+struct NormNode : torch::autograd::Function<NormNode> {
   struct Rest {
     bool w, b, res;  // whether they have a gradient
     at::ScalarType type;
   };
-  static variable_list forward(AutogradContext* ctx, const Tensor& x_, const Maybe& w_, const Maybe& b_, const Maybe& res_, const RmsArgs& a) {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x_, const Maybe& w_, const Maybe& b_, const Maybe& res_, const NormArgs& a) {
     at::AutoDispatchBelowADInplaceOrView guard;
     const Tensor x = x_.contiguous(), w = given(w_), b = given(b_), res = res_ ? res_->contiguous() : Tensor();
-    RmsOut o = rms_forward(x, w, b, res, a, true);
-    ctx->save_for_backward({o.kept.defined() ? o.kept : x, w, b, o.rstd});
+    NormOut o = norm_forward(x, w, b, res, a, true);
+    ctx->save_for_backward({o.kept.defined() ? o.kept : x, w, b, o.rstd, o.mean});
     ctx->set_materialize_grads(false);
     hold(ctx, Rest{asks(w), asks(b), res_ && asks(*res_), x.scalar_type()});
     return o.kept.defined() ? variable_list{o.y, o.kept} : variable_list{o.y};
@@ -782,7 +794,7 @@ struct RmsNode : torch::autograd::Function<RmsNode> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     at::AutoDispatchBelowADInplaceOrView guard;
     const auto saved = ctx->get_saved_variables();
-    const Tensor &kept = saved[0], &w = saved[1], &b = saved[2], &rstd = saved[3];
+    const Tensor &kept = saved[0], &w = saved[1], &b = saved[2], &rstd = saved[3], &mean = saved[4];
     const Rest& r = held<Rest>(ctx);
     c10::DeviceGuard on_device(kept.device());
     const int64_t N = kept.size(-1), M = kept.numel() / N;
@@ -793,11 +805,17 @@ struct RmsNode : torch::autograd::Function<RmsNode> {
     if (M == 0)
       return {dx, r.w ? at::zeros_like(w) : Tensor(), r.b ? at::zeros_like(b) : Tensor(), r.res ? (dres_in.defined() ? dres_in : dx) : Tensor(),
               Tensor()};
-    const int64_t parts = fla_rms_norm_workgroups(M, N);
+    const int64_t parts = mean.defined() ? fla_layer_norm_workgroups(M, N) : fla_rms_norm_workgroups(M, N);
     Tensor dw = r.w ? fresh({parts, N}, kept, at::kFloat) : Tensor(), db = r.b ? fresh({parts, N}, kept, at::kFloat) : Tensor();
-    check(fla_rms_norm_bwd(ptr(dy), ptr(kept), dt(kept), ptr(w), w.defined() ? dt(w) : dt(kept), fptr(rstd), ptr(dres), ptr(dx),
-                           ptr(dres_in), fptr(dw), fptr(db), M, N, dt(dx), stream_of(kept)),
-          "fla_rms_norm_bwd");
+    const int wt = w.defined() ? dt(w) : dt(kept);
+    if (mean.defined())
+      check(fla_layer_norm_bwd(ptr(dy), ptr(kept), dt(kept), ptr(w), wt, fptr(mean), fptr(rstd), ptr(dres), ptr(dx), ptr(dres_in), fptr(dw),
+                               fptr(db), M, N, dt(dx), stream_of(kept)),
+            "fla_layer_norm_bwd");
+    else
+      check(fla_rms_norm_bwd(ptr(dy), ptr(kept), dt(kept), ptr(w), wt, fptr(rstd), ptr(dres), ptr(dx), ptr(dres_in), fptr(dw), fptr(db), M, N,
+                             dt(dx), stream_of(kept)),
+            "fla_rms_norm_bwd");
     return {dx, r.w ? sum_partials(dw, w.sizes(), w.scalar_type()) : Tensor(), r.b ? sum_partials(db, b.sizes(), b.scalar_type()) : Tensor(),
             r.res ? (dres_in.defined() ? dres_in : dx) : Tensor(), Tensor()};
   }
@@ -813,6 +831,11 @@ bool arg_bool(PyObject* o) {
   const int r = PyObject_IsTrue(o);
   if (r < 0) throw python_error();
   return r != 0;
+}
+long arg_long(PyObject* o) {
+  const long r = PyLong_AsLong(o);
+  if (r == -1 && PyErr_Occurred()) throw python_error();
+  return r;
 }
 double arg_double(PyObject* o) {
   const double r = PyFloat_AsDouble(o);
@@ -1199,36 +1222,36 @@ PyObject* py_hgrn(PyObject*, PyObject* const* p, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// rms_norm(x, weight | None, bias | None, residual | None, eps, prenorm, residual_in_fp32, quantize, normalise)
+// norm(x, weight | None, bias | None, residual | None, eps, prenorm, residual_in_fp32, rows8, kind): rows8 FLA_ROWS_*, kind a NormKind
 //   -> y, (y, residual_out), (q, scale) or ((q, scale), residual_out)
-PyObject* py_rms_norm(PyObject*, PyObject* const* p, Py_ssize_t n) {
+PyObject* py_norm(PyObject*, PyObject* const* p, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   expect(n, 9);
   Tensor x = arg_tensor(p[0]), w = arg_tensor(p[1]), b = arg_tensor(p[2]), res = arg_tensor(p[3]);
-  RmsArgs a{};
+  NormArgs a{};
   a.eps = arg_double(p[4]);
   const bool prenorm = arg_bool(p[5]), in_f32 = arg_bool(p[6]);
-  a.quantize = arg_bool(p[7]);
-  a.normalise = arg_bool(p[8]);
-  const char* who = a.normalise ? "fla_amd rms_norm" : "fla_amd quantize_rows";
+  a.rows8 = arg_long(p[7]);
+  a.kind = (NormKind)arg_long(p[8]);
+  const char* who = a.kind == kLayer ? "fla_amd layer_norm" : a.kind == kRms ? "fla_amd rms_norm" : "fla_amd quantize_rows";
   TORCH_CHECK_VALUE(x.defined() && x.dim() >= 1 && x.size(-1) > 0, who, ": x is [..., N], N at least 1");
   TORCH_CHECK_TYPE(floating(x), who, ": x in bf16, fp16 or fp32, not ", x.scalar_type());
   const int64_t N = x.size(-1);
   for (const Tensor* t : {&w, &b}) {
     if (!t->defined()) continue;
-    TORCH_CHECK_TYPE(t->is_floating_point(), "fla_amd rms_norm: weight and bias in a floating type");
-    TORCH_CHECK_VALUE(t->numel() == N && t->dim() == 1, "fla_amd rms_norm: weight and bias hold ", N, " values");
+    TORCH_CHECK_TYPE(t->is_floating_point(), who, ": weight and bias in a floating type");
+    TORCH_CHECK_VALUE(t->numel() == N && t->dim() == 1, who, ": weight and bias hold ", N, " values");
   }
   if (res.defined()) {
-    TORCH_CHECK_VALUE(res.sizes() == x.sizes(), "fla_amd rms_norm: the residual has x's shape");
+    TORCH_CHECK_VALUE(res.sizes() == x.sizes(), who, ": the residual has x's shape");
     TORCH_CHECK_TYPE(res.scalar_type() == x.scalar_type() || res.scalar_type() == at::kFloat,
-                     "fla_amd rms_norm: the residual is in x's type or in fp32");
+                     who, ": the residual is in x's type or in fp32");
   }
-  const int64_t most = a.normalise ? 16384 : 1 << 23;
+  const int64_t most = a.kind != kRowsOnly ? 16384 : 1 << 23;
   TORCH_CHECK_NOT_IMPLEMENTED(N <= most, who, ": rows of at most ", most, " elements, not ", N);
   need_gpu({&x, &w, &b, &res});
   const bool grad = wants_grad({&x, &w, &b, &res});
-  TORCH_CHECK(!(grad && a.quantize), "fla_amd: rows in 8 bits have no gradient; call it under torch.no_grad()");
+  TORCH_CHECK(!(grad && a.rows8), "fla_amd: rows in 8 bits have no gradient; call it under torch.no_grad()");
   c10::DeviceGuard on_device(x.device());
   // one type for both, x's or fp32
   auto fits = [&](const Tensor& t) { return !t.defined() || t.scalar_type() == x.scalar_type(); };
@@ -1240,15 +1263,15 @@ PyObject* py_rms_norm(PyObject*, PyObject* const* p, Py_ssize_t n) {
   if (!prenorm && !grad) a.kept_type.reset();   // nobody asks for the sum
   Tensor y, scale, kept;
   if (grad) {
-    auto out = RmsNode::apply(x, maybe(w), maybe(b), maybe(res), a);
+    auto out = NormNode::apply(x, maybe(w), maybe(b), maybe(res), a);
     y = out[0];
     if (out.size() > 1) kept = out[1];
   } else {
     at::AutoDispatchBelowADInplaceOrView guard;
-    RmsOut o = rms_forward(x.contiguous(), w, b, res.defined() ? res.contiguous() : res, a, false);
+    NormOut o = norm_forward(x.contiguous(), w, b, res.defined() ? res.contiguous() : res, a, false);
     y = o.y, scale = o.scale, kept = o.kept;
   }
-  PyObject* first = a.quantize ? pair(y, scale) : THPVariable_Wrap(y);
+  PyObject* first = a.rows8 ? pair(y, scale) : THPVariable_Wrap(y);
   if (!prenorm) return first;
   PyObject* t = PyTuple_New(2);
   if (!first || !t) throw python_error();
@@ -1264,8 +1287,7 @@ PyObject* py_quant_linear(PyObject*, PyObject* const* p, Py_ssize_t n) {
   expect(n, 8);
   Tensor x = arg_tensor(p[0]), sx = arg_tensor(p[1]), w = arg_tensor(p[2]), sw = arg_tensor(p[3]), bias = arg_tensor(p[4]),
          res = arg_tensor(p[5]);
-  const long act = PyLong_AsLong(p[6]);
-  if (act == -1 && PyErr_Occurred()) throw python_error();
+  const long act = arg_long(p[6]);
   const auto type = arg_bool(p[7]) ? at::kBFloat16 : at::kHalf;
   TORCH_CHECK_TYPE(x.defined() && w.defined() && sx.defined() && sw.defined() && x.scalar_type() == at::kFloat8_e4m3fn &&
                        w.scalar_type() == at::kFloat8_e4m3fn && sx.scalar_type() == at::kFloat && sw.scalar_type() == at::kFloat,
@@ -1326,7 +1348,7 @@ PyMethodDef kMethods[] = {
     ENTRY("short_conv_step", py_conv_update<true>),
     ENTRY("norm_swish_gate", py_norm_gate),
     ENTRY("hgrn", py_hgrn),
-    ENTRY("rms_norm", py_rms_norm),
+    ENTRY("norm", py_norm),
     ENTRY("quant_linear", py_quant_linear),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fla_host", nullptr, -1, kMethods};

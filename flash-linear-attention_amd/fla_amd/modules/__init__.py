@@ -6,7 +6,7 @@ from .fused_norm_gate import (FusedLayerNormSwishGate, FusedRMSNormSwishGate, La
                               layer_norm_swish_gate_fn, rms_norm_swish_gate_fn)
 from .gate_activations import gdn_gate, gdn_gate_bwd, gdn_gate_fwd, gla_gate, gla_gate_bwd, gla_gate_fwd
 from .l2norm import L2NormFunction, l2_norm, l2norm_bwd, l2norm_fwd
-from .layernorm import RMSNorm, quantize_rows, rms_norm
+from .layernorm import LayerNorm, RMSNorm, layer_norm, quantize_rows, rms_norm
 from .quant_linear import QuantLinear, quant_linear
 
 __all__ = [
@@ -15,6 +15,6 @@ __all__ = [
     "layer_norm_swish_gate_fn", "rms_norm_swish_gate_fn",
     "L2NormFunction", "l2_norm", "l2norm_fwd", "l2norm_bwd",
     "gla_gate", "gla_gate_fwd", "gla_gate_bwd", "gdn_gate", "gdn_gate_fwd", "gdn_gate_bwd",
-    "RMSNorm", "rms_norm", "quantize_rows",
+    "RMSNorm", "rms_norm", "LayerNorm", "layer_norm", "quantize_rows",
     "QuantLinear", "quant_linear",
 ]

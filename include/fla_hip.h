@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define FLA_ABI_VERSION 23
+#define FLA_ABI_VERSION 24
 
 enum fla_dtype { FLA_F32 = 0, FLA_BF16 = 1, FLA_F16 = 2 };
 
@@ -846,6 +846,27 @@ int fla_rms_norm_fwd(const void* x, const void* residual, int residual_dtype, co
 int fla_rms_norm_bwd(const void* dy, const void* kept, int kept_dtype, const void* weight, int weight_dtype, const float* rstd,
                      const void* dresidual, void* dx, void* dresidual_in, float* dw_partial, float* db_partial, int64_t M,
                      int64_t N, int dtype, fla_stream_t stream);
+
+/* fla_rms_norm_rows8_fwd: the forward with the 8-bit type as an argument, `scale` given.  FLA_ROWS_E4M3: as above; FLA_ROWS_INT8: whole numbers
+ * of -127 to 127, scale = max(max|y|, 1e-30) / 127, the nearest to y / scale, halves to even.  A row of integers that holds an infinity or NaN has that
+ * scale.  Without normalise, residual and residual_out N <= 2^23. */
+enum fla_rows8 { FLA_ROWS_NONE = 0, FLA_ROWS_E4M3 = 1, FLA_ROWS_INT8 = 2 };
+int fla_rms_norm_rows8_fwd(const void* x, const void* residual, int residual_dtype, const void* weight, const void* bias,
+                           int weight_dtype, void* y, float* scale, void* residual_out, int residual_out_dtype, int64_t M,
+                           int64_t N, float eps, int normalise, int rows8, int dtype, fla_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Layer norm of rows with the residual's addition (interface of LayerNorm / layer_norm, fla/modules/layernorm.py):
+ *   s = x + residual,  mu = mean s,  y = (s - mu) / sqrt(mean (s - mu)^2 + eps) * weight (+ bias).
+ * Operands, types and limits as for the RMS norm; mean, rstd fp32 [M], both or neither, for the backward.  rows8: FLA_ROWS_NONE (scale
+ * NULL) or the type of the 8-bit rows in y, with `scale`.  dw_partial, db_partial: fp32 [fla_layer_norm_workgroups(M, N), N]. */
+int fla_layer_norm_workgroups(int64_t M, int64_t N);
+int fla_layer_norm_fwd(const void* x, const void* residual, int residual_dtype, const void* weight, const void* bias,
+                       int weight_dtype, void* y, float* scale, void* residual_out, int residual_out_dtype, float* mean, float* rstd,
+                       int64_t M, int64_t N, float eps, int rows8, int dtype, fla_stream_t stream);
+int fla_layer_norm_bwd(const void* dy, const void* kept, int kept_dtype, const void* weight, int weight_dtype, const float* mean,
+                       const float* rstd, const void* dresidual, void* dx, void* dresidual_in, float* dw_partial, float* db_partial,
+                       int64_t M, int64_t N, int dtype, fla_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Product of 8-bit rows, the projection behind the norm above (no counterpart in the reference, whose projections are
