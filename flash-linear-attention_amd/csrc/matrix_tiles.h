@@ -1,0 +1,220 @@
+// Tiles of a matrix product  c[m,n] = sum_k a(m,k) b(n,k)  on the 32x32 matrix instructions, each operand with its contraction index
+// contiguous (rows [m][k]) or strided (rows [k][m]), 16-bit elements or 8-bit integers, sums in 32 bits.
+//
+// Four waves share a BM x BN tile, a wave holds a quarter of it (MT x NT tiles of 32 x 32) and, where the tile is 256 x 256, has a SIMD's
+// registers to itself.  Slices of 128 bytes of k travel straight from memory into a ring of RING pieces of LDS.  While one half of a slice is
+// multiplied, the fragments of the next half are read; one barrier a slice, ahead of its second half, orders everything: behind it the next slice is
+// there for every wave, and as everybody's fragments of this one are in registers its piece is free.
+//
+// A wave's quarter of 128 x 128 reads 32 fragments for 64 instructions: 128 KB a slice and CU, half of what LDS passes in that time.  (Eight waves
+// of 128 x 64 read 192 KB, which with the 64 KB of the copies is all of it.)
+//
+// Memory is read through buffer descriptors that end where the operand ends: rows and pieces behind it are zeros, by the hardware's range check.
+#pragma once
+#include "fla_common.h"
+
+namespace {
+
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// 16 bytes of a row of the operands and the instruction that takes them
+template <typename T>
+struct Mat {   // bf16, f16
+  typedef f32x16 acc;
+  static FLA_DEVICE acc mma(i32x4 a, i32x4 b, acc c) {
+    typedef typename Elem<T>::v8 v8;
+    return Elem<T>::mfma32(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c);
+  }
+};
+template <>
+struct Mat<int8_t> {
+  typedef i32x16 acc;
+  static FLA_DEVICE acc mma(i32x4 a, i32x4 b, acc c) { return __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, 0, 0, 0); }
+};
+
+// The transposing read of four rows.  __restrict__ gives the access an alias scope: of one without any the compiler takes it that it may read what copies
+// in flight write, and waits for all of them ahead of every read.  (The tiles wait where it is needed.)
+FLA_DEVICE s16x4 lds_read_tr(lds_s16x4* __restrict__ p) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16(p); }
+
+constexpr int kSliceBytes = 128;          // of k
+constexpr uint32_t kMatBeyond = 1u << 31; // an offset that no descriptor reaches
+constexpr int64_t kMatMaxDim = 1 << 22;   // elements of a row of an operand: 256 rows are less than 2^31 bytes
+
+// From where on a slice is read, and to where the operand goes
+struct MatSource {
+  const char *from, *end;
+  int left;   // of k, in bytes (contiguous operands)
+  FLA_DEVICE __amdgpu_buffer_rsrc_t descriptor() const {
+    const int64_t bytes = end - from;
+    return __builtin_amdgcn_make_buffer_rsrc((void*)from, 0, bytes < 0 ? 0 : bytes < (int64_t)kMatBeyond - 1 ? (int)bytes : (int)(kMatBeyond - 1), 0x00027000);
+  }
+};
+FLA_DEVICE void mat_copy(__amdgpu_buffer_rsrc_t from, uint32_t at, char* lds) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)lds, 16, (int)at, 0, 0, 0);
+}
+
+// One operand of a tile, ROWS of it; STRIDED: rows of memory are [k][ROWS], otherwise [ROWS][k].  PAIR: rows of two matrices, 32 of the one and 32 of the
+// other in turn (the products of one row with both are then in one lane).
+//
+// LDS layout of a slice.  Contiguous: ROWS rows of 128 bytes, the 16-byte pieces of a row permuted by a key of the row.  A b128 read serves lanes
+// 0-3, 12-15, 20-27 together, then 4-11, 16-19, 28-31, and the same of the upper half: with these keys each sixteen meet all 64 banks once.
+// Strided (16-bit types): 64 rows of ROWS elements, their 64-byte quarters permuted by a key of k.  The transposing read takes 64 bytes of each of four
+// rows for 32 lanes, which the keys spread over all banks.
+template <int ROWS, bool STRIDED, bool PAIR = false>
+struct Operand;
+
+template <int ROWS, bool PAIR>
+struct Operand<ROWS, false, PAIR> {
+  static constexpr int kSources = PAIR ? 2 : 1, kBytes = ROWS * kSliceBytes, kCopies = ROWS / 32;   // copy instructions of each of four waves for a slice
+  static_assert(kCopies >= 1, "whole copies");
+  static FLA_DEVICE int key(int r) { return (r >> 1 & 1) | (r >> 3 & 3) << 1; }
+  uint32_t at[kCopies];
+  int piece[kCopies];      // bytes of k ahead of what this lane copies
+  FLA_DEVICE void start(int wave, int lane, uint32_t pitch) {
+#pragma unroll
+    for (int q = 0; q < kCopies; ++q) {
+      const int r = (wave * kCopies + q) * 8 + (lane >> 3);
+      piece[q] = ((lane & 7) ^ key(r)) * 16;
+      at[q] = (uint32_t)(PAIR ? r / 64 * 32 + r % 32 : r) * pitch + piece[q];
+    }
+  }
+  FLA_DEVICE void copy(int q, char* lds, const MatSource* from, int wave) const {
+    const MatSource& s = from[PAIR ? (wave * kCopies + q) / 4 & 1 : 0];
+    mat_copy(s.descriptor(), piece[q] < s.left ? at[q] : kMatBeyond, lds + (wave * kCopies + q) * 1024);
+  }
+  // rows r0 .. r0+31 of the tile as the instruction takes them, quarter h of the slice
+  static FLA_DEVICE i32x4 fragment(const char* lds, int r0, int h, int lane) {
+    const int r = lane & 31;
+    return *(const i32x4*)(lds + (r0 + r) * kSliceBytes + (((2 * h + (lane >> 5)) ^ key(r)) * 16));
+  }
+};
+
+template <int ROWS>
+struct Operand<ROWS, true, false> {
+  static constexpr int kSources = 1, kBytes = ROWS * kSliceBytes, kCopies = ROWS / 32, kPieces = ROWS / 8, kDeep = 64 / kPieces;   // kDeep: k of a copy
+  static FLA_DEVICE int key(int k) { return ROWS > 64 ? k & 3 : k >> 1 & 1; }
+  uint32_t at[kCopies];
+  FLA_DEVICE void start(int wave, int lane, uint32_t pitch) {
+#pragma unroll
+    for (int q = 0; q < kCopies; ++q) {
+      const int k = (wave * kCopies + q) * kDeep + lane / kPieces;
+      at[q] = (uint32_t)k * pitch + ((lane % kPieces) ^ key(k) << 2) * 16;
+    }
+  }
+  FLA_DEVICE void copy(int q, char* lds, const MatSource* from, int wave) const { mat_copy(from->descriptor(), at[q], lds + (wave * kCopies + q) * 1024); }
+  static FLA_DEVICE i32x4 fragment(const char* lds, int r0, int h, int lane) {
+    const int j = lane & 15, k = 16 * h + 8 * (lane >> 5) + (j >> 2);
+    const char* p = lds + k * ROWS * 2 + ((r0 >> 5) ^ key(k)) * 64 + (lane >> 4 & 1) * 32 + (j & 3) * 8;
+    const i32x2 lo = __builtin_bit_cast(i32x2, lds_read_tr((lds_s16x4*)p));
+    const i32x2 hi = __builtin_bit_cast(i32x2, lds_read_tr((lds_s16x4*)(p + 4 * ROWS * 2)));   // (the same key)
+    return i32x4{lo[0], lo[1], hi[0], hi[1]};
+  }
+};
+
+// The sums of a tile.  Lane l of wave (wm, wn) holds in acc[i][j][r] the sum of m = wm BM/2 + 32 i + l % 32 and n = wn BN/2 + 32 j + 8 (r / 4) + 4 (l / 32) + r % 4.
+template <typename T, int BM, int BN, int RING, bool SM, bool SN, bool PAIR = false>
+struct MatTile {
+  static constexpr int MT = BM / 64, NT = BN / 64, kPiece = (BM + BN) * kSliceBytes, kLds = RING * kPiece;
+  typedef Operand<BM, SM> OpM;
+  typedef Operand<BN, SN, PAIR> OpN;
+  typedef typename Mat<T>::acc acc_t;
+  struct Frags {
+    i32x4 m[MT][2], n[NT][2];
+  };
+  static constexpr int kCopies = OpM::kCopies + OpN::kCopies;
+
+  // `source(s, m, n)`: where slice s lies (n: an array of OpN::kSources); asked for slices behind the last one too, of which nothing may be left, or what
+  // may be read (they are copied and not multiplied).  Slices first .. last - 1, at least one.
+  template <typename F>
+  static FLA_DEVICE void run(char* lds, const OpM& om, const OpN& on, int first, int last, const F& source, acc_t (&acc)[MT][NT]) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j] = acc_t{};
+    struct Slice {
+      MatSource m[1], n[OpN::kSources];
+      char* lds;
+    };
+    auto slice = [&](int s, int piece) {
+      Slice c;
+      source(s, c.m, c.n);
+      c.lds = lds + piece * kPiece;
+      return c;
+    };
+    auto copy = [&](const Slice& c, int q) {
+      if (q < OpM::kCopies) om.copy(q, c.lds, c.m, wave);
+      else on.copy(q - OpM::kCopies, c.lds + OpM::kBytes, c.n, wave);
+    };
+    constexpr int kFrags = 2 * (MT + NT), kProducts = 2 * MT * NT;
+    auto read = [&](Frags& f, const char* from, int half, int q) {   // (in the order in which they are multiplied)
+      const int h = q / (MT + NT), g = q % (MT + NT);
+      if (g < NT) f.n[g][h] = OpN::fragment(from + OpM::kBytes, (wn * NT + g) * 32, 2 * half + h, lane);
+      else f.m[g - NT][h] = OpM::fragment(from, (wm * MT + g - NT) * 32, 2 * half + h, lane);
+    };
+    // The products of half a slice, between them the reads of the next half and, with COPIES, the copies of a slice.  The order of the instructions is
+    // kept: both go in the first three quarters of the products (copies in the first half 2 % slower, over the whole slice 10 %: they arrive late).
+    auto half = [&](const Frags& now, Frags& next, const char* from, int which, const Slice& c, bool copies) {
+      constexpr int r = kProducts * 3 / 4 > 0 ? kProducts * 3 / 4 : 1;
+#pragma unroll
+      for (int g = 0; g < kProducts; ++g) {
+        const int h = g / (MT * NT), i = g / NT % MT, j = g % NT;
+        acc[i][j] = Mat<T>::mma(now.n[j][h], now.m[i][h], acc[i][j]);
+        if (g < r) {
+#pragma unroll
+          for (int q = g * kFrags / r; q < (g + 1) * kFrags / r; ++q) read(next, from, which, q);
+          if (copies)
+#pragma unroll
+            for (int q = g * kCopies / r; q < (g + 1) * kCopies / r; ++q) copy(c, q);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    int piece = 0;   // of slice s
+#pragma unroll
+    for (int d = 0; d < RING; ++d) {
+      const Slice c = slice(first + d, d);
+#pragma unroll
+      for (int q = 0; q < kCopies; ++q) copy(c, q);
+    }
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"((RING - 1) * kCopies) : "memory");
+    Frags f[2];
+#pragma unroll
+    for (int q = 0; q < kFrags; ++q) read(f[0], lds, 0, q);
+    Slice c;
+    for (int s = first; s < last; ++s) {
+      half(f[0], f[1], lds + piece * kPiece, 1, c, false);
+      // this wave's copies of slice s + 1 have arrived and its fragments of s are read; then everybody's
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"((RING - 2) * kCopies) : "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      c = slice(s + RING, piece);
+      piece = piece + 1 < RING ? piece + 1 : 0;
+      half(f[1], f[0], lds + piece * kPiece, 0, c, true);
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // no copy into LDS outlives the workgroup
+  }
+};
+
+// The tile of a workgroup.  Neighbouring workgroup numbers go to different XCDs: each XCD takes a run of tiles, eight rows of tiles deep, that share
+// operands in its L2.
+FLA_DEVICE void mat_tile_of(uint32_t block, uint32_t tm_all, uint32_t tn_all, uint32_t* tm, uint32_t* tn) {
+  const uint32_t total = tm_all * tn_all, xcd = block % 8, per = total / 8, rest = total % 8;
+  const uint32_t id = xcd * per + (xcd < rest ? xcd : rest) + block / 8;
+  const uint32_t deep = tm_all < 8 ? tm_all : 8, band = id / (deep * tn_all), in = id - band * deep * tn_all;
+  const uint32_t rows_in = tm_all - band * deep < deep ? tm_all - band * deep : deep, col = in / rows_in;
+  *tm = band * deep + in - col * rows_in, *tn = col;
+}
+
+// Eight consecutive n a lane from two runs of four, packed in pairs (a, b: the lane's of r / 4 even and of the odd one behind it): lane l then holds
+// those from 8 (r / 4 + l / 32) on.
+FLA_DEVICE i32x4 mat_join(u32x2 a, u32x2 b) {
+  const u32x2 p = __builtin_amdgcn_permlane32_swap(a[0], b[0], false, false), q = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
+  return i32x4{(int)p[0], (int)q[0], (int)p[1], (int)q[1]};
+}
+
+}  // namespace

@@ -10,6 +10,7 @@
 // own rounding to 8 bits is a thousand times that.  Results leave in 16 bits only.  The alternative, conversion to bf16 and the instruction
 // that keeps whole products, runs at half the rate.
 #include "fla_common.h"
+#include "linear_epilogue.h"
 
 namespace {
 
@@ -30,30 +31,8 @@ struct LinearParams {
   bool wide;             // rows of y and of the residual can be taken 16 bytes at a time
 };
 
-template <int ACT>
-FLA_DEVICE float activate(float v) {
-  if (ACT == FLA_ACT_SILU) return v * __builtin_amdgcn_rcpf(1.f + __expf(-v));
-  if (ACT == FLA_ACT_GELU) return 0.5f * v * (1.f + erff(v * 0.70710678f));
-  if (ACT == FLA_ACT_RELU) return v < 0.f ? 0.f : v;      // (NaN stays)
-  return v;
-}
-
 // both e4m3, no block scales
 FLA_DEVICE f32x4 mfma8(i32x8 a, i32x8 b, f32x4 c) { return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0, 0, 0); }
-
-// COUNT values at any element address; unless FULL, the first `valid` of them one by one
-template <typename T, int COUNT, bool FULL>
-FLA_DEVICE void load_some(const T* p, int valid, float* o) {
-  if (FULL) {
-    typedef T vec __attribute__((ext_vector_type(COUNT), aligned(alignof(T))));
-    const vec v = *(const vec*)p;
-#pragma unroll
-    for (int i = 0; i < COUNT; ++i) o[i] = (float)v[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < COUNT; ++i) o[i] = i < valid ? (float)p[i] : 0.f;
-  }
-}
 
 // COUNT (4 or 8) consecutive n of row m from their sums.  FULL: all of them exist, and they can be taken 16 bytes at a time.
 template <typename T, int COUNT, int ACT, bool FULL>
@@ -87,19 +66,6 @@ FLA_DEVICE void finish(const LinearParams& p, int64_t m, int64_t n, const float*
 template <typename T>
 FLA_DEVICE float bias_of(const LinearParams& p, int64_t n) {
   return !p.bias || n >= p.N ? 0.f : p.bias_f32 ? ((const float*)p.bias)[n] : (float)((const T*)p.bias)[n];
-}
-
-// the activation as a constant: one branch a tile instead of one an element
-template <int V>
-struct Const {
-  static constexpr int value = V;
-};
-template <typename F>
-FLA_DEVICE void with_activation(int act, const F& f) {
-  if (act == FLA_ACT_SILU) f(Const<FLA_ACT_SILU>());
-  else if (act == FLA_ACT_GELU) f(Const<FLA_ACT_GELU>());
-  else if (act == FLA_ACT_RELU) f(Const<FLA_ACT_RELU>());
-  else f(Const<FLA_ACT_NONE>());
 }
 
 // ------------------------------------------------------------------------------------------------ tiles

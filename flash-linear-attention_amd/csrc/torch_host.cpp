@@ -821,6 +821,101 @@ struct NormNode : torch::autograd::Function<NormNode> {
   }
 };
 
+// ---------------------------------------------------------------------------------------------------- gated product
+// Rows at 16-byte addresses; with `pieces`, of a multiple of so many elements: zeros are added behind them
+Tensor whole_rows(const Tensor& t, int64_t pieces = 1) {
+  const int64_t K = t.size(-1), more = (pieces - K % pieces) % pieces;
+  Tensor c = more ? at::constant_pad_nd(t, {0, more}) : t.contiguous();
+  return (uintptr_t)c.data_ptr() % 16 == 0 ? c : c.clone();
+}
+
+struct GatedNode : torch::autograd::Function<GatedNode> {
+  struct Rest {
+    bool x, wg, wu, bg, bu;  // whether they have a gradient
+    at::ScalarType bg_type, bu_type;
+    int64_t F;
+    long act;
+  };
+  // kept: g and u [2, M, ld] for a backward, or NULL
+  static Tensor run(const Tensor& x_, const Tensor& wg_, const Tensor& wu_, const Tensor& bg_, const Tensor& bu_, long act, Tensor* kept) {
+    const int64_t F = wg_.size(0), K0 = x_.size(-1), M = x_.numel() / K0, ld = (F + 7) / 8 * 8;
+    auto shape = x_.sizes().vec();
+    shape.back() = F;
+    Tensor h = fresh(shape, x_, x_.scalar_type());
+    if (kept) *kept = fresh({2, M, ld}, x_, x_.scalar_type());
+    if (M == 0) return h;
+    const Tensor x = whole_rows(x_, 8), wg = whole_rows(wg_, 8), wu = whole_rows(wu_, 8);
+    const bool same = (!bg_.defined() || bg_.scalar_type() == x.scalar_type()) && (!bu_.defined() || bu_.scalar_type() == x.scalar_type());
+    const Tensor bg = same ? (bg_.defined() ? bg_.contiguous() : bg_) : f32(bg_), bu = same ? (bu_.defined() ? bu_.contiguous() : bu_) : f32(bu_);
+    const int64_t K = x.size(-1);
+    const int splits = fla_gated_linear_splits(M, F, K, 2);
+    const Tensor sums = splits > 1 ? fresh({splits, M, 2, F}, x, at::kFloat) : Tensor();
+    char* keep = kept ? (char*)kept->data_ptr() : nullptr;
+    check(fla_gated_linear_fwd(ptr(x), ptr(wg), ptr(wu), ptr(bg), ptr(bu), same ? dt(x) : FLA_F32, ptr(h), keep,
+                               keep ? keep + M * ld * 2 : nullptr, ld, M, F, K, (int)act, dt(x), ptr(sums), stream_of(x)),
+          "fla_gated_linear_fwd");
+    return h;
+  }
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu, const Maybe& bg_, const Maybe& bu_, long act) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const Tensor bg = given(bg_), bu = given(bu_);
+    Tensor kept;
+    Tensor h = run(x, wg, wu, bg, bu, act, &kept);
+    const Rest r{asks(x), asks(wg), asks(wu), asks(bg), asks(bu), bg.defined() ? bg.scalar_type() : at::kFloat, bu.defined() ? bu.scalar_type() : at::kFloat,
+                 wg.size(0), act};
+    // (x for the weights' gradients, the weights for x's)
+    ctx->save_for_backward({r.wg || r.wu ? x : Tensor(), r.x ? wg : Tensor(), r.x ? wu : Tensor(), kept});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    hold(ctx, r);
+    return h;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    at::AutoDispatchBelowADInplaceOrView guard;
+    const auto saved = ctx->get_saved_variables();
+    const Tensor& kept = saved[3];
+    const Rest& r = held<Rest>(ctx);
+    const auto shape = ctx->saved_data["shape"].toIntVector();
+    c10::DeviceGuard on_device(kept.device());
+    const int64_t M = kept.size(1), ld = kept.size(2), F = r.F, K0 = shape.back(), K = (K0 + 7) / 8 * 8;
+    const auto type = kept.scalar_type();
+    Tensor dx, dwg, dwu, dbg, dbu;
+    if (M == 0) {
+      auto zeros = [&](bool wanted, at::IntArrayRef sizes, at::ScalarType t) { return wanted ? at::zeros(sizes, kept.options().dtype(t)) : Tensor(); };
+      return {zeros(r.x, shape, type), zeros(r.wg, {F, K0}, type), zeros(r.wu, {F, K0}, type), zeros(r.bg, {F}, r.bg_type), zeros(r.bu, {F}, r.bu_type),
+              Tensor()};
+    }
+    const Tensor dh = as(grads[0], type).contiguous();
+    const Tensor d = fresh_like(kept);
+    const int64_t rows = fla_gated_linear_bwd_rows(M), parts = (M + rows - 1) / rows, half = M * ld * 2;
+    const Tensor pg = r.bg ? fresh({parts, F}, kept, at::kFloat) : Tensor(), pu = r.bu ? fresh({parts, F}, kept, at::kFloat) : Tensor();
+    const fla_stream_t stream = stream_of(kept);
+    char *g = (char*)kept.data_ptr(), *dg = (char*)d.data_ptr();
+    check(fla_gated_linear_bwd_gate(ptr(dh), g, g + half, dg, dg + half, fptr(pg), fptr(pu), ld, M, F, (int)r.act, dt(kept), stream),
+          "fla_gated_linear_bwd_gate");
+    if (r.bg) dbg = sum_partials(pg, {F}, r.bg_type);
+    if (r.bu) dbu = sum_partials(pu, {F}, r.bu_type);
+    if (r.x) {
+      const Tensor wg = whole_rows(saved[1], 8), wu = whole_rows(saved[2], 8);
+      dx = fresh({M, K}, kept, type);
+      const int splits = fla_gated_linear_bwd_dx_splits(M, F, K);
+      const Tensor sums = splits > 1 ? fresh({splits, M, K}, kept, at::kFloat) : Tensor();
+      check(fla_gated_linear_bwd_dx(dg, dg + half, ptr(wg), ptr(wu), ptr(dx), ld, M, F, K, dt(kept), fptr(sums), stream), "fla_gated_linear_bwd_dx");
+      dx = (K == K0 ? dx : dx.narrow(1, 0, K0).contiguous()).view(shape);
+    }
+    if (r.wg || r.wu) {
+      const Tensor x = whole_rows(saved[0], 8);
+      if (r.wg) dwg = fresh({F, K}, kept, type);
+      if (r.wu) dwu = fresh({F, K}, kept, type);
+      const int splits = fla_gated_linear_bwd_dw_splits(M, F, K, r.wg && r.wu);
+      const Tensor sums = splits > 1 ? fresh({r.wg && r.wu ? 2 : 1, splits, F, K}, kept, at::kFloat) : Tensor();
+      check(fla_gated_linear_bwd_dw(dg, dg + half, ptr(x), ptr(dwg), ptr(dwu), ld, M, F, K, dt(kept), fptr(sums), stream), "fla_gated_linear_bwd_dw");
+      if (K != K0 && r.wg) dwg = dwg.narrow(1, 0, K0).contiguous();
+      if (K != K0 && r.wu) dwu = dwu.narrow(1, 0, K0).contiguous();
+    }
+    return {dx, dwg, dwu, dbg, dbu, Tensor()};
+  }
+};
+
 // ---------------------------------------------------------------------------------------------------- Python entries
 Tensor arg_tensor(PyObject* o) {
   if (o == Py_None) return Tensor();
@@ -1334,6 +1429,34 @@ PyObject* py_quant_linear(PyObject*, PyObject* const* p, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// gated_linear(x, gate_weight, up_weight, gate_bias | None, up_bias | None, activation)
+PyObject* py_gated_linear(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 6);
+  const Tensor x = arg_tensor(p[0]), wg = arg_tensor(p[1]), wu = arg_tensor(p[2]), bg = arg_tensor(p[3]), bu = arg_tensor(p[4]);
+  const long act = arg_long(p[5]);
+  TORCH_CHECK_VALUE(x.defined() && wg.defined() && wu.defined() && x.dim() >= 1 && wg.dim() == 2 && wg.sizes() == wu.sizes() &&
+                        wg.size(1) == x.size(-1) && wg.size(0) > 0 && wg.size(1) > 0,
+                    "fla_amd gated_linear: x is [..., K], both weights [F, K], neither empty");
+  TORCH_CHECK_TYPE(is16(x) && wg.scalar_type() == x.scalar_type() && wu.scalar_type() == x.scalar_type(),
+                   "fla_amd gated_linear: x and both weights in bf16 or in fp16, not ", x.scalar_type(), ", ", wg.scalar_type(), " and ",
+                   wu.scalar_type());
+  const int64_t F = wg.size(0), K = wg.size(1);
+  for (const Tensor* t : {&bg, &bu}) {
+    if (!t->defined()) continue;
+    TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == F, "fla_amd gated_linear: biases hold ", F, " values");
+    TORCH_CHECK_TYPE(t->is_floating_point(), "fla_amd gated_linear: biases in a floating type");
+  }
+  TORCH_CHECK_NOT_IMPLEMENTED(F <= 1 << 22 && K <= 1 << 22 && x.numel() / K <= 0x7fffffff,
+                              "fla_amd gated_linear: weights of at most 2^22 rows and columns, x of less than 2^31 rows");
+  need_gpu({&x, &wg, &wu, &bg, &bu});
+  c10::DeviceGuard on_device(x.device());
+  if (wants_grad({&x, &wg, &wu, &bg, &bu})) return THPVariable_Wrap(GatedNode::apply(x, wg, wu, maybe(bg), maybe(bu), act));
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return THPVariable_Wrap(GatedNode::run(x, wg, wu, bg, bu, act, nullptr));
+  END_HANDLE_TH_ERRORS
+}
+
 #define ENTRY(name, fn) {name, (PyCFunction)(void (*)(void))fn, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {
     ENTRY("plan", py_plan),
@@ -1350,6 +1473,7 @@ PyMethodDef kMethods[] = {
     ENTRY("hgrn", py_hgrn),
     ENTRY("norm", py_norm),
     ENTRY("quant_linear", py_quant_linear),
+    ENTRY("gated_linear", py_gated_linear),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fla_host", nullptr, -1, kMethods};
 

@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define FLA_ABI_VERSION 24
+#define FLA_ABI_VERSION 25
 
 enum fla_dtype { FLA_F32 = 0, FLA_BF16 = 1, FLA_F16 = 2 };
 
@@ -880,6 +880,37 @@ int fla_quant_linear_splits(int64_t M, int64_t N, int64_t K);
 int fla_quant_linear(const void* x, const float* x_scale, const void* weight, const float* weight_scale, const void* bias,
                      int bias_dtype, const void* residual, int residual_dtype, void* y, int64_t M, int64_t N, int64_t K,
                      int activation, int dtype, float* workspace, fla_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * The gated product of a feed-forward block (no counterpart in the reference in one operator: its
+ * blocks call torch.nn.Linear twice and the activation of fla/modules/activations.py):
+ *   g = x gate_weight' + gate_bias,  u = x up_weight' + up_bias,  h[m,f] = act(g) u.
+ * x [M,K], weights [F,K], h [M,F] in `dtype`, bf16 or fp16; K % 8 == 0, K, F <= 2^22; x and the weights at 16-byte addresses, any F and address of h (multiples of 8
+ * and of 16 bytes take the wide stores).  Biases [F] in `dtype` or fp32 (one type for both), or NULL.  activation: enum fla_activation.
+ * gate_out, up_out [M,ld], both or neither: g and u for the backward, ld = F rounded up to a multiple of 8, columns behind F unspecified.  A product of few tiles and
+ * a long K is summed in slices of K: fla_gated_linear_splits (element_bytes: 2, or 1 for rows in 8 bits) gives their number, and where it is more
+ * than one `workspace` holds [splits, M, 2, F] fp32 (int32 for rows of integers) at a 16-byte address.
+ *
+ * Backward, in three steps:
+ *   _bwd_gate: dgate = dh u act'(g), dup = dh act(g), both [M,ld] with zeros behind F, from the kept g and u; *_bias_partial: fp32
+ *     [ceil(M / fla_gated_linear_bwd_rows(M)), F] or NULL, their column sums are the biases' gradients.
+ *   _bwd_dx: dx [M,K] = dgate gate_weight + dup up_weight; workspace: fp32 [splits, M, K] where _dx_splits is more than one.
+ *   _bwd_dw: dgate_weight = dgate' x, dup_weight = dup' x [F,K], either may be NULL (both: whether both are asked for); workspace: fp32
+ *     [1 or 2, splits, F, K] where _dw_splits is more than one. */
+int fla_gated_linear_splits(int64_t M, int64_t F, int64_t K, int element_bytes);
+int fla_gated_linear_fwd(const void* x, const void* gate_weight, const void* up_weight, const void* gate_bias, const void* up_bias,
+                         int bias_dtype, void* h, void* gate_out, void* up_out, int64_t ld, int64_t M, int64_t F, int64_t K,
+                         int activation, int dtype, void* workspace, fla_stream_t stream);
+int fla_gated_linear_bwd_rows(int64_t M);
+int fla_gated_linear_bwd_gate(const void* dh, const void* gate, const void* up, void* dgate, void* dup, float* dgate_bias_partial,
+                              float* dup_bias_partial, int64_t ld, int64_t M, int64_t F, int activation, int dtype,
+                              fla_stream_t stream);
+int fla_gated_linear_bwd_dx_splits(int64_t M, int64_t F, int64_t K);
+int fla_gated_linear_bwd_dx(const void* dgate, const void* dup, const void* gate_weight, const void* up_weight, void* dx, int64_t ld,
+                            int64_t M, int64_t F, int64_t K, int dtype, float* workspace, fla_stream_t stream);
+int fla_gated_linear_bwd_dw_splits(int64_t M, int64_t F, int64_t K, int both);
+int fla_gated_linear_bwd_dw(const void* dgate, const void* dup, const void* x, void* dgate_weight, void* dup_weight, int64_t ld, int64_t M,
+                            int64_t F, int64_t K, int dtype, float* workspace, fla_stream_t stream);
 
 /* Diagnostics: C[M,N] (fp32) = A[M,Kd] * B[N,Kd]^T with bf16 operands, computed
  * with the same MFMA fragment helpers the kernels use (mode 0: 32x32x16 tiles,
