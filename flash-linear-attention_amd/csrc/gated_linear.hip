@@ -8,6 +8,7 @@
 // contraction, its second operand strided in memory; the weights' gradients as one launch of products with both operands strided.
 #include "linear_epilogue.h"
 #include "matrix_panels.h"
+#include "matrix_plan.h"
 #include "matrix_tiles.h"
 #include "row_vec.h"
 
@@ -28,26 +29,6 @@ struct GatedParams {
 template <typename O>
 FLA_DEVICE float gated_bias(const void* b, int f32, int64_t n, int64_t F) {
   return !b || n >= F ? 0.f : f32 ? ((const float*)b)[n] : (float)((const O*)b)[n];
-}
-
-// eight consecutive elements of a row from n on, of which those below N exist
-template <typename O>
-FLA_DEVICE void store_piece(O* row, int64_t n, int64_t N, bool wide, i32x4 v) {
-  if (wide && n + 8 <= N) {
-    *(i32x4*)(row + n) = v;
-  } else {
-    const typename Elem<O>::v8 e = __builtin_bit_cast(typename Elem<O>::v8, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (n + i < N) row[n + i] = e[i];
-  }
-}
-template <typename O>
-FLA_DEVICE u32x2 pack4(const float* v) {
-  typename Elem<O>::v4 e;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) e[i] = (O)v[i];
-  return __builtin_bit_cast(u32x2, e);
 }
 
 // T: type of the operands, O: of h
@@ -383,37 +364,8 @@ __global__ __launch_bounds__(256) void grad_finish_kernel(const float* part, T* 
 }
 
 // ------------------------------------------------------------------------------------------------ host
-// Which tile and how many slices of the contraction: the estimated time of each, in slices' time of a CU.
-enum TileKind { kBig, kMiddle, kSmall };
-struct TilePlan {
-  TileKind kind;
-  int splits;
-};
-constexpr int kTileM[3] = {256, 128, 64}, kTileN[3] = {256, 128, 128}, kTilePerCu[3] = {1, 2, 3};
-TilePlan plan_tiles(int64_t M, int64_t N, int64_t slices, int batch, double bytes_per_sum) {
-  // us for a slice of 128 bytes of k of a tile, with as many tiles on the CU as it holds
-  constexpr double kSlice[3] = {1.55, 0.55, 0.36};
-  TilePlan best{kBig, 1};
-  double time = 0;
-  for (int t = 0; t < 3; ++t) {
-    const int64_t tiles = batch * fla_cdiv(M, kTileM[t]) * fla_cdiv(N, kTileN[t]);
-    for (int splits = 1; splits <= 16; splits *= 2) {
-      if (splits > 1 && (slices < 4 * splits || tiles * splits > 1024)) break;
-      const int64_t n = tiles * splits, rounds = fla_cdiv(n, 256 * kTilePerCu[t]), in_last = n - (rounds - 1) * 256 * kTilePerCu[t];
-      // a CU with some of its tiles missing runs the others faster, but not as much
-      const double last = 0.5 + 0.5 * (double)fla_cdiv(in_last, 256) / kTilePerCu[t];
-      double est = (double)(fla_cdiv(slices, splits) + 4) * kSlice[t] * kTilePerCu[t] * ((double)(rounds - 1) + last) + 3;
-      if (splits > 1) est += 4 + 2 * splits * bytes_per_sum * batch * (double)M * (double)N / 4e6;
-      if ((t == 0 && splits == 1) || est < time) best = {(TileKind)t, splits}, time = est;
-    }
-  }
-  best.splits = (int)fla_cdiv(slices, fla_cdiv(slices, best.splits));   // none of them empty
-  return best;
-}
 TilePlan plan_dx(int64_t M, int64_t F, int64_t K) { return plan_tiles(M, K, 2 * fla_cdiv(F * 2, kSliceBytes), 1, 4); }
 TilePlan plan_dw(int64_t M, int64_t F, int64_t K, int batch) { return plan_tiles(F, K, fla_cdiv(M, 64), batch, 4); }
-
-constexpr int64_t kMaxGrid = (int64_t)1 << 24;   // workgroups of 256 threads in a launch of less than 2^32
 
 template <typename T, typename O>
 int launch_forward(const GatedParams& p, TileKind kind, hipStream_t st) {
@@ -486,13 +438,6 @@ int gated_forward(GatedParams& p, hipStream_t st) {
   return launch_forward<T, O>(p, plan.kind, st);
 }
 
-bool sizes_ok(int64_t M, int64_t F, int64_t K) { return M <= 0x7fffffff && F <= kMatMaxDim && K <= kMatMaxDim; }
-bool aligned16(std::initializer_list<const void*> ps) {
-  uintptr_t any = 0;
-  for (const void* p : ps) any |= (uintptr_t)p;
-  return any % 16 == 0;
-}
-
 }  // namespace
 
 extern "C" int fla_gated_linear_splits(int64_t M, int64_t F, int64_t K, int element_bytes) {
@@ -516,6 +461,24 @@ extern "C" int fla_gated_linear_fwd(const void* x, const void* gate_weight, cons
   p.act = activation, p.bias_f32 = bias_dtype == FLA_F32, p.wide = F % 8 == 0 && aligned16({h});
   hipStream_t st = (hipStream_t)stream;
   return dtype == FLA_BF16 ? gated_forward<bf16, bf16>(p, st) : gated_forward<f16, f16>(p, st);
+}
+
+extern "C" int fla_int8_gated_linear_fwd(const void* x, const float* x_scale, const void* gate_weight, const float* gate_scale, const void* up_weight,
+                                         const float* up_scale, const void* gate_bias, const void* up_bias, int bias_dtype, void* h, int64_t M,
+                                         int64_t F, int64_t K, int activation, int dtype, void* workspace, fla_stream_t stream) {
+  FLA_REQUIRE(x && x_scale && gate_weight && gate_scale && up_weight && up_scale && h && M >= 0 && F > 0 && K > 0, FLA_E_INVALID);
+  FLA_REQUIRE(activation >= FLA_ACT_NONE && activation <= FLA_ACT_RELU, FLA_E_INVALID);
+  FLA_REQUIRE(dtype == FLA_BF16 || dtype == FLA_F16, FLA_E_UNSUPPORTED);
+  FLA_REQUIRE((!gate_bias && !up_bias) || bias_dtype == dtype || bias_dtype == FLA_F32, FLA_E_UNSUPPORTED);
+  FLA_REQUIRE(sizes_ok(M, F, K) && K % 16 == 0 && K <= FLA_INT8_MAX_K, FLA_E_UNSUPPORTED);
+  FLA_REQUIRE(aligned16({x, gate_weight, up_weight, workspace}), FLA_E_ALIGNMENT);
+  if (M == 0) return FLA_OK;
+  GatedParams p{};
+  p.x = (const char*)x, p.wg = (const char*)gate_weight, p.wu = (const char*)up_weight, p.sx = x_scale, p.sg = gate_scale, p.su = up_scale;
+  p.bg = gate_bias, p.bu = up_bias, p.h = h, p.part = workspace, p.M = M, p.F = F, p.K = K, p.ldk = (F + 7) / 8 * 8;
+  p.act = activation, p.bias_f32 = bias_dtype == FLA_F32, p.wide = F % 8 == 0 && aligned16({h});
+  hipStream_t st = (hipStream_t)stream;
+  return dtype == FLA_BF16 ? gated_forward<int8_t, bf16>(p, st) : gated_forward<int8_t, f16>(p, st);
 }
 
 extern "C" int fla_gated_linear_bwd_rows(int64_t M) { return M <= 0 ? 1 : (int)(fla_cdiv(M, 256) < 32 ? 32 : fla_cdiv(M, 256)); }

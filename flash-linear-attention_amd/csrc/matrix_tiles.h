@@ -217,4 +217,24 @@ FLA_DEVICE i32x4 mat_join(u32x2 a, u32x2 b) {
   return i32x4{(int)p[0], (int)q[0], (int)p[1], (int)q[1]};
 }
 
+// eight consecutive elements of a row from n on, of which those below N exist
+template <typename O>
+FLA_DEVICE void store_piece(O* row, int64_t n, int64_t N, bool wide, i32x4 v) {
+  if (wide && n + 8 <= N) {
+    *(i32x4*)(row + n) = v;
+  } else {
+    const typename Elem<O>::v8 e = __builtin_bit_cast(typename Elem<O>::v8, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (n + i < N) row[n + i] = e[i];
+  }
+}
+template <typename O>
+FLA_DEVICE u32x2 pack4(const float* v) {
+  typename Elem<O>::v4 e;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) e[i] = (O)v[i];
+  return __builtin_bit_cast(u32x2, e);
+}
+
 }  // namespace

@@ -1376,24 +1376,43 @@ PyObject* py_norm(PyObject*, PyObject* const* p, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// quant_linear(x, x_scale, weight, weight_scale, bias | None, residual | None, activation, bf16)
+// The type of results, as a number of fla_dtype
+at::ScalarType result_type(PyObject* o) {
+  const long t = arg_long(o);
+  return t == FLA_F32 ? at::kFloat : t == FLA_BF16 ? at::kBFloat16 : at::kHalf;
+}
+// Whether pairs of rows in 8 bits and their scales are of one type and of the shapes of a product; whether it is integers
+bool int8_rows(const char* who, const Tensor& x, const Tensor& sx, std::initializer_list<const Tensor*> ws, std::initializer_list<const Tensor*> sws) {
+  const bool known = x.defined() && (x.scalar_type() == at::kFloat8_e4m3fn || x.scalar_type() == at::kChar);
+  bool one = known && sx.defined() && sx.scalar_type() == at::kFloat;
+  for (const Tensor* w : ws) one = one && w->defined() && w->scalar_type() == x.scalar_type();
+  for (const Tensor* s : sws) one = one && s->defined() && s->scalar_type() == at::kFloat;
+  TORCH_CHECK_TYPE(one, who, ": x and weight are pairs of rows in torch.float8_e4m3fn, or in torch.int8, and their fp32 scales");
+  const Tensor& first = **ws.begin();
+  for (const Tensor* w : ws)
+    TORCH_CHECK_VALUE(x.dim() >= 1 && w->dim() == 2 && w->size(1) == x.size(-1) && w->size(0) > 0 && w->sizes() == first.sizes(), who,
+                      ": x is [..., K], weight [N, K]");
+  TORCH_CHECK_VALUE(sx.sizes() == x.sizes().slice(0, x.dim() - 1), who, ": one scale for every row of x and of weight");
+  for (const Tensor* s : sws)
+    TORCH_CHECK_VALUE(s->dim() == 1 && s->size(0) == first.size(0), who, ": one scale for every row of x and of weight");
+  const bool ints = x.scalar_type() == at::kChar;
+  const int64_t K = x.size(-1), most = ints ? FLA_INT8_MAX_K : 1 << 23;
+  TORCH_CHECK_NOT_IMPLEMENTED(K > 0 && K % 16 == 0 && K <= most, who, ": rows of a multiple of 16 elements, at most ", most, ", not ", K);
+  return ints;
+}
+
+// quant_linear(x, x_scale, weight, weight_scale, bias | None, residual | None, activation, type)
 PyObject* py_quant_linear(PyObject*, PyObject* const* p, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   expect(n, 8);
   Tensor x = arg_tensor(p[0]), sx = arg_tensor(p[1]), w = arg_tensor(p[2]), sw = arg_tensor(p[3]), bias = arg_tensor(p[4]),
          res = arg_tensor(p[5]);
   const long act = arg_long(p[6]);
-  const auto type = arg_bool(p[7]) ? at::kBFloat16 : at::kHalf;
-  TORCH_CHECK_TYPE(x.defined() && w.defined() && sx.defined() && sw.defined() && x.scalar_type() == at::kFloat8_e4m3fn &&
-                       w.scalar_type() == at::kFloat8_e4m3fn && sx.scalar_type() == at::kFloat && sw.scalar_type() == at::kFloat,
-                   "fla_amd quant_linear: x and weight are pairs of rows in torch.float8_e4m3fn and their fp32 scales");
-  TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && w.size(1) == x.size(-1) && w.size(0) > 0,
-                    "fla_amd quant_linear: x is [..., K], weight [N, K]");
+  const auto type = result_type(p[7]);
+  const bool ints = int8_rows("fla_amd quant_linear", x, sx, {&w}, {&sw});
   const int64_t K = x.size(-1), N = w.size(0);
-  TORCH_CHECK_VALUE(sx.sizes() == x.sizes().slice(0, x.dim() - 1) && sw.dim() == 1 && sw.size(0) == N,
-                    "fla_amd quant_linear: one scale for every row of x and of weight");
-  TORCH_CHECK_NOT_IMPLEMENTED(K > 0 && K % 16 == 0 && K <= 1 << 23,
-                              "fla_amd quant_linear: rows of a multiple of 16 elements, at most 2^23, not ", K);
+  TORCH_CHECK_NOT_IMPLEMENTED(ints || type != at::kFloat, "fla_amd quant_linear: results of torch.float8_e4m3fn rows in bf16 or fp16");
+  TORCH_CHECK_NOT_IMPLEMENTED(!ints || N <= 1 << 22, "fla_amd quant_linear: integer weights of at most 2^22 rows");
   if (bias.defined()) {
     TORCH_CHECK_VALUE(bias.dim() == 1 && bias.size(0) == N, "fla_amd quant_linear: bias holds ", N, " values");
     TORCH_CHECK_TYPE(bias.is_floating_point(), "fla_amd quant_linear: bias in a floating type");
@@ -1410,22 +1429,62 @@ PyObject* py_quant_linear(PyObject*, PyObject* const* p, Py_ssize_t n) {
               "fla_amd: products of 8-bit rows have no gradient; call them under torch.no_grad()");
   c10::DeviceGuard on_device(x.device());
   at::AutoDispatchBelowADInplaceOrView guard;
-  auto aligned = [](const Tensor& t) {
-    const Tensor c = t.contiguous();
-    return (uintptr_t)c.data_ptr() % 16 == 0 ? c : c.clone();
-  };
   Tensor y = at::empty(shape, x.options().dtype(type));
   if (y.numel() == 0) return THPVariable_Wrap(y);
-  x = aligned(x), w = aligned(w), sx = sx.contiguous(), sw = sw.contiguous();
+  x = whole_rows(x), w = whole_rows(w), sx = sx.contiguous(), sw = sw.contiguous();
   if (bias.defined()) bias = (bias.scalar_type() == type ? bias : f32(bias)).contiguous();
   if (res.defined()) res = res.contiguous();
   const int64_t M = x.numel() / K;
-  const int splits = fla_quant_linear_splits(M, N, K);
-  const Tensor sums = splits > 1 ? fresh({splits, M, N}, x, at::kFloat) : Tensor();
-  check(fla_quant_linear(ptr(x), fptr(sx), ptr(w), fptr(sw), ptr(bias), bias.defined() ? dt(bias) : FLA_F32, ptr(res),
-                         res.defined() ? dt(res) : FLA_F32, ptr(y), M, N, K, (int)act, dt(y), fptr(sums), stream_of(x)),
-        "fla_quant_linear");
+  const int splits = ints ? fla_int8_linear_splits(M, N, K) : fla_quant_linear_splits(M, N, K);
+  const Tensor sums = splits > 1 ? fresh({splits, M, N}, x, ints ? at::kInt : at::kFloat) : Tensor();
+  const int bt = bias.defined() ? dt(bias) : FLA_F32, rt = res.defined() ? dt(res) : FLA_F32;
+  if (ints)
+    check(fla_int8_linear(ptr(x), fptr(sx), ptr(w), fptr(sw), ptr(bias), bt, ptr(res), rt, ptr(y), M, N, K, (int)act, dt(y), ptr(sums), stream_of(x)),
+          "fla_int8_linear");
+  else
+    check(fla_quant_linear(ptr(x), fptr(sx), ptr(w), fptr(sw), ptr(bias), bt, ptr(res), rt, ptr(y), M, N, K, (int)act, dt(y), fptr(sums), stream_of(x)),
+          "fla_quant_linear");
   return THPVariable_Wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// quant_gated_linear(x, x_scale, gate_weight, gate_scale, up_weight, up_scale, gate_bias | None, up_bias | None, activation, type)
+PyObject* py_quant_gated_linear(PyObject*, PyObject* const* p, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  expect(n, 10);
+  Tensor x = arg_tensor(p[0]), sx = arg_tensor(p[1]), wg = arg_tensor(p[2]), sg = arg_tensor(p[3]), wu = arg_tensor(p[4]), su = arg_tensor(p[5]),
+         bg = arg_tensor(p[6]), bu = arg_tensor(p[7]);
+  const long act = arg_long(p[8]);
+  const auto type = result_type(p[9]);
+  const bool ints = int8_rows("fla_amd quant_gated_linear", x, sx, {&wg, &wu}, {&sg, &su});
+  TORCH_CHECK_NOT_IMPLEMENTED(ints, "fla_amd quant_gated_linear: rows in torch.int8");
+  const int64_t K = x.size(-1), F = wg.size(0), M = x.numel() / K;
+  TORCH_CHECK_NOT_IMPLEMENTED(F <= 1 << 22, "fla_amd quant_gated_linear: weights of at most 2^22 rows");
+  for (const Tensor* t : {&bg, &bu}) {
+    if (!t->defined()) continue;
+    TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == F, "fla_amd quant_gated_linear: biases hold ", F, " values");
+    TORCH_CHECK_TYPE(t->is_floating_point(), "fla_amd quant_gated_linear: biases in a floating type");
+  }
+  need_gpu({&x, &sx, &wg, &sg, &wu, &su, &bg, &bu});
+  TORCH_CHECK(!wants_grad({&sx, &sg, &su, &bg, &bu}), "fla_amd: products of 8-bit rows have no gradient; call them under torch.no_grad()");
+  c10::DeviceGuard on_device(x.device());
+  at::AutoDispatchBelowADInplaceOrView guard;
+  auto shape = x.sizes().vec();
+  shape.back() = F;
+  Tensor h = at::empty(shape, x.options().dtype(type));
+  if (h.numel() == 0) return THPVariable_Wrap(h);
+  x = whole_rows(x), wg = whole_rows(wg), wu = whole_rows(wu), sx = sx.contiguous(), sg = sg.contiguous(), su = su.contiguous();
+  auto fits = [&](const Tensor& t) { return !t.defined() || t.scalar_type() == type; };
+  const bool same = fits(bg) && fits(bu);
+  if (!same) bg = f32(bg), bu = f32(bu);
+  if (bg.defined()) bg = bg.contiguous();
+  if (bu.defined()) bu = bu.contiguous();
+  const int splits = fla_gated_linear_splits(M, F, K, 1);
+  const Tensor sums = splits > 1 ? fresh({splits, M, 2, F}, x, at::kInt) : Tensor();
+  check(fla_int8_gated_linear_fwd(ptr(x), fptr(sx), ptr(wg), fptr(sg), ptr(wu), fptr(su), ptr(bg), ptr(bu), same ? dt(h) : FLA_F32, ptr(h), M, F, K,
+                                  (int)act, dt(h), ptr(sums), stream_of(x)),
+        "fla_int8_gated_linear_fwd");
+  return THPVariable_Wrap(h);
   END_HANDLE_TH_ERRORS
 }
 
@@ -1474,6 +1533,7 @@ PyMethodDef kMethods[] = {
     ENTRY("norm", py_norm),
     ENTRY("quant_linear", py_quant_linear),
     ENTRY("gated_linear", py_gated_linear),
+    ENTRY("quant_gated_linear", py_quant_gated_linear),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fla_host", nullptr, -1, kMethods};
 

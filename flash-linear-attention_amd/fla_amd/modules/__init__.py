@@ -8,7 +8,7 @@ from .gate_activations import gdn_gate, gdn_gate_bwd, gdn_gate_fwd, gla_gate, gl
 from .gated_mlp import GatedMLP, gated_linear
 from .l2norm import L2NormFunction, l2_norm, l2norm_bwd, l2norm_fwd
 from .layernorm import LayerNorm, RMSNorm, layer_norm, quantize_rows, rms_norm
-from .quant_linear import QuantLinear, quant_linear
+from .quant_linear import QuantLinear, quant_gated_linear, quant_linear
 
 __all__ = [
     "ShortConvolution", "causal_conv1d", "causal_conv1d_update",
@@ -17,6 +17,6 @@ __all__ = [
     "L2NormFunction", "l2_norm", "l2norm_fwd", "l2norm_bwd",
     "gla_gate", "gla_gate_fwd", "gla_gate_bwd", "gdn_gate", "gdn_gate_fwd", "gdn_gate_bwd",
     "RMSNorm", "rms_norm", "LayerNorm", "layer_norm", "quantize_rows",
-    "QuantLinear", "quant_linear",
+    "QuantLinear", "quant_linear", "quant_gated_linear",
     "GatedMLP", "gated_linear",
 ]

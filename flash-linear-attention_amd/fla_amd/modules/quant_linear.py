@@ -1,5 +1,5 @@
-"""Projections with operands in 8 bits, for serving: rows of ``x`` and of the weight in ``torch.float8_e4m3fn`` with a scale each, bias, activation
-and residual in the product's epilogue."""
+"""Projections with operands in 8 bits, for serving: rows of ``x`` and of the weight in ``torch.float8_e4m3fn`` or in ``torch.int8`` with a scale each, bias,
+activation and residual in the product's epilogue; and the gated product of rows in integers."""
 from __future__ import annotations
 
 from typing import Optional, Tuple, Union
@@ -11,6 +11,8 @@ from .._native import host
 from .layernorm import quantize_rows
 
 _ACTIVATIONS = {None: 0, "silu": 1, "swish": 1, "gelu": 2, "relu": 3}
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}     # enum fla_dtype
+_MOST = {torch.float8_e4m3fn: 1 << 23, torch.int8: 131056}           # elements of a row
 Rows = Tuple[torch.Tensor, torch.Tensor]
 
 
@@ -19,42 +21,63 @@ def quant_linear(x: Rows, weight: Rows, bias: Optional[torch.Tensor] = None, act
     """``act(x @ weight.T + bias) + residual`` for ``x`` ``[..., K]`` and ``weight`` ``[N, K]``, each a pair ``(q, scale)`` as
     :func:`quantize_rows` and :func:`rms_norm` with ``quantize=True`` return it.
 
+    Rows of both in ``torch.float8_e4m3fn``, or of both in ``torch.int8`` (``quantize=torch.int8``), a scale for each token and each channel.
+
     ``activation``: ``None``, ``"silu"`` (``"swish"``), ``"gelu"`` (of the error function) or ``"relu"``; ``residual`` ``[..., N]`` and ``bias`` in the
-    output's type or in fp32; ``output_dtype`` bf16 or fp16 (the matrix instruction's sums of 8-bit products hold about 16 bits, fp32
-    results are refused).  ``K`` in multiples of 16, at most 2^23.  The matrix instruction cuts each
+    output's type or in fp32; ``output_dtype`` bf16 or fp16, and fp32 for integers (the matrix instruction's sums of e4m3 products hold about 16 bits, fp32
+    results are refused).  ``K`` in multiples of 16, at most 2^23, of integers at most 131056 (beyond that a sum could pass 2^31; below it sums of integers are exact).
+    Of e4m3 the matrix instruction cuts each
     product at 2^-13 of the largest of the eight it adds at once, the sums of eight are added in fp32: 1.2e-5 of a sum, 1/40 of half a step of
     fp16.  One launch, or two where there are few tiles and K is summed in slices.  There is no gradient, and a call that wants one is refused."""
     if activation not in _ACTIVATIONS:
         raise ValueError(f"fla_amd quant_linear: unknown activation {activation!r}")
+    if output_dtype not in _TYPES or (output_dtype is torch.float32 and x[0].dtype is not torch.int8):
+        raise NotImplementedError(f"fla_amd quant_linear: results in bf16 or fp16, of integers also in fp32, not {output_dtype}")
+    return host().quant_linear(x[0], x[1], weight[0], weight[1], bias, residual, _ACTIVATIONS[activation], _TYPES[output_dtype])
+
+
+def quant_gated_linear(x: Rows, gate_weight: Rows, up_weight: Rows, gate_bias: Optional[torch.Tensor] = None, up_bias: Optional[torch.Tensor] = None,
+                       activation: Optional[str] = "silu", output_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """:func:`gated_linear` for serving: ``act(x @ gate_weight.T + gate_bias) * (x @ up_weight.T + up_bias)``, ``x`` ``[..., K]`` and both weights
+    ``[F, K]`` pairs ``(q, scale)`` in ``torch.int8`` as :func:`quantize_rows` and the norms return them.  Results in bf16 or fp16; biases in any floating
+    type.  ``K`` in multiples of 16, at most 131056; sums are exact.  There is no gradient, and a call that wants one is refused."""
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"fla_amd quant_gated_linear: unknown activation {activation!r}")
     if output_dtype not in (torch.bfloat16, torch.float16):
-        raise NotImplementedError(f"fla_amd quant_linear: results in bf16 or fp16, not {output_dtype}")
-    return host().quant_linear(x[0], x[1], weight[0], weight[1], bias, residual, _ACTIVATIONS[activation], output_dtype is torch.bfloat16)
+        raise NotImplementedError(f"fla_amd quant_gated_linear: results in bf16 or fp16, not {output_dtype}")
+    return host().quant_gated_linear(x[0], x[1], gate_weight[0], gate_weight[1], up_weight[0], up_weight[1], gate_bias, up_bias,
+                                     _ACTIVATIONS[activation], _TYPES[output_dtype])
 
 
 class QuantLinear(nn.Module):
     """A ``torch.nn.Linear`` for serving with its weight in 8 bits: ``forward(x, residual=None)`` takes 16-bit or fp32 rows, which it quantises first,
-    or the pair that a norm with ``quantize=True`` returned.  ``in_features`` in multiples of 16, at most 2^23."""
+    or the pair that a norm with ``quantize`` returned.  ``dtype``: ``torch.float8_e4m3fn`` or ``torch.int8``, of the weight and of the rows.
+    ``in_features`` in multiples of 16, at most 2^23, of integers at most 131056."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, activation: Optional[str] = None,
-                 output_dtype: torch.dtype = torch.bfloat16, device=None):
+                 output_dtype: torch.dtype = torch.bfloat16, device=None, dtype: torch.dtype = torch.float8_e4m3fn):
         super().__init__()
         if activation not in _ACTIVATIONS:
             raise ValueError(f"fla_amd quant_linear: unknown activation {activation!r}")
-        if in_features <= 0 or in_features % 16 or in_features > 1 << 23:
-            raise NotImplementedError(f"fla_amd quant_linear: rows of a multiple of 16 elements, at most 2^23, not {in_features}")
+        if dtype not in _MOST:
+            raise ValueError(f"fla_amd quant_linear: weights in torch.float8_e4m3fn or torch.int8, not {dtype}")
+        if in_features <= 0 or in_features % 16 or in_features > _MOST[dtype]:
+            most = "at most 2^23" if dtype is torch.float8_e4m3fn else f"at most {_MOST[dtype]}"
+            raise NotImplementedError(f"fla_amd quant_linear: rows of a multiple of 16 elements, {most}, not {in_features}")
         self.in_features, self.out_features, self.activation, self.output_dtype = in_features, out_features, activation, output_dtype
-        self.register_buffer("weight", torch.zeros(out_features, in_features, device=device).to(torch.float8_e4m3fn))
+        self.register_buffer("weight", torch.zeros(out_features, in_features, device=device).to(dtype))
         self.register_buffer("weight_scale", torch.zeros(out_features, device=device))
         self.register_buffer("bias", torch.zeros(out_features, device=device) if bias else None)
 
     @classmethod
     @torch.no_grad()
-    def from_linear(cls, linear: nn.Linear, activation: Optional[str] = None, output_dtype: Optional[torch.dtype] = None) -> "QuantLinear":
+    def from_linear(cls, linear: nn.Linear, activation: Optional[str] = None, output_dtype: Optional[torch.dtype] = None,
+                    dtype: torch.dtype = torch.float8_e4m3fn) -> "QuantLinear":
         """The layer with ``linear``'s weight rounded to 8 bits, row by row, on its device."""
         if output_dtype is None:
             output_dtype = linear.weight.dtype if linear.weight.dtype in (torch.bfloat16, torch.float16) else torch.bfloat16
-        new = cls(linear.in_features, linear.out_features, linear.bias is not None, activation, output_dtype, linear.weight.device)
-        new.weight, new.weight_scale = quantize_rows(linear.weight)
+        new = cls(linear.in_features, linear.out_features, linear.bias is not None, activation, output_dtype, linear.weight.device, dtype)
+        new.weight, new.weight_scale = quantize_rows(linear.weight, dtype)
         if linear.bias is not None:
             new.bias = linear.bias.detach().clone()
         return new
@@ -74,5 +97,5 @@ class QuantLinear(nn.Module):
 
     def forward(self, x: Union[torch.Tensor, Rows], residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         if isinstance(x, torch.Tensor):
-            x = quantize_rows(x)
+            x = quantize_rows(x, self.weight.dtype)
         return quant_linear(x, (self.weight, self.weight_scale), self.bias, self.activation, residual, self.output_dtype)

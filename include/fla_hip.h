@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define FLA_ABI_VERSION 25
+#define FLA_ABI_VERSION 26
 
 enum fla_dtype { FLA_F32 = 0, FLA_BF16 = 1, FLA_F16 = 2 };
 
@@ -881,6 +881,14 @@ int fla_quant_linear(const void* x, const float* x_scale, const void* weight, co
                      int bias_dtype, const void* residual, int residual_dtype, void* y, int64_t M, int64_t N, int64_t K,
                      int activation, int dtype, float* workspace, fla_stream_t stream);
 
+/* Product of rows in 8-bit integers (FLA_ROWS_INT8), as above but for: sums are exact (int32), K % 16 == 0 and K <= FLA_INT8_MAX_K, beyond which a
+ * sum could pass 2^31; N <= 2^22; y in fp32 too; workspace: int32 [fla_int8_linear_splits, M, N] at a 16-byte address where they are more than one. */
+#define FLA_INT8_MAX_K 131056
+int fla_int8_linear_splits(int64_t M, int64_t N, int64_t K);
+int fla_int8_linear(const void* x, const float* x_scale, const void* weight, const float* weight_scale, const void* bias,
+                    int bias_dtype, const void* residual, int residual_dtype, void* y, int64_t M, int64_t N, int64_t K,
+                    int activation, int dtype, void* workspace, fla_stream_t stream);
+
 /* ------------------------------------------------------------------------
  * The gated product of a feed-forward block (no counterpart in the reference in one operator: its
  * blocks call torch.nn.Linear twice and the activation of fla/modules/activations.py):
@@ -901,6 +909,11 @@ int fla_gated_linear_splits(int64_t M, int64_t F, int64_t K, int element_bytes);
 int fla_gated_linear_fwd(const void* x, const void* gate_weight, const void* up_weight, const void* gate_bias, const void* up_bias,
                          int bias_dtype, void* h, void* gate_out, void* up_out, int64_t ld, int64_t M, int64_t F, int64_t K,
                          int activation, int dtype, void* workspace, fla_stream_t stream);
+/* The same of rows in 8-bit integers, x and both weights with a scale per row (see fla_int8_linear); h in bf16 or fp16. */
+int fla_int8_gated_linear_fwd(const void* x, const float* x_scale, const void* gate_weight, const float* gate_scale,
+                              const void* up_weight, const float* up_scale, const void* gate_bias, const void* up_bias,
+                              int bias_dtype, void* h, int64_t M, int64_t F, int64_t K, int activation, int dtype, void* workspace,
+                              fla_stream_t stream);
 int fla_gated_linear_bwd_rows(int64_t M);
 int fla_gated_linear_bwd_gate(const void* dh, const void* gate, const void* up, void* dgate, void* dup, float* dgate_bias_partial,
                               float* dup_bias_partial, int64_t ld, int64_t M, int64_t F, int activation, int dtype,
