@@ -32,110 +32,130 @@ FLA_DEVICE float gated_bias(const void* b, int f32, int64_t n, int64_t F) {
 }
 
 // T: type of the operands, O: of h
-template <typename T, typename O, int BM, int BN, int PER_SIMD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PER_SIMD, PER_SIMD))) void gated_tile_kernel(GatedParams p) {
-  typedef MatTile<T, BM, BN, 2, false, false, true> Tile;
-  constexpr bool INT = sizeof(T) == 1;
-  constexpr int HN = BN / 2;      // columns of h
-  __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
-  uint32_t tm, tn;
-  mat_tile_of(blockIdx.x, (uint32_t)((p.M + BM - 1) / BM), (uint32_t)((p.F + HN - 1) / HN), &tm, &tn);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * HN;
-  const int pitch = (int)(p.K * sizeof(T));
-  typename Tile::OpM om;
-  typename Tile::OpN on;
-  om.start(wave, lane, pitch);
-  on.start(wave, lane, pitch);
-  const char *xb = p.x + m0 * pitch, *gb = p.wg + n0 * pitch, *ub = p.wu + n0 * pitch;
-  const char *xe = p.x + p.M * pitch, *ge = p.wg + p.F * pitch, *ue = p.wu + p.F * pitch;
-  const int slices = (pitch + kSliceBytes - 1) / kSliceBytes, per = (slices + p.splits - 1) / p.splits;
-  const int first = blockIdx.y * per, last = first + per < slices ? first + per : slices;
-  typename Tile::acc_t acc[Tile::MT][Tile::NT];
-  Tile::run(lds, om, on, first, last, [&](int s, MatSource* m, MatSource* n) {
-    const int k = s * kSliceBytes;
-    m[0] = MatSource{xb + k, xe, pitch - k};
-    n[0] = MatSource{gb + k, ge, pitch - k};
-    n[1] = MatSource{ub + k, ue, pitch - k};
-  }, acc);
+template <typename T, typename O, int BM, int BN, bool HALVES>
+struct GatedJob {
+  static constexpr bool INT = sizeof(T) == 1, kHalves = HALVES;
+  static constexpr int HN = BN / 2;                     // columns of h
+  typedef MatTile<T, BM, BN, 2, false, false, true> Whole;
+  typedef MatTile<T, BM, HALVES ? BN / 2 : BN, 2, false, false, true> Half;
+  static constexpr int LATER = Whole::MT * Whole::NT;   // stores of h
+  static constexpr int kLds = Whole::kLds + 2 * 4 * HN * 4;
 
-  const int wm = wave >> 1, wn = wave & 1, lr = lane & 31, lh = lane >> 5;
-  const int64_t mw = m0 + wm * (BM / 2) + lr;
-  if (p.splits > 1) {   // gated_finish_kernel adds the slices' sums
-    typedef typename std::conditional<INT, int, float>::type S;
-    S* part = (S*)p.part + blockIdx.y * p.M * 2 * p.F;
+  const GatedParams& p;
+  char* lds;
+  int first, last, pitch;
+  int64_t m0, n0;
+  template <typename Tile>
+  FLA_DEVICE void start(Tile& t) const { t.start(pitch, pitch); }
+  FLA_DEVICE void at(uint32_t tm, uint32_t n) { m0 = (int64_t)tm * BM, n0 = (int64_t)n * (HN / 2); }
+  FLA_DEVICE void source(int s, MatSource* m, MatSource* n) const {
+    const int k = s * kSliceBytes;
+    m[0] = MatSource{p.x + m0 * pitch + k, p.x + p.M * pitch, pitch - k};
+    n[0] = MatSource{p.wg + n0 * pitch + k, p.wg + p.F * pitch, pitch - k};
+    n[1] = MatSource{p.wu + n0 * pitch + k, p.wu + p.F * pitch, pitch - k};
+  }
+  // Biases and scales of the columns: a wave each, as they lie in memory; zeros where there are none
+  FLA_DEVICE char* column(int side, int which) const { return lds + Whole::kLds + (side * 4 + which) * HN * 4; }
+  FLA_DEVICE void columns(int side) const {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const char* from = (const char*)(wave == 0 ? p.bg : wave == 1 ? p.bu : wave == 2 ? (const void*)p.sg : (const void*)p.su);
+    const int e = wave >= 2 || p.bias_f32 ? 4 : (int)sizeof(O);
+    const __amdgpu_buffer_rsrc_t d = MatSource{from + n0 * e, from ? from + (p.F * e + 3) / 4 * 4 : nullptr, 0}.descriptor();   // (whole words)
 #pragma unroll
-    for (int i = 0; i < Tile::MT; ++i)
+    for (int q = 0; q < HN * 4 / 256; ++q)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(d, (__attribute__((address_space(3))) void*)(column(side, wave) + q * 256), 4, q * 256 + lane * 4, 0, 0, 0);
+  }
+  FLA_DEVICE f32x4 bias4(int side, int which, int n) const {
+    const char* c = column(side, which);
+    if (p.bias_f32) return *(const f32x4*)(c + n * 4);
+    const typename Elem<O>::v4 v = *(const typename Elem<O>::v4*)(c + n * 2);
+    return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+  }
+  // true: every store was made, and only those of h
+  template <typename Tile>
+  FLA_DEVICE bool finish(const Tile& t, const typename Tile::acc_t (&acc)[Tile::MT][Tile::NT], int side) const {
+    constexpr int TN = Tile::NT * 32;      // columns of h of the tile
+    const int lr = t.lane & 31, lh = t.lane >> 5;
+    const int64_t mw = m0 + t.wm * (BM / 2) + lr;
+    if (p.splits > 1) {   // gated_finish_kernel adds the slices' sums
+      typedef typename std::conditional<INT, int, float>::type S;
+      S* part = (S*)p.part + blockIdx.y * p.M * 2 * p.F;
 #pragma unroll
-      for (int j = 0; j < Tile::NT; ++j)
+      for (int i = 0; i < Tile::MT; ++i)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          typedef S S4 __attribute__((ext_vector_type(4), aligned(4)));
-          const int64_t m = mw + i * 32, n = n0 + wn * (HN / 2) + j / 2 * 32 + 8 * q + 4 * lh;
-          S* to = part + (m * 2 + j % 2) * p.F + n;
-          if (m < p.M && n + 4 <= p.F) {
-            *(S4*)to = S4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-          } else if (m < p.M) {
+        for (int j = 0; j < Tile::NT; ++j) {
+          const typename Tile::acc_t a = mat_sums<Tile>(acc, i, j);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (n + r < p.F) to[r] = acc[i][j][4 * q + r];
+          for (int q = 0; q < 4; ++q) {
+            typedef S S4 __attribute__((ext_vector_type(4), aligned(4)));
+            const int64_t m = mw + i * 32, n = n0 + t.wn * (TN / 2) + j / 2 * 32 + 8 * q + 4 * lh;
+            S* to = part + (m * 2 + j % 2) * p.F + n;
+            if (m < p.M && n + 4 <= p.F) {
+              *(S4*)to = S4{a[4 * q], a[4 * q + 1], a[4 * q + 2], a[4 * q + 3]};
+            } else if (m < p.M) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (n + r < p.F) to[r] = a[4 * q + r];
+            }
           }
+          mat_piece_end();
         }
-    return;
-  }
-  // biases and scales of the columns, behind everybody's last read of the slices
-  __syncthreads();
-  float *bgs = (float*)lds, *bus = bgs + HN, *sgs = bus + HN, *sus = sgs + HN;
-  for (int i = threadIdx.x; i < HN; i += 256) {
-    bgs[i] = gated_bias<O>(p.bg, p.bias_f32, n0 + i, p.F);
-    bus[i] = gated_bias<O>(p.bu, p.bias_f32, n0 + i, p.F);
-    if (INT) {
-      sgs[i] = n0 + i < p.F ? p.sg[n0 + i] : 0.f;
-      sus[i] = n0 + i < p.F ? p.su[n0 + i] : 0.f;
+      return false;
     }
-  }
-  __syncthreads();
-  with_activation(p.act, [&](auto act) {
+    with_activation(p.act, [&](auto act) {
 #pragma unroll
-    for (int i = 0; i < Tile::MT; ++i) {
-      const int64_t m = mw + i * 32;
-      const float sx = INT && m < p.M ? p.sx[m] : 1.f;
+      for (int i = 0; i < Tile::MT; ++i) {
+        const int64_t m = mw + i * 32;
+        const float sx = INT && m < p.M ? p.sx[m] : 1.f;
 #pragma unroll
-      for (int h = 0; h < Tile::NT / 2; ++h)
+        for (int h = 0; h < Tile::NT / 2; ++h) {
+          const typename Tile::acc_t gs = mat_sums<Tile>(acc, i, 2 * h), us = mat_sums<Tile>(acc, i, 2 * h + 1);
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int nl = wn * (HN / 2) + h * 32 + 16 * q + 4 * lh;     // of the first run of four; the second is eight further
-          u32x2 hv[2], gv[2], uv[2];
+          for (int q = 0; q < 2; ++q) {
+            const int nl = t.wn * (TN / 2) + h * 32 + 16 * q + 4 * lh;     // of the first run of four; the second is eight further
+            u32x2 hv[2], gv[2], uv[2];
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const f32x4 bg = *(const f32x4*)(bgs + nl + 8 * e), bu = *(const f32x4*)(bus + nl + 8 * e);
-            float g[4], u[4], v[4];
+            for (int e = 0; e < 2; ++e) {
+              const f32x4 bg = bias4(side, 0, nl + 8 * e), bu = bias4(side, 1, nl + 8 * e);
+              f32x4 sg, su;
+              if (INT) sg = *(const f32x4*)(column(side, 2) + (nl + 8 * e) * 4), su = *(const f32x4*)(column(side, 3) + (nl + 8 * e) * 4);
+              float g[4], u[4], v[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              g[r] = (float)acc[i][2 * h][8 * q + 4 * e + r], u[r] = (float)acc[i][2 * h + 1][8 * q + 4 * e + r];
-              if (INT) {
-                g[r] = fmaf(g[r], sx * sgs[nl + 8 * e + r], bg[r]);
-                u[r] = fmaf(u[r], sx * sus[nl + 8 * e + r], bu[r]);
-              } else {
-                g[r] += bg[r], u[r] += bu[r];
+              for (int r = 0; r < 4; ++r) {
+                g[r] = (float)gs[8 * q + 4 * e + r], u[r] = (float)us[8 * q + 4 * e + r];
+                if (INT) g[r] = fmaf(g[r], sx * sg[r], bg[r]), u[r] = fmaf(u[r], sx * su[r], bu[r]);
+                else g[r] += bg[r], u[r] += bu[r];
+                v[r] = activate_gate<decltype(act)::value>(g[r]) * u[r];
               }
-              v[r] = activate_gate<decltype(act)::value>(g[r]) * u[r];
+              hv[e] = pack4<O>(v), gv[e] = pack4<O>(g), uv[e] = pack4<O>(u);
             }
-            hv[e] = pack4<O>(v), gv[e] = pack4<O>(g), uv[e] = pack4<O>(u);
-          }
-          const i32x4 ho = mat_join(hv[0], hv[1]);
-          const int64_t n = n0 + wn * (HN / 2) + h * 32 + 16 * q + 8 * lh;
-          if (m < p.M) store_piece((O*)p.h + m * p.F, n, p.F, p.wide, ho);
-          if (!INT && p.g) {
-            const i32x4 go = mat_join(gv[0], gv[1]), uo = mat_join(uv[0], uv[1]);
-            if (m < p.M) {
-              store_piece((O*)p.g + m * p.ldk, n, p.ldk, true, go);
-              store_piece((O*)p.u + m * p.ldk, n, p.ldk, true, uo);
+            const i32x4 ho = mat_join(hv[0], hv[1]);
+            const int64_t n = n0 + t.wn * (TN / 2) + h * 32 + 16 * q + 8 * lh;
+            if (m < p.M) store_piece((O*)p.h + m * p.F, n, p.F, p.wide, ho);
+            if (!INT && p.g) {
+              const i32x4 go = mat_join(gv[0], gv[1]), uo = mat_join(uv[0], uv[1]);
+              if (m < p.M) {
+                store_piece((O*)p.g + m * p.ldk, n, p.ldk, true, go);
+                store_piece((O*)p.u + m * p.ldk, n, p.ldk, true, uo);
+              }
             }
+            mat_piece_end();
           }
         }
-    }
-  });
+      }
+    });
+    return !INT && !p.g && p.wide && m0 + BM <= p.M && n0 + TN <= p.F;
+  }
+};
+
+template <typename T, typename O, int BM, int BN, int PER_SIMD, bool HALVES>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PER_SIMD, PER_SIMD))) void gated_tile_kernel(GatedParams p, MatGrid grid) {
+  typedef GatedJob<T, O, BM, BN, HALVES> Job;
+  __shared__ __attribute__((aligned(1024))) char lds[Job::kLds];
+  const int pitch = (int)(p.K * sizeof(T)), slices = (pitch + kSliceBytes - 1) / kSliceBytes, per = (slices + p.splits - 1) / p.splits;
+  const int first = blockIdx.y * per;
+  Job job{p, lds, first, first + per < slices ? first + per : slices, pitch, 0, 0};
+  mat_run(lds, grid, job);
 }
 
 // h (g, u) from the sums of slices of K, added in their order: four columns a thread
@@ -265,88 +285,111 @@ struct GradParams {
   int splits;
 };
 
-template <typename T, int BM, int BN, typename Tile>
-FLA_DEVICE void grad_store(const typename Tile::acc_t (&acc)[Tile::MT][Tile::NT], T* y, float* part, int64_t m0, int64_t n0, int64_t rows, int64_t K) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
-  const int lr = lane & 31, lh = lane >> 5;
+// A tile of a gradient of `rows` rows of K elements; true: every store was made, 16 bytes each
+template <typename T, typename Tile>
+FLA_DEVICE bool grad_store(const Tile& t, const typename Tile::acc_t (&acc)[Tile::MT][Tile::NT], T* y, float* part, int64_t m0, int64_t n0, int64_t rows, int64_t K) {
+  const int lr = t.lane & 31, lh = t.lane >> 5;
 #pragma unroll
   for (int i = 0; i < Tile::MT; ++i) {
-    const int64_t m = m0 + wm * (BM / 2) + i * 32 + lr;
+    const int64_t m = m0 + (t.wm * Tile::MT + i) * 32 + lr;
 #pragma unroll
     for (int j = 0; j < Tile::NT; ++j) {
-      const int64_t n = n0 + wn * (BN / 2) + j * 32;
+      const int64_t n = n0 + (t.wn * Tile::NT + j) * 32;
+      const typename Tile::acc_t v = mat_sums<Tile>(acc, i, j);
       if (part) {
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           if (m < rows && n + 8 * q + 4 * lh < K)
-            *(f32x4*)(part + m * K + n + 8 * q + 4 * lh) = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+            *(f32x4*)(part + m * K + n + 8 * q + 4 * lh) = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
       } else {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           float a[4], b[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) a[r] = acc[i][j][8 * q + r], b[r] = acc[i][j][8 * q + 4 + r];
+          for (int r = 0; r < 4; ++r) a[r] = v[8 * q + r], b[r] = v[8 * q + 4 + r];
           const i32x4 o = mat_join(pack4<T>(a), pack4<T>(b));
           if (m < rows && n + 16 * q + 8 * lh < K) *(i32x4*)(y + m * K + n + 16 * q + 8 * lh) = o;      // (K is a multiple of 8)
         }
       }
+      mat_piece_end();
     }
   }
+  return !part && m0 + Tile::MT * 64 <= rows && n0 + Tile::NT * 64 <= K;
 }
 
 // dx = dg Wg + du Wu: the slices of the first product, then those of the second
-template <typename T, int BM, int BN, int PER_SIMD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PER_SIMD, PER_SIMD))) void gated_dx_kernel(GradParams p) {
-  typedef MatTile<T, BM, BN, 2, false, true> Tile;
-  __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
-  uint32_t tm, tn;
-  mat_tile_of(blockIdx.x, (uint32_t)((p.M + BM - 1) / BM), (uint32_t)((p.K + BN - 1) / BN), &tm, &tn);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-  const int pitch = (int)(p.ld * 2), wp = (int)(p.K * 2);
-  typename Tile::OpM om;
-  typename Tile::OpN on;
-  om.start(wave, lane, pitch);
-  on.start(wave, lane, wp);
-  const int each = (pitch + kSliceBytes - 1) / kSliceBytes, slices = 2 * each, per = (slices + p.splits - 1) / p.splits;
-  const int first = blockIdx.y * per, last = first + per < slices ? first + per : slices;
-  const int64_t rows = m0 * pitch, all = p.M * pitch, columns = n0 * 2, weights = p.F * wp;
-  typename Tile::acc_t acc[Tile::MT][Tile::NT];
-  Tile::run(lds, om, on, first, last, [&](int s, MatSource* m, MatSource* n) {
+template <typename T, int BM, int BN, bool HALVES>
+struct DxJob {
+  static constexpr bool kHalves = HALVES;
+  typedef MatTile<T, BM, BN, 2, false, true> Whole;
+  typedef MatTile<T, BM, HALVES ? BN / 2 : BN, 2, false, true> Half;
+  static constexpr int LATER = Whole::MT * Whole::NT * 2, kLds = Whole::kLds;
+  const GradParams& p;
+  int first, last, each;     // each: slices of one of the products
+  int64_t m0, n0;
+  template <typename Tile>
+  FLA_DEVICE void start(Tile& t) const { t.start((uint32_t)(p.ld * 2), (uint32_t)(p.K * 2)); }
+  FLA_DEVICE void at(uint32_t tm, uint32_t n) { m0 = (int64_t)tm * BM, n0 = (int64_t)n * (BN / 2); }
+  FLA_DEVICE void columns(int) const {}
+  FLA_DEVICE void source(int s, MatSource* m, MatSource* n) const {
     const bool second = s >= each;
-    const int k = (second ? s - each : s) * kSliceBytes;
+    const int k = (second ? s - each : s) * kSliceBytes, pitch = (int)(p.ld * 2);
     const char *d = second ? p.du : p.dg, *w = second ? p.b : p.a;
-    m[0] = MatSource{d + rows + k, d + all, pitch - k};
-    n[0] = MatSource{w + columns + (int64_t)(k / 2) * wp, w + weights, 0};
-  }, acc);
-  grad_store<T, BM, BN, Tile>(acc, (T*)p.y, p.splits > 1 ? p.part + blockIdx.y * p.M * p.K : nullptr, m0, n0, p.M, p.K);
+    m[0] = MatSource{d + m0 * pitch + k, d + p.M * pitch, pitch - k};
+    n[0] = MatSource{w + n0 * 2 + (int64_t)(k / 2) * (p.K * 2), w + p.F * p.K * 2, 0};
+  }
+  template <typename Tile>
+  FLA_DEVICE bool finish(const Tile& t, const typename Tile::acc_t (&acc)[Tile::MT][Tile::NT], int) const {
+    return grad_store(t, acc, (T*)p.y, p.splits > 1 ? p.part + blockIdx.y * p.M * p.K : nullptr, m0, n0, p.M, p.K);
+  }
+};
+template <typename T, int BM, int BN, int PER_SIMD, bool HALVES>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PER_SIMD, PER_SIMD))) void gated_dx_kernel(GradParams p, MatGrid grid) {
+  typedef DxJob<T, BM, BN, HALVES> Job;
+  __shared__ __attribute__((aligned(1024))) char lds[Job::kLds];
+  const int each = (int)((p.ld * 2 + kSliceBytes - 1) / kSliceBytes), per = (2 * each + p.splits - 1) / p.splits, first = blockIdx.y * per;
+  Job job{p, first, first + per < 2 * each ? first + per : 2 * each, each, 0, 0};
+  mat_run(lds, grid, job);
 }
 
-// dWg = dg' x (blockIdx.z 0), dWu = du' x
-template <typename T, int BM, int BN, int PER_SIMD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PER_SIMD, PER_SIMD))) void gated_dw_kernel(GradParams p) {
-  typedef MatTile<T, BM, BN, 2, true, true> Tile;
-  __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
-  uint32_t tm, tn;
-  mat_tile_of(blockIdx.x, (uint32_t)((p.F + BM - 1) / BM), (uint32_t)((p.K + BN - 1) / BN), &tm, &tn);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-  const int64_t dp = p.ld * 2, xp = p.K * 2;
-  typename Tile::OpM om;
-  typename Tile::OpN on;
-  om.start(wave, lane, (uint32_t)dp);
-  on.start(wave, lane, (uint32_t)xp);
-  const bool up = p.y2 && (!p.y || blockIdx.z);
-  const char *d = (up ? p.du : p.dg), *db = d + m0 * 2, *de = d + p.M * dp, *xb = p.a + n0 * 2, *xe = p.a + p.M * xp;
-  const int slices = (int)((p.M + 63) / 64), per = (slices + p.splits - 1) / p.splits;
-  const int first = blockIdx.y * per, last = first + per < slices ? first + per : slices;
-  typename Tile::acc_t acc[Tile::MT][Tile::NT];
-  Tile::run(lds, om, on, first, last, [&](int s, MatSource* m, MatSource* n) {
-    m[0] = MatSource{db + (int64_t)s * 64 * dp, de, 0};
-    n[0] = MatSource{xb + (int64_t)s * 64 * xp, xe, 0};
-  }, acc);
-  grad_store<T, BM, BN, Tile>(acc, (T*)(up ? p.y2 : p.y), p.splits > 1 ? p.part + ((int64_t)blockIdx.z * p.splits + blockIdx.y) * p.F * p.K : nullptr, m0, n0,
-                              p.F, p.K);
+// dWg = dg' x and dWu = du' x, the rows of tiles of the one and then those of the other (or one of them alone)
+template <typename T, int BM, int BN, bool HALVES>
+struct DwJob {
+  static constexpr bool kHalves = HALVES;
+  typedef MatTile<T, BM, BN, 2, true, true> Whole;
+  typedef MatTile<T, BM, HALVES ? BN / 2 : BN, 2, true, true> Half;
+  static constexpr int LATER = Whole::MT * Whole::NT * 2, kLds = Whole::kLds;
+  const GradParams& p;
+  int first, last;
+  uint32_t rows;      // of tiles of one weight
+  bool up;
+  int64_t m0, n0;
+  template <typename Tile>
+  FLA_DEVICE void start(Tile& t) const { t.start((uint32_t)(p.ld * 2), (uint32_t)(p.K * 2)); }
+  FLA_DEVICE void at(uint32_t tm, uint32_t n) {
+    up = !p.y || tm >= rows;
+    m0 = (int64_t)(tm >= rows ? tm - rows : tm) * BM, n0 = (int64_t)n * (BN / 2);
+  }
+  FLA_DEVICE void columns(int) const {}
+  FLA_DEVICE void source(int s, MatSource* m, MatSource* n) const {
+    const int64_t dp = p.ld * 2, xp = p.K * 2;
+    const char* d = up ? p.du : p.dg;
+    m[0] = MatSource{d + m0 * 2 + (int64_t)s * 64 * dp, d + p.M * dp, 0};
+    n[0] = MatSource{p.a + n0 * 2 + (int64_t)s * 64 * xp, p.a + p.M * xp, 0};
+  }
+  template <typename Tile>
+  FLA_DEVICE bool finish(const Tile& t, const typename Tile::acc_t (&acc)[Tile::MT][Tile::NT], int) const {
+    const bool second = up && p.y;
+    return grad_store(t, acc, (T*)(up ? p.y2 : p.y), p.splits > 1 ? p.part + ((second ? p.splits : 0) + (int64_t)blockIdx.y) * p.F * p.K : nullptr, m0, n0, p.F, p.K);
+  }
+};
+template <typename T, int BM, int BN, int PER_SIMD, bool HALVES>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PER_SIMD, PER_SIMD))) void gated_dw_kernel(GradParams p, MatGrid grid) {
+  typedef DwJob<T, BM, BN, HALVES> Job;
+  __shared__ __attribute__((aligned(1024))) char lds[Job::kLds];
+  const int slices = (int)((p.M + 63) / 64), per = (slices + p.splits - 1) / p.splits, first = blockIdx.y * per;
+  Job job{p, first, first + per < slices ? first + per : slices, (uint32_t)((p.F + BM - 1) / BM), false, 0, 0};
+  mat_run(lds, grid, job);
 }
 
 // the sums of slices, added in their order: four elements a thread
@@ -364,17 +407,18 @@ __global__ __launch_bounds__(256) void grad_finish_kernel(const float* part, T* 
 }
 
 // ------------------------------------------------------------------------------------------------ host
-TilePlan plan_dx(int64_t M, int64_t F, int64_t K) { return plan_tiles(M, K, 2 * fla_cdiv(F * 2, kSliceBytes), 1, 4); }
-TilePlan plan_dw(int64_t M, int64_t F, int64_t K, int batch) { return plan_tiles(F, K, fla_cdiv(M, 64), batch, 4); }
+TilePlan plan_dx(int64_t M, int64_t F, int64_t K) { return plan_tiles(M, K, 2 * fla_cdiv(F * 2, kSliceBytes), 1); }
+TilePlan plan_dw(int64_t M, int64_t F, int64_t K, int batch) { return plan_tiles(F, K, fla_cdiv(M, 64), batch); }
 
 template <typename T, typename O>
 int launch_forward(const GatedParams& p, TileKind kind, hipStream_t st) {
-  const int64_t total = fla_cdiv(p.M, kTileM[kind]) * fla_cdiv(p.F, kTileN[kind] / 2);
-  FLA_REQUIRE(total < kMaxGrid, FLA_E_UNSUPPORTED);
-  const dim3 grid((unsigned)total, p.splits);
-  if (kind == kBig) hipLaunchKernelGGL((gated_tile_kernel<T, O, 256, 256, 1>), grid, dim3(256), 0, st, p);
-  else if (kind == kMiddle) hipLaunchKernelGGL((gated_tile_kernel<T, O, 128, 128, 2>), grid, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((gated_tile_kernel<T, O, 64, 128, 3>), grid, dim3(256), 0, st, p);
+  MatGrid g{};
+  dim3 grid;
+  const int rc = grid_of(kind, fla_cdiv(p.M, kTileM[kind]), fla_cdiv(p.F, kTileN[kind] / 2), p.splits, &g, &grid);
+  if (rc != FLA_OK) return rc;
+  if (kind == kBig) hipLaunchKernelGGL((gated_tile_kernel<T, O, 256, 256, 1, true>), grid, dim3(256), 0, st, p, g);
+  else if (kind == kMiddle) hipLaunchKernelGGL((gated_tile_kernel<T, O, 128, 128, 2, false>), grid, dim3(256), 0, st, p, g);
+  else hipLaunchKernelGGL((gated_tile_kernel<T, O, 64, 128, 3, false>), grid, dim3(256), 0, st, p, g);
   FLA_CHECK_LAUNCH();
   if (p.splits > 1) {
     hipLaunchKernelGGL((gated_finish_kernel<T, O>), dim3((unsigned)fla_cdiv(p.M * fla_cdiv(p.ldk, 4), 256)), dim3(256), 0, st, p);
@@ -384,12 +428,13 @@ int launch_forward(const GatedParams& p, TileKind kind, hipStream_t st) {
 }
 template <typename T>
 int launch_dx(const GradParams& p, TileKind kind, hipStream_t st) {
-  const int64_t total = fla_cdiv(p.M, kTileM[kind]) * fla_cdiv(p.K, kTileN[kind]);
-  FLA_REQUIRE(total < kMaxGrid, FLA_E_UNSUPPORTED);
-  const dim3 grid((unsigned)total, p.splits);
-  if (kind == kBig) hipLaunchKernelGGL((gated_dx_kernel<T, 256, 256, 1>), grid, dim3(256), 0, st, p);
-  else if (kind == kMiddle) hipLaunchKernelGGL((gated_dx_kernel<T, 128, 128, 2>), grid, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((gated_dx_kernel<T, 64, 128, 3>), grid, dim3(256), 0, st, p);
+  MatGrid g{};
+  dim3 grid;
+  const int rc = grid_of(kind, fla_cdiv(p.M, kTileM[kind]), fla_cdiv(p.K, kTileN[kind]), p.splits, &g, &grid);
+  if (rc != FLA_OK) return rc;
+  if (kind == kBig) hipLaunchKernelGGL((gated_dx_kernel<T, 256, 256, 1, true>), grid, dim3(256), 0, st, p, g);
+  else if (kind == kMiddle) hipLaunchKernelGGL((gated_dx_kernel<T, 128, 128, 2, false>), grid, dim3(256), 0, st, p, g);
+  else hipLaunchKernelGGL((gated_dx_kernel<T, 64, 128, 3, false>), grid, dim3(256), 0, st, p, g);
   FLA_CHECK_LAUNCH();
   if (p.splits > 1) {
     const int64_t n = p.M * p.K;
@@ -400,13 +445,14 @@ int launch_dx(const GradParams& p, TileKind kind, hipStream_t st) {
 }
 template <typename T>
 int launch_dw(const GradParams& p, TileKind kind, hipStream_t st) {
-  const int64_t total = fla_cdiv(p.F, kTileM[kind]) * fla_cdiv(p.K, kTileN[kind]);
-  FLA_REQUIRE(total < kMaxGrid, FLA_E_UNSUPPORTED);
   const unsigned batch = p.y && p.y2 ? 2 : 1;
-  const dim3 grid((unsigned)total, p.splits, batch);
-  if (kind == kBig) hipLaunchKernelGGL((gated_dw_kernel<T, 256, 256, 1>), grid, dim3(256), 0, st, p);
-  else if (kind == kMiddle) hipLaunchKernelGGL((gated_dw_kernel<T, 128, 128, 2>), grid, dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((gated_dw_kernel<T, 64, 128, 3>), grid, dim3(256), 0, st, p);
+  MatGrid g{};
+  dim3 grid;
+  const int rc = grid_of(kind, batch * fla_cdiv(p.F, kTileM[kind]), fla_cdiv(p.K, kTileN[kind]), p.splits, &g, &grid);
+  if (rc != FLA_OK) return rc;
+  if (kind == kBig) hipLaunchKernelGGL((gated_dw_kernel<T, 256, 256, 1, true>), grid, dim3(256), 0, st, p, g);
+  else if (kind == kMiddle) hipLaunchKernelGGL((gated_dw_kernel<T, 128, 128, 2, false>), grid, dim3(256), 0, st, p, g);
+  else hipLaunchKernelGGL((gated_dw_kernel<T, 64, 128, 3, false>), grid, dim3(256), 0, st, p, g);
   FLA_CHECK_LAUNCH();
   if (p.splits > 1) {
     const int64_t n = p.F * p.K;
@@ -428,7 +474,7 @@ int launch_panel(const GatedParams& p, hipStream_t st) {
   FLA_CHECK_LAUNCH();
   return FLA_OK;
 }
-TilePlan plan_gated(int64_t M, int64_t F, int64_t row_bytes) { return plan_tiles(M, 2 * F, fla_cdiv(row_bytes, kSliceBytes), 1, 4); }
+TilePlan plan_gated(int64_t M, int64_t F, int64_t row_bytes) { return plan_tiles(M, 2 * F, fla_cdiv(row_bytes, kSliceBytes), 1); }
 template <typename T, typename O>
 int gated_forward(GatedParams& p, hipStream_t st) {
   if (p.M <= kPanelRows) return launch_panel<T, O>(p, st);
@@ -453,7 +499,7 @@ extern "C" int fla_gated_linear_fwd(const void* x, const void* gate_weight, cons
   FLA_REQUIRE((!gate_bias && !up_bias) || bias_dtype == dtype || bias_dtype == FLA_F32, FLA_E_UNSUPPORTED);
   FLA_REQUIRE(sizes_ok(M, F, K) && K % 8 == 0, FLA_E_UNSUPPORTED);
   FLA_REQUIRE(!gate_out || (ld >= F && ld % 8 == 0 && ld < F + 8), FLA_E_UNSUPPORTED);
-  FLA_REQUIRE(aligned16({x, gate_weight, up_weight, gate_out, up_out, workspace}), FLA_E_ALIGNMENT);
+  FLA_REQUIRE(aligned16({x, gate_weight, up_weight, gate_out, up_out, workspace}) && aligned4({gate_bias, up_bias}), FLA_E_ALIGNMENT);
   if (M == 0) return FLA_OK;
   GatedParams p{};
   p.x = (const char*)x, p.wg = (const char*)gate_weight, p.wu = (const char*)up_weight, p.bg = gate_bias, p.bu = up_bias, p.h = h;
@@ -471,7 +517,7 @@ extern "C" int fla_int8_gated_linear_fwd(const void* x, const float* x_scale, co
   FLA_REQUIRE(dtype == FLA_BF16 || dtype == FLA_F16, FLA_E_UNSUPPORTED);
   FLA_REQUIRE((!gate_bias && !up_bias) || bias_dtype == dtype || bias_dtype == FLA_F32, FLA_E_UNSUPPORTED);
   FLA_REQUIRE(sizes_ok(M, F, K) && K % 16 == 0 && K <= FLA_INT8_MAX_K, FLA_E_UNSUPPORTED);
-  FLA_REQUIRE(aligned16({x, gate_weight, up_weight, workspace}), FLA_E_ALIGNMENT);
+  FLA_REQUIRE(aligned16({x, gate_weight, up_weight, workspace}) && aligned4({gate_bias, up_bias}), FLA_E_ALIGNMENT);
   if (M == 0) return FLA_OK;
   GatedParams p{};
   p.x = (const char*)x, p.wg = (const char*)gate_weight, p.wu = (const char*)up_weight, p.sx = x_scale, p.sg = gate_scale, p.su = up_scale;

@@ -128,29 +128,49 @@ struct MatTile {
   };
   static constexpr int kCopies = OpM::kCopies + OpN::kCopies;
 
+  OpM om;
+  OpN on;
+  int lane, wave, wm, wn;
+  FLA_DEVICE void start(uint32_t pitch_m, uint32_t pitch_n) {
+    lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
+    om.start(wave, lane, pitch_m);
+    on.start(wave, lane, pitch_n);
+  }
+  struct Slice {
+    MatSource m[1], n[OpN::kSources];
+    char* lds;
+  };
   // `source(s, m, n)`: where slice s lies (n: an array of OpN::kSources); asked for slices behind the last one too, of which nothing may be left, or what
-  // may be read (they are copied and not multiplied).  Slices first .. last - 1, at least one.
+  // may be read (they are copied and not multiplied).
   template <typename F>
-  static FLA_DEVICE void run(char* lds, const OpM& om, const OpN& on, int first, int last, const F& source, acc_t (&acc)[MT][NT]) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
+  static FLA_DEVICE Slice slice(char* lds, const F& source, int s, int piece) {
+    Slice c;
+    source(s, c.m, c.n);
+    c.lds = lds + piece * kPiece;
+    return c;
+  }
+  FLA_DEVICE void copy(const Slice& c, int q) const {
+    if (q < OpM::kCopies) om.copy(q, c.lds, c.m, wave);
+    else on.copy(q - OpM::kCopies, c.lds + OpM::kBytes, c.n, wave);
+  }
+  // The first slices are on their way; nobody reads LDS.
+  template <typename F>
+  FLA_DEVICE void begin(char* lds, int first, const F& source) const {
+#pragma unroll
+    for (int d = 0; d < RING; ++d) {
+      const Slice c = slice(lds, source, first + d, d);
+#pragma unroll
+      for (int q = 0; q < kCopies; ++q) copy(c, q);
+    }
+  }
+  // Slices first .. last - 1, at least one, behind begin().  LATER: with `later`, so many memory operations of this wave were issued behind it
+  // (the stores of the tile before, which need not be waited for).
+  template <int LATER, typename F>
+  FLA_DEVICE void multiply(char* lds, int first, int last, bool later, const F& source, acc_t (&acc)[MT][NT]) const {
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) acc[i][j] = acc_t{};
-    struct Slice {
-      MatSource m[1], n[OpN::kSources];
-      char* lds;
-    };
-    auto slice = [&](int s, int piece) {
-      Slice c;
-      source(s, c.m, c.n);
-      c.lds = lds + piece * kPiece;
-      return c;
-    };
-    auto copy = [&](const Slice& c, int q) {
-      if (q < OpM::kCopies) om.copy(q, c.lds, c.m, wave);
-      else on.copy(q - OpM::kCopies, c.lds + OpM::kBytes, c.n, wave);
-    };
     constexpr int kFrags = 2 * (MT + NT), kProducts = 2 * MT * NT;
     auto read = [&](Frags& f, const char* from, int half, int q) {   // (in the order in which they are multiplied)
       const int h = q / (MT + NT), g = q % (MT + NT);
@@ -175,39 +195,120 @@ struct MatTile {
         __builtin_amdgcn_sched_barrier(0);
       }
     };
-    int piece = 0;   // of slice s
-#pragma unroll
-    for (int d = 0; d < RING; ++d) {
-      const Slice c = slice(first + d, d);
-#pragma unroll
-      for (int q = 0; q < kCopies; ++q) copy(c, q);
-    }
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"((RING - 1) * kCopies) : "memory");
+    constexpr int kNewer = (RING - 1) * kCopies, kMost = 63;   // (the counter's largest value)
+    if (later) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kNewer + LATER < kMost ? kNewer + LATER : kMost) : "memory");
+    else asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kNewer) : "memory");
+    asm volatile("s_barrier" ::: "memory");
     Frags f[2];
 #pragma unroll
     for (int q = 0; q < kFrags; ++q) read(f[0], lds, 0, q);
+    int piece = 0;   // of slice s
     Slice c;
     for (int s = first; s < last; ++s) {
       half(f[0], f[1], lds + piece * kPiece, 1, c, false);
       // this wave's copies of slice s + 1 have arrived and its fragments of s are read; then everybody's
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"((RING - 2) * kCopies) : "memory");
+      if (later && s == first) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"((RING - 2) * kCopies + LATER < kMost ? (RING - 2) * kCopies + LATER : kMost) : "memory");
+      else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"((RING - 2) * kCopies) : "memory");
+      asm volatile("s_barrier" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
-      c = slice(s + RING, piece);
+      c = slice(lds, source, s + RING, piece);
       piece = piece + 1 < RING ? piece + 1 : 0;
       half(f[1], f[0], lds + piece * kPiece, 0, c, true);
     }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // no copy into LDS outlives the workgroup
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // no copy into LDS outlives the tile
   }
 };
 
-// The tile of a workgroup.  Neighbouring workgroup numbers go to different XCDs: each XCD takes a run of tiles, eight rows of tiles deep, that share
-// operands in its L2.
-FLA_DEVICE void mat_tile_of(uint32_t block, uint32_t tm_all, uint32_t tn_all, uint32_t* tm, uint32_t* tn) {
-  const uint32_t total = tm_all * tn_all, xcd = block % 8, per = total / 8, rest = total % 8;
-  const uint32_t id = xcd * per + (xcd < rest ? xcd : rest) + block / 8;
+// Neighbouring workgroup numbers go to different XCDs: each XCD takes a run of `total` tiles
+FLA_DEVICE uint32_t mat_turn(uint32_t block, uint32_t total) {
+  const uint32_t xcd = block % 8, per = total / 8, rest = total % 8;
+  return xcd * per + (xcd < rest ? xcd : rest) + block / 8;
+}
+// Tile number `id`: eight rows of tiles deep, so that those side by side share operands in an L2
+FLA_DEVICE void mat_place(uint32_t id, uint32_t tm_all, uint32_t tn_all, uint32_t* tm, uint32_t* tn) {
   const uint32_t deep = tm_all < 8 ? tm_all : 8, band = id / (deep * tn_all), in = id - band * deep * tn_all;
   const uint32_t rows_in = tm_all - band * deep < deep ? tm_all - band * deep : deep, col = in / rows_in;
   *tm = band * deep + in - col * rows_in, *tn = col;
+}
+
+// The tiles of a launch of one workgroup a CU: `whole` of them by workgroups in turn, and, where the rest would leave half of the CUs or more without
+// one, the rest as `halves` tiles of half the columns.
+struct MatGrid {
+  uint32_t tm, tn, whole, halves;
+};
+// A workgroup's tiles, one behind the other.  The first copies of a tile are on their way while the sums of the one before are brought out: what is waited for
+// between two tiles is a barrier.  JOB:
+//   Whole, Half        MatTile types;  LATER  memory operations of a wave that finish() of a whole tile issues where it returns true
+//   at(tm, n)          remembers where the tile lies: row of tiles tm, first column n (in units of half tiles)
+//   columns(side)      sends what goes by column into LDS, half `side` of it;   source(s, m, n)   as for MatTile
+//   finish(tile, acc, side)   brings a tile out
+template <typename Job>
+FLA_DEVICE void mat_run(char* lds, const MatGrid& grid, Job& job) {
+  typedef typename Job::Whole Whole;
+  typedef typename Job::Half Half;
+  Whole whole;
+  job.start(whole);
+  uint32_t u = blockIdx.x;
+  int side = 0;
+  bool later = false;
+  auto begin = [&](uint32_t id) {
+    uint32_t tm, tn;
+    mat_place(id, grid.tm, grid.tn, &tm, &tn);
+    job.at(tm, tn * 2);
+    job.columns(side);
+    whole.begin(lds, job.first, [&](int s, MatSource* m, MatSource* n) { job.source(s, m, n); });
+  };
+  auto source = [&](int s, MatSource* m, MatSource* n) { job.source(s, m, n); };
+  const bool half = blockIdx.x < grid.halves;
+  if (u < grid.whole) {
+    begin(mat_turn(u, grid.whole));
+    for (;;) {
+      typename Whole::acc_t acc[Whole::MT][Whole::NT];
+      whole.template multiply<Job::LATER>(lds, job.first, job.last, later, source, acc);
+      u += gridDim.x;
+      const bool more = u < grid.whole;
+      const Job done = job;
+      if (more) {
+        asm volatile("s_barrier" ::: "memory");   // nobody reads the slices any more
+        side ^= 1;
+        begin(mat_turn(u, grid.whole));
+      }
+      later = done.finish(whole, acc, more ? side ^ 1 : side);
+      if (!more) break;
+    }
+  }
+  if constexpr (Job::kHalves) {
+    if (half) {
+      Half tile;
+      job.start(tile);
+      const uint32_t id = mat_turn(blockIdx.x, grid.halves);
+      uint32_t tm, tn;
+      mat_place(grid.whole + id / 2, grid.tm, grid.tn, &tm, &tn);
+      __syncthreads();
+      side ^= 1;
+      job.at(tm, tn * 2 + id % 2);
+      job.columns(side);
+      tile.begin(lds, job.first, source);
+      typename Half::acc_t acc[Half::MT][Half::NT];
+      tile.template multiply<0>(lds, job.first, job.last, false, source, acc);
+      job.finish(tile, acc, side);
+    }
+  }
+}
+
+// Between the pieces of a tile that are brought out: without it the compiler brings the operands of all of them into registers first
+FLA_DEVICE void mat_piece_end() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// The sums of 32 x 32 elements as they are brought out.  Those of a tile that has all the accumulation registers stay there until then: left to itself the
+// compiler moves all 256 into ordinary registers at the loop's end and spills what lives on.
+template <typename Tile>
+FLA_DEVICE typename Tile::acc_t mat_sums(const typename Tile::acc_t (&acc)[Tile::MT][Tile::NT], int i, int j) {
+  typename Tile::acc_t v = acc[i][j];
+  if constexpr (Tile::MT * Tile::NT == 16) asm volatile("" : "+a"(v));
+  return v;
 }
 
 // Eight consecutive n a lane from two runs of four, packed in pairs (a, b: the lane's of r / 4 even and of the odd one behind it): lane l then holds
@@ -217,16 +318,20 @@ FLA_DEVICE i32x4 mat_join(u32x2 a, u32x2 b) {
   return i32x4{(int)p[0], (int)q[0], (int)p[1], (int)q[1]};
 }
 
-// eight consecutive elements of a row from n on, of which those below N exist
+// eight consecutive elements (of 16 bits) of a row from n on, of which those below N exist
 template <typename O>
 FLA_DEVICE void store_piece(O* row, int64_t n, int64_t N, bool wide, i32x4 v) {
   if (wide && n + 8 <= N) {
     *(i32x4*)(row + n) = v;
-  } else {
-    const typename Elem<O>::v8 e = __builtin_bit_cast(typename Elem<O>::v8, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (n + i < N) row[n + i] = e[i];
+  } else {   // (a loop: unrolled, the pieces of a tile are a hundred thousand bytes of code)
+    uint16_t* to = (uint16_t*)(row + n);
+    const int count = N - n < 8 ? (int)(N - n) : 8;
+#pragma unroll 1
+    for (int i = 0; i < count; ++i) {
+      to[i] = (uint16_t)v[0];
+      v[0] = __builtin_amdgcn_alignbit(v[1], v[0], 16), v[1] = __builtin_amdgcn_alignbit(v[2], v[1], 16);
+      v[2] = __builtin_amdgcn_alignbit(v[3], v[2], 16), v[3] = (int)((uint32_t)v[3] >> 16);
+    }
   }
 }
 template <typename O>

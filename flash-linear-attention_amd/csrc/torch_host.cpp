@@ -829,6 +829,13 @@ Tensor whole_rows(const Tensor& t, int64_t pieces = 1) {
   return (uintptr_t)c.data_ptr() % 16 == 0 ? c : c.clone();
 }
 
+// A bias, or none, at an address of whole words
+Tensor whole_bias(const Tensor& b) {
+  if (!b.defined()) return b;
+  const Tensor c = b.contiguous();
+  return (uintptr_t)c.data_ptr() % 4 == 0 ? c : c.clone();
+}
+
 struct GatedNode : torch::autograd::Function<GatedNode> {
   struct Rest {
     bool x, wg, wu, bg, bu;  // whether they have a gradient
@@ -846,7 +853,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
     if (M == 0) return h;
     const Tensor x = whole_rows(x_, 8), wg = whole_rows(wg_, 8), wu = whole_rows(wu_, 8);
     const bool same = (!bg_.defined() || bg_.scalar_type() == x.scalar_type()) && (!bu_.defined() || bu_.scalar_type() == x.scalar_type());
-    const Tensor bg = same ? (bg_.defined() ? bg_.contiguous() : bg_) : f32(bg_), bu = same ? (bu_.defined() ? bu_.contiguous() : bu_) : f32(bu_);
+    const Tensor bg = whole_bias(same ? bg_ : f32(bg_)), bu = whole_bias(same ? bu_ : f32(bu_));
     const int64_t K = x.size(-1);
     const int splits = fla_gated_linear_splits(M, F, K, 2);
     const Tensor sums = splits > 1 ? fresh({splits, M, 2, F}, x, at::kFloat) : Tensor();
@@ -1432,7 +1439,7 @@ PyObject* py_quant_linear(PyObject*, PyObject* const* p, Py_ssize_t n) {
   Tensor y = at::empty(shape, x.options().dtype(type));
   if (y.numel() == 0) return THPVariable_Wrap(y);
   x = whole_rows(x), w = whole_rows(w), sx = sx.contiguous(), sw = sw.contiguous();
-  if (bias.defined()) bias = (bias.scalar_type() == type ? bias : f32(bias)).contiguous();
+  if (bias.defined()) bias = whole_bias(bias.scalar_type() == type ? bias : f32(bias));
   if (res.defined()) res = res.contiguous();
   const int64_t M = x.numel() / K;
   const int splits = ints ? fla_int8_linear_splits(M, N, K) : fla_quant_linear_splits(M, N, K);
@@ -1477,8 +1484,7 @@ PyObject* py_quant_gated_linear(PyObject*, PyObject* const* p, Py_ssize_t n) {
   auto fits = [&](const Tensor& t) { return !t.defined() || t.scalar_type() == type; };
   const bool same = fits(bg) && fits(bu);
   if (!same) bg = f32(bg), bu = f32(bu);
-  if (bg.defined()) bg = bg.contiguous();
-  if (bu.defined()) bu = bu.contiguous();
+  bg = whole_bias(bg), bu = whole_bias(bu);
   const int splits = fla_gated_linear_splits(M, F, K, 1);
   const Tensor sums = splits > 1 ? fresh({splits, M, 2, F}, x, at::kInt) : Tensor();
   check(fla_int8_gated_linear_fwd(ptr(x), fptr(sx), ptr(wg), fptr(sg), ptr(wu), fptr(su), ptr(bg), ptr(bu), same ? dt(h) : FLA_F32, ptr(h), M, F, K,

@@ -882,7 +882,7 @@ int fla_quant_linear(const void* x, const float* x_scale, const void* weight, co
                      int activation, int dtype, float* workspace, fla_stream_t stream);
 
 /* Product of rows in 8-bit integers (FLA_ROWS_INT8), as above but for: sums are exact (int32), K % 16 == 0 and K <= FLA_INT8_MAX_K, beyond which a
- * sum could pass 2^31; N <= 2^22; y in fp32 too; workspace: int32 [fla_int8_linear_splits, M, N] at a 16-byte address where they are more than one. */
+ * sum could pass 2^31; N <= 2^22; y in fp32 too; bias at a 4-byte address; workspace: int32 [fla_int8_linear_splits, M, N] at a 16-byte address where they are more than one. */
 #define FLA_INT8_MAX_K 131056
 int fla_int8_linear_splits(int64_t M, int64_t N, int64_t K);
 int fla_int8_linear(const void* x, const float* x_scale, const void* weight, const float* weight_scale, const void* bias,
@@ -894,7 +894,7 @@ int fla_int8_linear(const void* x, const float* x_scale, const void* weight, con
  * blocks call torch.nn.Linear twice and the activation of fla/modules/activations.py):
  *   g = x gate_weight' + gate_bias,  u = x up_weight' + up_bias,  h[m,f] = act(g) u.
  * x [M,K], weights [F,K], h [M,F] in `dtype`, bf16 or fp16; K % 8 == 0, K, F <= 2^22; x and the weights at 16-byte addresses, any F and address of h (multiples of 8
- * and of 16 bytes take the wide stores).  Biases [F] in `dtype` or fp32 (one type for both), or NULL.  activation: enum fla_activation.
+ * and of 16 bytes take the wide stores).  Biases [F] in `dtype` or fp32 (one type for both) at 4-byte addresses, or NULL.  activation: enum fla_activation.
  * gate_out, up_out [M,ld], both or neither: g and u for the backward, ld = F rounded up to a multiple of 8, columns behind F unspecified.  A product of few tiles and
  * a long K is summed in slices of K: fla_gated_linear_splits (element_bytes: 2, or 1 for rows in 8 bits) gives their number, and where it is more
  * than one `workspace` holds [splits, M, 2, F] fp32 (int32 for rows of integers) at a 16-byte address.
