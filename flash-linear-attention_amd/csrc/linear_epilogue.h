@@ -72,4 +72,17 @@ FLA_DEVICE void with_activation(int act, const F& f) {
   else f(Const<FLA_ACT_NONE>());
 }
 
+// the same where a kernel is made for one activation (ACT; -1: for all)
+template <int ACT, typename F>
+FLA_DEVICE void with_this_activation(int act, const F& f) {
+  if constexpr (ACT >= 0) f(Const<ACT>());
+  else with_activation(act, f);
+}
+// f(Const<activation>), on the host
+template <typename F>
+int for_activation(int act, const F& f) {
+  return act == FLA_ACT_SILU ? f(Const<FLA_ACT_SILU>()) : act == FLA_ACT_GELU ? f(Const<FLA_ACT_GELU>()) : act == FLA_ACT_RELU ? f(Const<FLA_ACT_RELU>())
+                                                                                                        : f(Const<FLA_ACT_NONE>());
+}
+
 }  // namespace

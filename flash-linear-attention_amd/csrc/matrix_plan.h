@@ -17,12 +17,13 @@ constexpr int kTileM[3] = {256, 128, 64}, kTileN[3] = {256, 128, 128}, kTilePerC
 constexpr bool rest_in_halves(int64_t tiles) { return tiles % kCUs != 0 && tiles % kCUs <= kCUs / 2 && tiles > kCUs; }
 
 // Which tile and how many slices of the contraction, by an estimate of the time of each.
-TilePlan plan_tiles(int64_t M, int64_t N, int64_t slices, int batch) {
+// From `most` on in size.
+TilePlan plan_tiles(int64_t M, int64_t N, int64_t slices, int batch, TileKind most = kBig) {
   // us for a slice of 128 bytes of k of a tile, with as many tiles on the CU as it holds, and for a half tile
-  constexpr double kSlice[3] = {1.55, 0.55, 0.36}, kHalf = 0.6;
-  TilePlan best{kBig, 1};
+  constexpr double kSlice[3] = {1.6, 0.49, 0.3}, kHalf = 0.6;
+  TilePlan best{most, 1};
   double time = 0;
-  for (int t = 0; t < 3; ++t) {
+  for (int t = most; t < 3; ++t) {
     const int64_t tiles = batch * fla_cdiv(M, kTileM[t]) * fla_cdiv(N, kTileN[t]), room = kCUs * kTilePerCu[t];
     for (int splits = 1; splits <= 16; splits *= 2) {
       if (splits > 1 && (slices < 4 * splits || tiles * splits > 1024)) break;
@@ -32,7 +33,7 @@ TilePlan plan_tiles(int64_t M, int64_t N, int64_t slices, int batch) {
       if (t == kBig && splits == 1 && rest_in_halves(n)) last = kHalf;
       double est = (double)(fla_cdiv(slices, splits) + 4) * kSlice[t] * kTilePerCu[t] * ((double)(rounds - 1) + last) + 3;
       if (splits > 1) est += 4 + 8 * splits * batch * (double)M * (double)N / 4e6;     // the sums go out and in
-      if ((t == 0 && splits == 1) || est < time) best = {(TileKind)t, splits}, time = est;
+      if ((t == most && splits == 1) || est < time) best = {(TileKind)t, splits}, time = est;
     }
   }
   best.splits = (int)fla_cdiv(slices, fla_cdiv(slices, best.splits));   // none of them empty

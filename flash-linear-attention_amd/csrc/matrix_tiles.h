@@ -163,10 +163,10 @@ struct MatTile {
       for (int q = 0; q < kCopies; ++q) copy(c, q);
     }
   }
-  // Slices first .. last - 1, at least one, behind begin().  LATER: with `later`, so many memory operations of this wave were issued behind it
-  // (the stores of the tile before, which need not be waited for).
+  // Slices first .. last - 1, at least one, behind begin().  LATER, three times LATER: with `later` 1 and 2 so many memory operations of this wave were
+  // issued behind it (the stores of the tile before, which need not be waited for).
   template <int LATER, typename F>
-  FLA_DEVICE void multiply(char* lds, int first, int last, bool later, const F& source, acc_t (&acc)[MT][NT]) const {
+  FLA_DEVICE void multiply(char* lds, int first, int last, int later, const F& source, acc_t (&acc)[MT][NT]) const {
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -195,8 +195,10 @@ struct MatTile {
         __builtin_amdgcn_sched_barrier(0);
       }
     };
-    constexpr int kNewer = (RING - 1) * kCopies, kMost = 63;   // (the counter's largest value)
-    if (later) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kNewer + LATER < kMost ? kNewer + LATER : kMost) : "memory");
+    constexpr int kNewer = (RING - 1) * kCopies;
+    constexpr auto most = [](int n) { return n < 63 ? n : 63; };   // (the counter's largest value)
+    if (later == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(most(kNewer + 3 * LATER)) : "memory");
+    else if (later) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(most(kNewer + LATER)) : "memory");
     else asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kNewer) : "memory");
     asm volatile("s_barrier" ::: "memory");
     Frags f[2];
@@ -207,7 +209,8 @@ struct MatTile {
     for (int s = first; s < last; ++s) {
       half(f[0], f[1], lds + piece * kPiece, 1, c, false);
       // this wave's copies of slice s + 1 have arrived and its fragments of s are read; then everybody's
-      if (later && s == first) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"((RING - 2) * kCopies + LATER < kMost ? (RING - 2) * kCopies + LATER : kMost) : "memory");
+      if (later == 2 && s == first) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(most((RING - 2) * kCopies + 3 * LATER)) : "memory");
+      else if (later && s == first) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(most((RING - 2) * kCopies + LATER)) : "memory");
       else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"((RING - 2) * kCopies) : "memory");
       asm volatile("s_barrier" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
@@ -237,61 +240,67 @@ struct MatGrid {
   uint32_t tm, tn, whole, halves;
 };
 // A workgroup's tiles, one behind the other.  The first copies of a tile are on their way while the sums of the one before are brought out: what is waited for
-// between two tiles is a barrier.  JOB:
-//   Whole, Half        MatTile types;  LATER  memory operations of a wave that finish() of a whole tile issues where it returns true
+// between two tiles is a barrier.  Half of the workgroups take their half tile first: then not all of them write at the same time.  JOB:
+//   Whole, Half        MatTile types;  LATER  memory operations of a wave that finish() of a whole tile issues where it returns 1, a third of those where it returns 2
 //   at(tm, n)          remembers where the tile lies: row of tiles tm, first column n (in units of half tiles)
-//   columns(side)      sends what goes by column into LDS, half `side` of it;   source(s, m, n)   as for MatTile
+//   columns(side)      sends what goes by row and column into LDS, half `side` of it (a load in finish() would wait for the copies ahead of it);   source(s, m, n)   as for MatTile
 //   finish(tile, acc, side)   brings a tile out
 template <typename Job>
 FLA_DEVICE void mat_run(char* lds, const MatGrid& grid, Job& job) {
   typedef typename Job::Whole Whole;
   typedef typename Job::Half Half;
-  Whole whole;
-  job.start(whole);
-  uint32_t u = blockIdx.x;
-  int side = 0;
-  bool later = false;
-  auto begin = [&](uint32_t id) {
-    uint32_t tm, tn;
-    mat_place(id, grid.tm, grid.tn, &tm, &tn);
-    job.at(tm, tn * 2);
-    job.columns(side);
-    whole.begin(lds, job.first, [&](int s, MatSource* m, MatSource* n) { job.source(s, m, n); });
-  };
   auto source = [&](int s, MatSource* m, MatSource* n) { job.source(s, m, n); };
-  const bool half = blockIdx.x < grid.halves;
-  if (u < grid.whole) {
-    begin(mat_turn(u, grid.whole));
-    for (;;) {
-      typename Whole::acc_t acc[Whole::MT][Whole::NT];
-      whole.template multiply<Job::LATER>(lds, job.first, job.last, later, source, acc);
-      u += gridDim.x;
-      const bool more = u < grid.whole;
-      const Job done = job;
-      if (more) {
-        asm volatile("s_barrier" ::: "memory");   // nobody reads the slices any more
-        side ^= 1;
-        begin(mat_turn(u, grid.whole));
-      }
-      later = done.finish(whole, acc, more ? side ^ 1 : side);
-      if (!more) break;
-    }
-  }
-  if constexpr (Job::kHalves) {
-    if (half) {
+  int side = 0;
+  const bool early = blockIdx.x / 8 % 2;      // (every second one of an XCD's)
+#pragma unroll 1
+  for (int turn = 0; turn < 2; ++turn) {
+    if (Job::kHalves && early == (turn == 0)) {
+      if (blockIdx.x >= grid.halves) continue;
       Half tile;
       job.start(tile);
       const uint32_t id = mat_turn(blockIdx.x, grid.halves);
       uint32_t tm, tn;
       mat_place(grid.whole + id / 2, grid.tm, grid.tn, &tm, &tn);
       __syncthreads();
-      side ^= 1;
       job.at(tm, tn * 2 + id % 2);
       job.columns(side);
       tile.begin(lds, job.first, source);
       typename Half::acc_t acc[Half::MT][Half::NT];
-      tile.template multiply<0>(lds, job.first, job.last, false, source, acc);
+      tile.template multiply<0>(lds, job.first, job.last, 0, source, acc);
       job.finish(tile, acc, side);
+      side ^= 1;
+    } else if (!Job::kHalves && turn) {
+      break;
+    } else {
+      Whole whole;
+      job.start(whole);
+      uint32_t u = blockIdx.x;
+      auto begin = [&](uint32_t id) {
+        uint32_t tm, tn;
+        mat_place(id, grid.tm, grid.tn, &tm, &tn);
+        job.at(tm, tn * 2);
+        job.columns(side);
+        whole.begin(lds, job.first, source);
+      };
+      if (u >= grid.whole) continue;
+      __syncthreads();
+      begin(mat_turn(u, grid.whole));
+      int later = 0;
+      for (;;) {
+        typename Whole::acc_t acc[Whole::MT][Whole::NT];
+        whole.template multiply<Job::LATER>(lds, job.first, job.last, later, source, acc);
+        u += gridDim.x;
+        const bool more = u < grid.whole;
+        const Job done = job;
+        const int now = side;
+        side ^= 1;
+        if (more) {
+          asm volatile("s_barrier" ::: "memory");   // nobody reads the slices any more
+          begin(mat_turn(u, grid.whole));
+        }
+        later = done.finish(whole, acc, now);
+        if (!more) break;
+      }
     }
   }
 }
@@ -318,14 +327,15 @@ FLA_DEVICE i32x4 mat_join(u32x2 a, u32x2 b) {
   return i32x4{(int)p[0], (int)q[0], (int)p[1], (int)q[1]};
 }
 
-// eight consecutive elements (of 16 bits) of a row from n on, of which those below N exist
+// Eight consecutive elements (of 16 bits) of a row from n on, of which those below N exist, at any element address
 template <typename O>
-FLA_DEVICE void store_piece(O* row, int64_t n, int64_t N, bool wide, i32x4 v) {
-  if (wide && n + 8 <= N) {
-    *(i32x4*)(row + n) = v;
+FLA_DEVICE void store_piece(O* row, int64_t n, int64_t N, i32x4 v) {
+  typedef i32x4 any __attribute__((aligned(2)));
+  if (n + 8 <= N) {
+    *(any*)(row + n) = v;
   } else {   // (a loop: unrolled, the pieces of a tile are a hundred thousand bytes of code)
     uint16_t* to = (uint16_t*)(row + n);
-    const int count = N - n < 8 ? (int)(N - n) : 8;
+    const int count = (int)(N - n);
 #pragma unroll 1
     for (int i = 0; i < count; ++i) {
       to[i] = (uint16_t)v[0];

@@ -1442,7 +1442,7 @@ PyObject* py_quant_linear(PyObject*, PyObject* const* p, Py_ssize_t n) {
   if (bias.defined()) bias = whole_bias(bias.scalar_type() == type ? bias : f32(bias));
   if (res.defined()) res = res.contiguous();
   const int64_t M = x.numel() / K;
-  const int splits = ints ? fla_int8_linear_splits(M, N, K) : fla_quant_linear_splits(M, N, K);
+  const int splits = ints ? fla_int8_linear_splits(M, N, K, dt(y)) : fla_quant_linear_splits(M, N, K);
   const Tensor sums = splits > 1 ? fresh({splits, M, N}, x, ints ? at::kInt : at::kFloat) : Tensor();
   const int bt = bias.defined() ? dt(bias) : FLA_F32, rt = res.defined() ? dt(res) : FLA_F32;
   if (ints)

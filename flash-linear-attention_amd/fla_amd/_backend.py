@@ -16,7 +16,7 @@ _lib = None
 
 FLA_F32, FLA_BF16, FLA_F16 = 0, 1, 2
 FLA_H_ROW_MAJOR, FLA_H_FRAGMENT, FLA_H_FRAGMENT_T = 0, 1, 2
-ABI_VERSION = 26
+ABI_VERSION = 27
 
 _DTYPES = {torch.float32: FLA_F32, torch.bfloat16: FLA_BF16, torch.float16: FLA_F16}
 
@@ -119,7 +119,7 @@ SIGNATURES = {
     "fla_layer_norm_bwd": (c_int, [P, P, I, P, I, P, P, P, P, P, P, P, I64, I64, I, P]),
     "fla_quant_linear_splits": (c_int, [I64, I64, I64]),
     "fla_quant_linear": (c_int, [P, P, P, P, P, I, P, I, P, I64, I64, I64, I, I, P, P]),
-    "fla_int8_linear_splits": (c_int, [I64, I64, I64]),
+    "fla_int8_linear_splits": (c_int, [I64, I64, I64, I]),
     "fla_int8_linear": (c_int, [P, P, P, P, P, I, P, I, P, I64, I64, I64, I, I, P, P]),
     "fla_int8_gated_linear_fwd": (c_int, [P] * 8 + [I, P, I64, I64, I64, I, I, P, P]),
     "fla_gated_linear_splits": (c_int, [I64, I64, I64, I]),

@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define FLA_ABI_VERSION 26
+#define FLA_ABI_VERSION 27
 
 enum fla_dtype { FLA_F32 = 0, FLA_BF16 = 1, FLA_F16 = 2 };
 
@@ -884,7 +884,7 @@ int fla_quant_linear(const void* x, const float* x_scale, const void* weight, co
 /* Product of rows in 8-bit integers (FLA_ROWS_INT8), as above but for: sums are exact (int32), K % 16 == 0 and K <= FLA_INT8_MAX_K, beyond which a
  * sum could pass 2^31; N <= 2^22; y in fp32 too; bias at a 4-byte address; workspace: int32 [fla_int8_linear_splits, M, N] at a 16-byte address where they are more than one. */
 #define FLA_INT8_MAX_K 131056
-int fla_int8_linear_splits(int64_t M, int64_t N, int64_t K);
+int fla_int8_linear_splits(int64_t M, int64_t N, int64_t K, int dtype);
 int fla_int8_linear(const void* x, const float* x_scale, const void* weight, const float* weight_scale, const void* bias,
                     int bias_dtype, const void* residual, int residual_dtype, void* y, int64_t M, int64_t N, int64_t K,
                     int activation, int dtype, void* workspace, fla_stream_t stream);

@@ -67,7 +67,7 @@ def test_library_entries_refuse():
     lin = lambda x=at, M=2, N=8, K=32, act=0, dtype=1, bt=1, ws=None: lib.fla_int8_linear(x, at, at, at, at, bt, None, 0, at, M, N, K, act, dtype, ws, None)
     assert lin(x=None) == -1 and lin(N=0) == -1 and lin(act=7) == -1 and lin(dtype=3) == -2 and lin(bt=2) == -2
     assert lin(K=24) == -2 and lin(K=131072) == -2 and lin(N=(1 << 22) + 1) == -2 and lin(x=at + 8) == -3 and lin(M=0) == 0
-    split = lib.fla_int8_linear_splits(100, 128, 8192)
+    split = lib.fla_int8_linear_splits(100, 128, 8192, 1)
     assert split > 1 and lin(M=100, N=128, K=8192) == -1 and lin(M=100, N=128, K=8192, ws=at + 4) == -3
     gated = lambda x=at, K=32, act=1, dtype=1: lib.fla_int8_gated_linear_fwd(x, at, at, at, at, at, None, None, 0, at, 2, 8, K, act, dtype, None, None)
     assert gated(x=None) == -1 and gated(K=24) == -2 and gated(K=131072) == -2 and gated(act=9) == -1 and gated(dtype=0) == -2 and gated(x=at + 4) == -3
