@@ -163,26 +163,48 @@ template <typename T, typename O>
 __global__ __launch_bounds__(256) void gated_finish_kernel(GatedParams p) {
   constexpr bool INT = sizeof(T) == 1;
   typedef typename std::conditional<INT, int, float>::type S;
+  typedef S S4 __attribute__((ext_vector_type(4), aligned(4)));
   const int64_t per = (p.ldk + 3) / 4, id = (int64_t)blockIdx.x * 256 + threadIdx.x, m = id / per, n0 = id % per * 4;
   if (m >= p.M) return;
+  const bool whole = n0 + 4 <= p.F;
+  S4 g = {0, 0, 0, 0}, u = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const S* from = (const S*)p.part + (s * p.M + m) * 2 * p.F + n0;
+    if (whole) {
+      g += *(const S4*)from, u += *(const S4*)(from + p.F);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n0 + i < p.F) g[i] += from[i], u[i] += from[p.F + i];
+    }
+  }
   const float sx = INT ? p.sx[m] : 1.f;
+  float gf[4], uf[4], v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t n = n0 + i;
+    const float bg = gated_bias<O>(p.bg, p.bias_f32, n, p.F), bu = gated_bias<O>(p.bu, p.bias_f32, n, p.F);
+    gf[i] = INT ? fmaf((float)g[i], n < p.F ? sx * p.sg[n] : 0.f, bg) : (float)g[i] + bg;
+    uf[i] = INT ? fmaf((float)u[i], n < p.F ? sx * p.su[n] : 0.f, bu) : (float)u[i] + bu;
+  }
   with_activation(p.act, [&](auto act) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t n = n0 + i;
-      S g = 0, u = 0;
-      if (n < p.F)
-        for (int s = 0; s < p.splits; ++s) {
-          const S* from = (const S*)p.part + (s * p.M + m) * 2 * p.F + n;
-          g += from[0], u += from[p.F];
-        }
-      const float bg = gated_bias<O>(p.bg, p.bias_f32, n, p.F), bu = gated_bias<O>(p.bu, p.bias_f32, n, p.F);
-      const float gf = INT ? fmaf((float)g, n < p.F ? sx * p.sg[n] : 0.f, bg) : (float)g + bg;
-      const float uf = INT ? fmaf((float)u, n < p.F ? sx * p.su[n] : 0.f, bu) : (float)u + bu;
-      if (n < p.F) ((O*)p.h)[m * p.F + n] = (O)(activate_gate<decltype(act)::value>(gf) * uf);
-      if (!INT && p.g && n < p.ldk) ((O*)p.g)[m * p.ldk + n] = (O)gf, ((O*)p.u)[m * p.ldk + n] = (O)uf;
-    }
+    for (int i = 0; i < 4; ++i) v[i] = activate_gate<decltype(act)::value>(gf[i]) * uf[i];
   });
+  O* h = (O*)p.h + m * p.F + n0;
+  if (whole) {
+    typedef u32x2 any __attribute__((aligned(2)));
+    *(any*)h = pack4<O>(v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n0 + i < p.F) h[i] = (O)v[i];
+  }
+  if (!INT && p.g && n0 < p.ldk) {     // (ldk is a multiple of 8)
+    *(u32x2*)((O*)p.g + m * p.ldk + n0) = pack4<O>(gf);
+    *(u32x2*)((O*)p.u + m * p.ldk + n0) = pack4<O>(uf);
+  }
 }
 
 // At most MT x 16 rows of x: sixteen columns of h to a workgroup
@@ -257,7 +279,7 @@ int launch_panel(const GatedParams& p, hipStream_t st) {
   FLA_CHECK_LAUNCH();
   return FLA_OK;
 }
-TilePlan plan_gated(int64_t M, int64_t F, int64_t row_bytes) { return plan_tiles(M, 2 * F, fla_cdiv(row_bytes, kSliceBytes), 1); }
+TilePlan plan_gated(int64_t M, int64_t F, int64_t row_bytes) { return plan_tiles(M, 2 * F, fla_cdiv(row_bytes, kSliceBytes), 1, true); }
 template <typename T, typename O>
 int gated_forward(GatedParams& p, hipStream_t st) {
   if (p.M <= kPanelRows) return launch_panel<T, O>(p, st);

@@ -16,23 +16,30 @@ constexpr int kTileM[3] = {256, 128, 64}, kTileN[3] = {256, 128, 128}, kTilePerC
 // What is left behind whole rounds of big tiles goes in tiles of half the columns where a CU then has one at most
 constexpr bool rest_in_halves(int64_t tiles) { return tiles % kCUs != 0 && tiles % kCUs <= kCUs / 2 && tiles > kCUs; }
 
-// Which tile and how many slices of the contraction, by an estimate of the time of each.
-// From `most` on in size.
-TilePlan plan_tiles(int64_t M, int64_t N, int64_t slices, int batch, TileKind most = kBig) {
-  // us for a slice of 128 bytes of k of a tile, with as many tiles on the CU as it holds, and for a half tile
-  constexpr double kSlice[3] = {1.6, 0.49, 0.3}, kHalf = 0.6;
+// Which tile and how many slices of the contraction, by an estimate of the time of each; from `most` on in size.  What it rests on (us for a slice of 128 bytes of k of
+// every tile on a CU, measured in products of 70 to 8192 rows, bf16):
+//                        256 x 256, one a CU       128 x 128, one and two   64 x 128, one, two and three
+//   both contiguous      1.05 (few CUs) to 1.6     1.25  1.7                0.9   1.5   1.95
+//   one or both strided  1.05 to 1.6               0.72  0.97               0.58  0.65  0.9
+// Rows of 128 bytes out of two weights come slower than the strided operand's 256 and 512 bytes on end: where both are contiguous the tile with the fewest bytes wins early.
+// Ends: 12, 8 and 7 us for the first tile of a CU, half of that for each further one; sums of slices go out and in at 5 TB/s behind 5 us.
+// Measured with all three tiles and 1 to 8 slices (us; M x K to F): forward 70 x 2048 to 5632: 28 - 47, taken 30; 200 x 4096 to 11008: 70 - 168, taken 70; 500 x 4096 to 4096: 65 - 140, taken 65;
+// 1003 x 1000 to 2731: 35 - 95, taken 35.  dx of the last: 29 - 120, taken 29; of 2048 x 2048 to 5632: 100 - 208, taken 100; its weights' gradients 92 - 146, taken 92.
+TilePlan plan_tiles(int64_t M, int64_t N, int64_t slices, int batch, bool contiguous, TileKind most = kBig) {
+  constexpr double kEnds[3] = {12, 8, 7}, kSlice[2][3][3] = {{{0, 0, 0}, {0.72, 0.97, 0}, {0.58, 0.65, 0.9}}, {{0, 0, 0}, {1.25, 1.7, 0}, {0.9, 1.5, 1.95}}};
   TilePlan best{most, 1};
   double time = 0;
   for (int t = most; t < 3; ++t) {
     const int64_t tiles = batch * fla_cdiv(M, kTileM[t]) * fla_cdiv(N, kTileN[t]), room = kCUs * kTilePerCu[t];
     for (int splits = 1; splits <= 16; splits *= 2) {
       if (splits > 1 && (slices < 4 * splits || tiles * splits > 1024)) break;
-      const int64_t n = tiles * splits, rounds = fla_cdiv(n, room), in_last = n - (rounds - 1) * room;
-      // a CU with some of its tiles missing runs the others faster, but not as much
-      double last = 0.5 + 0.5 * (double)fla_cdiv(in_last, kCUs) / kTilePerCu[t];
-      if (t == kBig && splits == 1 && rest_in_halves(n)) last = kHalf;
-      double est = (double)(fla_cdiv(slices, splits) + 4) * kSlice[t] * kTilePerCu[t] * ((double)(rounds - 1) + last) + 3;
-      if (splits > 1) est += 4 + 8 * splits * batch * (double)M * (double)N / 4e6;     // the sums go out and in
+      const int64_t n = tiles * splits, rounds = n / room, rest = n % room;
+      auto slice = [&](int64_t on) { return t == kBig ? 1.05 + 0.55 * (double)on / kCUs : kSlice[contiguous][t][fla_cdiv(on, kCUs) - 1]; };
+      double last = rest ? slice(rest) : 0;
+      if (t == kBig && splits == 1 && rest_in_halves(n)) last = 0.6 * slice(kCUs);
+      const int64_t turns = rounds + (rest > 0);
+      double est = (double)fla_cdiv(slices, splits) * ((double)rounds * slice(room) + last) + kEnds[t] * (0.5 + 0.5 * (double)turns);
+      if (splits > 1) est += 5 + 8 * splits * batch * (double)M * (double)N / 5e6;
       if ((t == most && splits == 1) || est < time) best = {(TileKind)t, splits}, time = est;
     }
   }
