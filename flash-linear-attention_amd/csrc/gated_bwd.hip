@@ -12,8 +12,8 @@ namespace {
 struct GatedBwdParams {
   const void *dh, *g, *u;     // [M,F], [M,ld], [M,ld]
   void *dg, *du;              // [M,ld]: columns behind F are zeros
-  float *pg, *pu;             // partial sums [gridDim.y, F] or NULL
-  int64_t M, F, ld, rows;     // rows: of a workgroup
+  float *pg, *pu;             // partial sums [gridDim.y, F], rows pld apart, or NULL
+  int64_t M, F, ld, pld, rows;     // rows: of a workgroup
   int act;
 };
 
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(256) void gated_bwd_kernel(GatedBwdParams p) {
     const int c = k & 511, which = k >> 9;
     const int64_t n = (int64_t)blockIdx.x * 512 + c;
     float* part = which ? p.pu : p.pg;
-    if (part && n < p.F) part[blockIdx.y * p.F + n] = ((sum[which][0][c] + sum[which][1][c]) + sum[which][2][c]) + sum[which][3][c];
+    if (part && n < p.F) part[blockIdx.y * p.pld + n] = ((sum[which][0][c] + sum[which][1][c]) + sum[which][2][c]) + sum[which][3][c];
   }
 }
 
@@ -235,16 +235,17 @@ int launch_dw(const GradParams& p, TileKind kind, hipStream_t st) {
 extern "C" int fla_gated_linear_bwd_rows(int64_t M) { return M <= 0 ? 1 : (int)(fla_cdiv(M, 256) < 32 ? 32 : fla_cdiv(M, 256)); }
 
 extern "C" int fla_gated_linear_bwd_gate(const void* dh, const void* gate, const void* up, void* dgate, void* dup, float* dgate_bias_partial,
-                                         float* dup_bias_partial, int64_t ld, int64_t M, int64_t F, int activation, int dtype,
+                                         float* dup_bias_partial, int64_t partial_ld, int64_t ld, int64_t M, int64_t F, int activation, int dtype,
                                          fla_stream_t stream) {
   FLA_REQUIRE(dh && gate && up && dgate && dup && M >= 0 && F > 0, FLA_E_INVALID);
   FLA_REQUIRE(activation >= FLA_ACT_NONE && activation <= FLA_ACT_RELU, FLA_E_INVALID);
   FLA_REQUIRE(dtype == FLA_BF16 || dtype == FLA_F16, FLA_E_UNSUPPORTED);
   FLA_REQUIRE(sizes_ok(M, F, 1) && ld >= F && ld % 8 == 0 && ld < F + 8, FLA_E_UNSUPPORTED);
+  FLA_REQUIRE((!dgate_bias_partial && !dup_bias_partial) || partial_ld >= F, FLA_E_INVALID);
   FLA_REQUIRE(aligned16({gate, up, dgate, dup}), FLA_E_ALIGNMENT);
   if (M == 0) return FLA_OK;
   GatedBwdParams p{};
-  p.dh = dh, p.g = gate, p.u = up, p.dg = dgate, p.du = dup, p.pg = dgate_bias_partial, p.pu = dup_bias_partial, p.M = M, p.F = F, p.ld = ld;
+  p.dh = dh, p.g = gate, p.u = up, p.dg = dgate, p.du = dup, p.pg = dgate_bias_partial, p.pu = dup_bias_partial, p.M = M, p.F = F, p.ld = ld, p.pld = partial_ld;
   p.act = activation, p.rows = fla_gated_linear_bwd_rows(M);
   const dim3 grid((unsigned)fla_cdiv(ld, 512), (unsigned)fla_cdiv(M, p.rows));
   hipStream_t st = (hipStream_t)stream;

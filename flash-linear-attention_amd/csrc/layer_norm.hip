@@ -12,7 +12,8 @@ extern "C" int fla_layer_norm_workgroups(int64_t M, int64_t N) { return norm_wor
 
 extern "C" int fla_layer_norm_bwd(const void* dy, const void* kept, int kept_dtype, const void* weight, int weight_dtype, const float* mean,
                                   const float* rstd, const void* dresidual, void* dx, void* dresidual_in, float* dw_partial,
-                                  float* db_partial, int64_t M, int64_t N, int dtype, fla_stream_t stream) {
-  return norm_backward<true>(dy, kept, kept_dtype, weight, weight_dtype, mean, rstd, dresidual, dx, dresidual_in, dw_partial, db_partial, M,
-                             N, dtype, stream);
+                                  float* db_partial, int64_t partial_ld, int64_t M, int64_t N, int dtype,
+                                  fla_stream_t stream) {
+  return norm_backward<true>(dy, kept, kept_dtype, weight, weight_dtype, mean, rstd, dresidual, dx, dresidual_in, dw_partial, db_partial,
+                             partial_ld, M, N, dtype, stream);
 }

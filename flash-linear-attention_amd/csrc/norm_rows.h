@@ -32,9 +32,9 @@ struct NormParams {
   const void* dres;     // [M,N] in the kept type, or NULL
   void* dx;
   void* dres_in;        // a copy of dx in the kept type, or NULL
-  float* dw_part;       // [gridDim.x, N] or NULL
+  float* dw_part;       // [gridDim.x, N], rows part_ld apart, or NULL
   float* db_part;
-  int64_t M;
+  int64_t M, part_ld;
   int N;
   float eps;
   int res_f32, res_out_f32, w_f32, plain;   // plain: rows are not normalised (8-bit rows of x itself)
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(bwd_block(TPR)) void norm_bwd_kernel(NormParams p) 
   for (int which = 0; which < (BIAS ? 2 : 1); ++which) {
     float* part = which ? p.db_part : p.dw_part;
     if (!part) continue;   // uniform
-    part += (int64_t)blockIdx.x * N;
+    part += (int64_t)blockIdx.x * p.part_ld;
 #pragma unroll
     for (int q = 0; q < NP; ++q) {
       const float* mine = which ? db[q] : dw[q];
@@ -483,18 +483,19 @@ int norm_workgroups(int64_t M, int64_t N) {
 
 template <bool MEAN>
 int norm_backward(const void* dy, const void* kept, int kept_dtype, const void* weight, int weight_dtype, const float* mean, const float* rstd,
-                  const void* dresidual, void* dx, void* dresidual_in, float* dw_partial, float* db_partial, int64_t M, int64_t N, int dtype,
-                  fla_stream_t stream) {
+                  const void* dresidual, void* dx, void* dresidual_in, float* dw_partial, float* db_partial, int64_t partial_ld, int64_t M, int64_t N,
+                  int dtype, fla_stream_t stream) {
   FLA_REQUIRE(dy && kept && rstd && dx && (!MEAN || mean) && M >= 0 && N > 0, FLA_E_INVALID);
   FLA_REQUIRE(N <= kMaxN && M <= 0x7fffffffLL && type_ok(kept_dtype, dtype), FLA_E_UNSUPPORTED);
   FLA_REQUIRE(!weight || type_ok(weight_dtype, dtype), FLA_E_UNSUPPORTED);
-  FLA_REQUIRE(((uintptr_t)dw_partial | (uintptr_t)db_partial) % 16 == 0, FLA_E_ALIGNMENT);
+  FLA_REQUIRE(partial_ld >= N, FLA_E_INVALID);
+  const bool w = wide(N, {dy, kept, weight, dresidual, dx, dresidual_in});
+  FLA_REQUIRE(((uintptr_t)dw_partial | (uintptr_t)db_partial | (w ? (uintptr_t)(partial_ld * 4) : 0)) % (w ? 16 : 4) == 0, FLA_E_ALIGNMENT);
   if (M == 0) return FLA_OK;
   NormParams p{};
   p.x = kept, p.w = weight, p.rstd = (float*)rstd, p.mean = (float*)mean, p.dy = dy, p.dres = dresidual, p.dx = dx, p.dres_in = dresidual_in;
-  p.dw_part = dw_partial, p.db_part = db_partial, p.M = M, p.N = (int)N;
+  p.dw_part = dw_partial, p.db_part = db_partial, p.part_ld = partial_ld, p.M = M, p.N = (int)N;
   p.w_f32 = weight_dtype == FLA_F32;
-  const bool w = wide(N, {dy, kept, weight, dresidual, dx, dresidual_in});
   const int grid = norm_workgroups(M, N);
   hipStream_t st = (hipStream_t)stream;
 #define D_(E, T)                                                                                                                            \

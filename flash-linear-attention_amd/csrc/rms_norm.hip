@@ -20,6 +20,7 @@ extern "C" int fla_rms_norm_workgroups(int64_t M, int64_t N) { return norm_workg
 extern "C" int fla_rms_norm_bwd(const void* dy, const void* kept, int kept_dtype, const void* weight, int weight_dtype, const float* rstd,
                                 const void* dresidual, void* dx, void* dresidual_in, float* dw_partial, float* db_partial, int64_t M,
                                 int64_t N, int dtype, fla_stream_t stream) {
-  return norm_backward<false>(dy, kept, kept_dtype, weight, weight_dtype, nullptr, rstd, dresidual, dx, dresidual_in, dw_partial, db_partial,
+  FLA_REQUIRE(((uintptr_t)dw_partial | (uintptr_t)db_partial) % 16 == 0, FLA_E_ALIGNMENT);
+  return norm_backward<false>(dy, kept, kept_dtype, weight, weight_dtype, nullptr, rstd, dresidual, dx, dresidual_in, dw_partial, db_partial, N,
                               M, N, dtype, stream);
 }

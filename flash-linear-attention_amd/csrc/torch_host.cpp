@@ -537,6 +537,32 @@ Tensor sum_partials(const Tensor& part, at::IntArrayRef shape, at::ScalarType ty
   return as(out, type);
 }
 
+// Two weights' partial sums side by side [parts, 2, n], added in one launch where both are of one type.  Either may be unwanted.
+struct PartialPair {
+  Tensor both, a, b;      // (both: where they are of one type)
+  int64_t n, ld;
+  at::ScalarType at_, bt_;
+  PartialPair(bool want_a, bool want_b, at::ScalarType ta, at::ScalarType tb, int64_t parts, int64_t n_, const Tensor& like) : n(n_), ld(n_), at_(ta), bt_(tb) {
+    if (want_a && want_b && ta == tb) {
+      both = fresh({parts, 2, n}, like, at::kFloat), ld = 2 * n;
+    } else {
+      if (want_a) a = fresh({parts, n}, like, at::kFloat);
+      if (want_b) b = fresh({parts, n}, like, at::kFloat);
+    }
+  }
+  float* first() const { return both.defined() ? fptr(both) : fptr(a); }
+  float* second() const { return both.defined() ? fptr(both) + n : fptr(b); }
+  void sums(Tensor* x, Tensor* y) const {
+    if (both.defined()) {
+      const Tensor s = sum_partials(both, {2, n}, at_);
+      *x = s.select(0, 0), *y = s.select(0, 1);
+    } else {
+      if (a.defined()) *x = sum_partials(a, {n}, at_);
+      if (b.defined()) *y = sum_partials(b, {n}, bt_);
+    }
+  }
+};
+
 struct L2NormNode : torch::autograd::Function<L2NormNode> {
   static Tensor run(const Tensor& x, double eps) {
     Tensor y = fresh_like(x);
@@ -806,16 +832,20 @@ struct NormNode : torch::autograd::Function<NormNode> {
       return {dx, r.w ? at::zeros_like(w) : Tensor(), r.b ? at::zeros_like(b) : Tensor(), r.res ? (dres_in.defined() ? dres_in : dx) : Tensor(),
               Tensor()};
     const int64_t parts = mean.defined() ? fla_layer_norm_workgroups(M, N) : fla_rms_norm_workgroups(M, N);
-    Tensor dw = r.w ? fresh({parts, N}, kept, at::kFloat) : Tensor(), db = r.b ? fresh({parts, N}, kept, at::kFloat) : Tensor();
     const int wt = w.defined() ? dt(w) : dt(kept);
-    if (mean.defined())
-      check(fla_layer_norm_bwd(ptr(dy), ptr(kept), dt(kept), ptr(w), wt, fptr(mean), fptr(rstd), ptr(dres), ptr(dx), ptr(dres_in), fptr(dw),
-                               fptr(db), M, N, dt(dx), stream_of(kept)),
+    if (mean.defined()) {
+      const PartialPair part(r.w, r.b, w.defined() ? w.scalar_type() : at::kFloat, b.defined() ? b.scalar_type() : at::kFloat, parts, N, kept);
+      check(fla_layer_norm_bwd(ptr(dy), ptr(kept), dt(kept), ptr(w), wt, fptr(mean), fptr(rstd), ptr(dres), ptr(dx), ptr(dres_in), part.first(),
+                               part.second(), part.ld, M, N, dt(dx), stream_of(kept)),
             "fla_layer_norm_bwd");
-    else
-      check(fla_rms_norm_bwd(ptr(dy), ptr(kept), dt(kept), ptr(w), wt, fptr(rstd), ptr(dres), ptr(dx), ptr(dres_in), fptr(dw), fptr(db), M, N,
-                             dt(dx), stream_of(kept)),
-            "fla_rms_norm_bwd");
+      Tensor gw, gb;
+      part.sums(&gw, &gb);
+      return {dx, gw, gb, r.res ? (dres_in.defined() ? dres_in : dx) : Tensor(), Tensor()};
+    }
+    Tensor dw = r.w ? fresh({parts, N}, kept, at::kFloat) : Tensor(), db = r.b ? fresh({parts, N}, kept, at::kFloat) : Tensor();
+    check(fla_rms_norm_bwd(ptr(dy), ptr(kept), dt(kept), ptr(w), wt, fptr(rstd), ptr(dres), ptr(dx), ptr(dres_in), fptr(dw), fptr(db), M, N,
+                           dt(dx), stream_of(kept)),
+          "fla_rms_norm_bwd");
     return {dx, r.w ? sum_partials(dw, w.sizes(), w.scalar_type()) : Tensor(), r.b ? sum_partials(db, b.sizes(), b.scalar_type()) : Tensor(),
             r.res ? (dres_in.defined() ? dres_in : dx) : Tensor(), Tensor()};
   }
@@ -894,13 +924,12 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
     const Tensor dh = as(grads[0], type).contiguous();
     const Tensor d = fresh_like(kept);
     const int64_t rows = fla_gated_linear_bwd_rows(M), parts = (M + rows - 1) / rows, half = M * ld * 2;
-    const Tensor pg = r.bg ? fresh({parts, F}, kept, at::kFloat) : Tensor(), pu = r.bu ? fresh({parts, F}, kept, at::kFloat) : Tensor();
+    const PartialPair part(r.bg, r.bu, r.bg_type, r.bu_type, parts, F, kept);
     const fla_stream_t stream = stream_of(kept);
     char *g = (char*)kept.data_ptr(), *dg = (char*)d.data_ptr();
-    check(fla_gated_linear_bwd_gate(ptr(dh), g, g + half, dg, dg + half, fptr(pg), fptr(pu), ld, M, F, (int)r.act, dt(kept), stream),
+    check(fla_gated_linear_bwd_gate(ptr(dh), g, g + half, dg, dg + half, part.first(), part.second(), part.ld, ld, M, F, (int)r.act, dt(kept), stream),
           "fla_gated_linear_bwd_gate");
-    if (r.bg) dbg = sum_partials(pg, {F}, r.bg_type);
-    if (r.bu) dbu = sum_partials(pu, {F}, r.bu_type);
+    part.sums(&dbg, &dbu);
     if (r.x) {
       const Tensor wg = whole_rows(saved[1], 8), wu = whole_rows(saved[2], 8);
       dx = fresh({M, K}, kept, type);

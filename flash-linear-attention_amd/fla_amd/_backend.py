@@ -16,7 +16,7 @@ _lib = None
 
 FLA_F32, FLA_BF16, FLA_F16 = 0, 1, 2
 FLA_H_ROW_MAJOR, FLA_H_FRAGMENT, FLA_H_FRAGMENT_T = 0, 1, 2
-ABI_VERSION = 27
+ABI_VERSION = 28
 
 _DTYPES = {torch.float32: FLA_F32, torch.bfloat16: FLA_BF16, torch.float16: FLA_F16}
 
@@ -116,7 +116,7 @@ SIGNATURES = {
     "fla_rms_norm_rows8_fwd": (c_int, [P, P, I, P, P, I, P, P, P, I, I64, I64, F, I, I, I, P]),
     "fla_layer_norm_workgroups": (c_int, [I64, I64]),
     "fla_layer_norm_fwd": (c_int, [P, P, I, P, P, I, P, P, P, I, P, P, I64, I64, F, I, I, P]),
-    "fla_layer_norm_bwd": (c_int, [P, P, I, P, I, P, P, P, P, P, P, P, I64, I64, I, P]),
+    "fla_layer_norm_bwd": (c_int, [P, P, I, P, I, P, P, P, P, P, P, P, I64, I64, I64, I, P]),
     "fla_quant_linear_splits": (c_int, [I64, I64, I64]),
     "fla_quant_linear": (c_int, [P, P, P, P, P, I, P, I, P, I64, I64, I64, I, I, P, P]),
     "fla_int8_linear_splits": (c_int, [I64, I64, I64, I]),
@@ -125,7 +125,7 @@ SIGNATURES = {
     "fla_gated_linear_splits": (c_int, [I64, I64, I64, I]),
     "fla_gated_linear_fwd": (c_int, [P] * 5 + [I, P, P, P, I64, I64, I64, I64, I, I, P, P]),
     "fla_gated_linear_bwd_rows": (c_int, [I64]),
-    "fla_gated_linear_bwd_gate": (c_int, [P] * 7 + [I64, I64, I64, I, I, P]),
+    "fla_gated_linear_bwd_gate": (c_int, [P] * 7 + [I64, I64, I64, I64, I, I, P]),
     "fla_gated_linear_bwd_dx_splits": (c_int, [I64, I64, I64]),
     "fla_gated_linear_bwd_dx": (c_int, [P] * 5 + [I64, I64, I64, I64, I, P, P]),
     "fla_gated_linear_bwd_dw_splits": (c_int, [I64, I64, I64, I]),

@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define FLA_ABI_VERSION 27
+#define FLA_ABI_VERSION 28
 
 enum fla_dtype { FLA_F32 = 0, FLA_BF16 = 1, FLA_F16 = 2 };
 
@@ -859,14 +859,15 @@ int fla_rms_norm_rows8_fwd(const void* x, const void* residual, int residual_dty
  * Layer norm of rows with the residual's addition (interface of LayerNorm / layer_norm, fla/modules/layernorm.py):
  *   s = x + residual,  mu = mean s,  y = (s - mu) / sqrt(mean (s - mu)^2 + eps) * weight (+ bias).
  * Operands, types and limits as for the RMS norm; mean, rstd fp32 [M], both or neither, for the backward.  rows8: FLA_ROWS_NONE (scale
- * NULL) or the type of the 8-bit rows in y, with `scale`.  dw_partial, db_partial: fp32 [fla_layer_norm_workgroups(M, N), N]. */
+ * NULL) or the type of the 8-bit rows in y, with `scale`.  dw_partial, db_partial: fp32
+ * [fla_layer_norm_workgroups(M, N), N], rows partial_ld elements apart (16-byte addresses and pitch where N % 8 == 0 and every operand is at one). */
 int fla_layer_norm_workgroups(int64_t M, int64_t N);
 int fla_layer_norm_fwd(const void* x, const void* residual, int residual_dtype, const void* weight, const void* bias,
                        int weight_dtype, void* y, float* scale, void* residual_out, int residual_out_dtype, float* mean, float* rstd,
                        int64_t M, int64_t N, float eps, int rows8, int dtype, fla_stream_t stream);
 int fla_layer_norm_bwd(const void* dy, const void* kept, int kept_dtype, const void* weight, int weight_dtype, const float* mean,
                        const float* rstd, const void* dresidual, void* dx, void* dresidual_in, float* dw_partial, float* db_partial,
-                       int64_t M, int64_t N, int dtype, fla_stream_t stream);
+                       int64_t partial_ld, int64_t M, int64_t N, int dtype, fla_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Product of 8-bit rows, the projection behind the norm above (no counterpart in the reference, whose projections are
@@ -901,7 +902,7 @@ int fla_int8_linear(const void* x, const float* x_scale, const void* weight, con
  *
  * Backward, in three steps:
  *   _bwd_gate: dgate = dh u act'(g), dup = dh act(g), both [M,ld] with zeros behind F, from the kept g and u; *_bias_partial: fp32
- *     [ceil(M / fla_gated_linear_bwd_rows(M)), F] or NULL, their column sums are the biases' gradients.
+ *     [ceil(M / fla_gated_linear_bwd_rows(M)), F], rows partial_ld elements apart, or NULL, their column sums are the biases' gradients.
  *   _bwd_dx: dx [M,K] = dgate gate_weight + dup up_weight; workspace: fp32 [splits, M, K] where _dx_splits is more than one.
  *   _bwd_dw: dgate_weight = dgate' x, dup_weight = dup' x [F,K], either may be NULL (both: whether both are asked for); workspace: fp32
  *     [1 or 2, splits, F, K] where _dw_splits is more than one. */
@@ -916,7 +917,7 @@ int fla_int8_gated_linear_fwd(const void* x, const float* x_scale, const void* g
                               fla_stream_t stream);
 int fla_gated_linear_bwd_rows(int64_t M);
 int fla_gated_linear_bwd_gate(const void* dh, const void* gate, const void* up, void* dgate, void* dup, float* dgate_bias_partial,
-                              float* dup_bias_partial, int64_t ld, int64_t M, int64_t F, int activation, int dtype,
+                              float* dup_bias_partial, int64_t partial_ld, int64_t ld, int64_t M, int64_t F, int activation, int dtype,
                               fla_stream_t stream);
 int fla_gated_linear_bwd_dx_splits(int64_t M, int64_t F, int64_t K);
 int fla_gated_linear_bwd_dx(const void* dgate, const void* dup, const void* gate_weight, const void* up_weight, void* dx, int64_t ld,

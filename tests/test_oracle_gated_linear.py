@@ -83,8 +83,9 @@ def test_library_entries_refuse():
     assert fwd(x=None) == -1 and fwd(K=0) == -1 and fwd(act=4) == -1 and fwd(g=at) == -1
     assert fwd(K=12) == -2 and fwd(dtype=0) == -2 and fwd(g=at, u=at, ld=32) == -2 and fwd(K=(1 << 22) + 8) == -2
     assert fwd(x=at + 8) == -3 and fwd(M=0) == 0
-    assert lib.fla_gated_linear_bwd_gate(at, at, at, at, at, None, None, 20, 2, 24, 1, 1, None) == -2
-    assert lib.fla_gated_linear_bwd_gate(at, at, at + 4, at, at, None, None, 24, 2, 24, 1, 1, None) == -3
+    assert lib.fla_gated_linear_bwd_gate(at, at, at, at, at, None, None, 0, 20, 2, 24, 1, 1, None) == -2
+    assert lib.fla_gated_linear_bwd_gate(at, at, at + 4, at, at, None, None, 0, 24, 2, 24, 1, 1, None) == -3
+    assert lib.fla_gated_linear_bwd_gate(at, at, at, at, at, at, None, 8, 24, 2, 24, 1, 1, None) == -1
     assert lib.fla_gated_linear_bwd_dx(at, at, at, at, at, 24, 2, 24, 12, 1, None, None) == -2
     assert lib.fla_gated_linear_bwd_dw(at, at, at, None, None, 24, 2, 24, 16, 1, None, None) == -1
     assert lib.fla_gated_linear_bwd_dw(at, at, at, at, at, 24, 0, 24, 16, 1, None, None) == -1

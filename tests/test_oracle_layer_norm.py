@@ -72,6 +72,7 @@ def test_library_entry_refuses():
     fwd = lambda scale, rows8, N=16, dtype=0: lib.fla_layer_norm_fwd(at, None, 0, None, None, 0, at, scale, None, 0, None, None, 1, N, 1e-5, rows8,
                                                                      dtype, None)
     assert fwd(None, 1) == -1 and fwd(at, 0) == -1 and fwd(at, 3) == -1 and fwd(None, 0, N=16385) == -2 and fwd(None, 0, N=0) == -1
-    assert lib.fla_layer_norm_bwd(at, at, 0, None, 0, None, at, None, at, None, None, None, 1, 16, 0, None) == -1      # no mean
-    assert lib.fla_layer_norm_bwd(at, at, 0, None, 0, at, at, None, at, None, at + 4, None, 1, 16, 0, None) == -3
+    assert lib.fla_layer_norm_bwd(at, at, 0, None, 0, None, at, None, at, None, None, None, 16, 1, 16, 0, None) == -1      # no mean
+    assert lib.fla_layer_norm_bwd(at, at, 0, None, 0, at, at, None, at, None, at + 4, None, 16, 1, 16, 0, None) == -3
+    assert lib.fla_layer_norm_bwd(at, at, 0, None, 0, at, at, None, at, None, at, None, 8, 1, 16, 0, None) == -1
     assert lib.fla_rms_norm_rows8_fwd(at, None, 0, None, None, 0, at, None, None, 0, 1, 16, 1e-5, 1, 2, 0, None) == -1
