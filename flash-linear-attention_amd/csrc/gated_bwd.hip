@@ -65,13 +65,14 @@ struct GradParams {
   const char *a, *b;         // dx: Wg, Wu [F,K];  weights' gradients: x [M,K], -
   void *y, *y2;              // dx [M,K];  dWg, dWu [F,K], either may be NULL
   float* part;               // sums of slices [splits, (2,) rows, K], or NULL
-  int64_t M, F, K, ld;
+  int64_t M, F, K, ld;       // K: columns of the operands, a multiple of 8
+  int64_t columns;           // of the results, those below K that are wanted
   int splits;
 };
 
-// A tile of a gradient of `rows` rows of K elements; 1: every store was made, 16 bytes each
+// A tile of a gradient of `rows` rows of `columns` elements, or of its sums of K; 1: every store was made, 16 bytes each
 template <typename T, typename Tile>
-FLA_DEVICE int grad_store(const Tile& t, const typename Tile::acc_t (&acc)[Tile::MT][Tile::NT], T* y, float* part, int64_t m0, int64_t n0, int64_t rows, int64_t K) {
+FLA_DEVICE int grad_store(const Tile& t, const typename Tile::acc_t (&acc)[Tile::MT][Tile::NT], T* y, float* part, int64_t m0, int64_t n0, int64_t rows, int64_t K, int64_t columns) {
   const int lr = t.lane & 31, lh = t.lane >> 5;
 #pragma unroll
   for (int i = 0; i < Tile::MT; ++i) {
@@ -92,13 +93,13 @@ FLA_DEVICE int grad_store(const Tile& t, const typename Tile::acc_t (&acc)[Tile:
 #pragma unroll
           for (int r = 0; r < 4; ++r) a[r] = v[8 * q + r], b[r] = v[8 * q + 4 + r];
           const i32x4 o = mat_join(pack4<T>(a), pack4<T>(b));
-          if (m < rows && n + 16 * q + 8 * lh < K) *(i32x4*)(y + m * K + n + 16 * q + 8 * lh) = o;      // (K is a multiple of 8)
+          if (m < rows) store_piece(y + m * columns, n + 16 * q + 8 * lh, columns, o);
         }
       }
       mat_piece_end();
     }
   }
-  return !part && m0 + Tile::MT * 64 <= rows && n0 + Tile::NT * 64 <= K;
+  return !part && m0 + Tile::MT * 64 <= rows && n0 + Tile::NT * 64 <= columns;
 }
 
 // dx = dg Wg + du Wu: the slices of the first product, then those of the second
@@ -124,7 +125,7 @@ struct DxJob {
   }
   template <typename Tile>
   FLA_DEVICE int finish(const Tile& t, const typename Tile::acc_t (&acc)[Tile::MT][Tile::NT], int) const {
-    return grad_store(t, acc, (T*)p.y, p.splits > 1 ? p.part + blockIdx.y * p.M * p.K : nullptr, m0, n0, p.M, p.K);
+    return grad_store(t, acc, (T*)p.y, p.splits > 1 ? p.part + blockIdx.y * p.M * p.K : nullptr, m0, n0, p.M, p.K, p.columns);
   }
 };
 template <typename T, int BM, int BN, int PER_SIMD, bool HALVES>
@@ -164,7 +165,7 @@ struct DwJob {
   template <typename Tile>
   FLA_DEVICE int finish(const Tile& t, const typename Tile::acc_t (&acc)[Tile::MT][Tile::NT], int) const {
     const bool second = up && p.y;
-    return grad_store(t, acc, (T*)(up ? p.y2 : p.y), p.splits > 1 ? p.part + ((second ? p.splits : 0) + (int64_t)blockIdx.y) * p.F * p.K : nullptr, m0, n0, p.F, p.K);
+    return grad_store(t, acc, (T*)(up ? p.y2 : p.y), p.splits > 1 ? p.part + ((second ? p.splits : 0) + (int64_t)blockIdx.y) * p.F * p.K : nullptr, m0, n0, p.F, p.K, p.columns);
   }
 };
 template <typename T, int BM, int BN, int PER_SIMD, bool HALVES>
@@ -176,10 +177,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PER_SIMD, P
   mat_run(lds, grid, job);
 }
 
-// the sums of slices, added in their order: four elements a thread
+// the sums of slices [splits, rows, K], added in their order: four elements a thread, of which those in `columns` leave
 template <typename T>
-__global__ __launch_bounds__(256) void grad_finish_kernel(const float* part, T* y, T* y2, int64_t n, int splits) {
-  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+__global__ __launch_bounds__(256) void grad_finish_kernel(const float* part, T* y, T* y2, int64_t rows, int64_t K, int64_t columns, int splits) {
+  const int64_t n = rows * K, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
   if (at >= n) return;
   const float* from = part + (int64_t)blockIdx.y * splits * n + at;
   f32x4 v = *(const f32x4*)from;
@@ -187,10 +188,17 @@ __global__ __launch_bounds__(256) void grad_finish_kernel(const float* part, T* 
   typename Elem<T>::v4 o;
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = (T)v[i];
-  *(typename Elem<T>::v4*)((blockIdx.y || !y ? y2 : y) + at) = o;
+  T* out = blockIdx.y || !y ? y2 : y;
+  if (columns == K) {
+    *(typename Elem<T>::v4*)(out + at) = o;
+  } else {
+    const int64_t m = at / K, c = at - m * K;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i < columns) out[m * columns + c + i] = o[i];
+  }
 }
 
-// ------------------------------------------------------------------------------------------------ host
 TilePlan plan_dx(int64_t M, int64_t F, int64_t K) { return plan_tiles(M, K, 2 * fla_cdiv(F * 2, kSliceBytes), 1, false); }
 TilePlan plan_dw(int64_t M, int64_t F, int64_t K, int batch) { return plan_tiles(F, K, fla_cdiv(M, 64), batch, false); }
 
@@ -206,7 +214,7 @@ int launch_dx(const GradParams& p, TileKind kind, hipStream_t st) {
   FLA_CHECK_LAUNCH();
   if (p.splits > 1) {
     const int64_t n = p.M * p.K;
-    hipLaunchKernelGGL((grad_finish_kernel<T>), dim3((unsigned)fla_cdiv(n, 1024)), dim3(256), 0, st, p.part, (T*)p.y, (T*)p.y, n, p.splits);
+    hipLaunchKernelGGL((grad_finish_kernel<T>), dim3((unsigned)fla_cdiv(n, 1024)), dim3(256), 0, st, p.part, (T*)p.y, (T*)p.y, p.M, p.K, p.columns, p.splits);
     FLA_CHECK_LAUNCH();
   }
   return FLA_OK;
@@ -224,7 +232,7 @@ int launch_dw(const GradParams& p, TileKind kind, hipStream_t st) {
   FLA_CHECK_LAUNCH();
   if (p.splits > 1) {
     const int64_t n = p.F * p.K;
-    hipLaunchKernelGGL((grad_finish_kernel<T>), dim3((unsigned)fla_cdiv(n, 1024), batch), dim3(256), 0, st, p.part, (T*)p.y, (T*)p.y2, n, p.splits);
+    hipLaunchKernelGGL((grad_finish_kernel<T>), dim3((unsigned)fla_cdiv(n, 1024), batch), dim3(256), 0, st, p.part, (T*)p.y, (T*)p.y2, p.F, p.K, p.columns, p.splits);
     FLA_CHECK_LAUNCH();
   }
   return FLA_OK;
@@ -258,17 +266,17 @@ extern "C" int fla_gated_linear_bwd_gate(const void* dh, const void* gate, const
 extern "C" int fla_gated_linear_bwd_dx_splits(int64_t M, int64_t F, int64_t K) { return M <= 0 || F <= 0 || K <= 0 ? 1 : plan_dx(M, F, K).splits; }
 
 extern "C" int fla_gated_linear_bwd_dx(const void* dgate, const void* dup, const void* gate_weight, const void* up_weight, void* dx, int64_t ld,
-                                       int64_t M, int64_t F, int64_t K, int dtype, float* workspace, fla_stream_t stream) {
+                                       int64_t columns, int64_t M, int64_t F, int64_t K, int dtype, float* workspace, fla_stream_t stream) {
   FLA_REQUIRE(dgate && dup && gate_weight && up_weight && dx && M >= 0 && F > 0 && K > 0, FLA_E_INVALID);
   FLA_REQUIRE(dtype == FLA_BF16 || dtype == FLA_F16, FLA_E_UNSUPPORTED);
-  FLA_REQUIRE(sizes_ok(M, F, K) && K % 8 == 0 && ld >= F && ld % 8 == 0 && ld < F + 8, FLA_E_UNSUPPORTED);
-  FLA_REQUIRE(aligned16({dgate, dup, gate_weight, up_weight, dx, workspace}), FLA_E_ALIGNMENT);
+  FLA_REQUIRE(sizes_ok(M, F, K) && K % 8 == 0 && ld >= F && ld % 8 == 0 && ld < F + 8 && columns > 0 && columns <= K, FLA_E_UNSUPPORTED);
+  FLA_REQUIRE(aligned16({dgate, dup, gate_weight, up_weight, columns == K ? dx : nullptr, workspace}), FLA_E_ALIGNMENT);
   if (M == 0) return FLA_OK;
   const TilePlan plan = plan_dx(M, F, K);
   FLA_REQUIRE(plan.splits == 1 || workspace, FLA_E_INVALID);
   GradParams p{};
   p.dg = (const char*)dgate, p.du = (const char*)dup, p.a = (const char*)gate_weight, p.b = (const char*)up_weight, p.y = dx, p.part = workspace;
-  p.M = M, p.F = F, p.K = K, p.ld = ld, p.splits = plan.splits;
+  p.M = M, p.F = F, p.K = K, p.ld = ld, p.columns = columns, p.splits = plan.splits;
   hipStream_t st = (hipStream_t)stream;
   return dtype == FLA_BF16 ? launch_dx<bf16>(p, plan.kind, st) : launch_dx<f16>(p, plan.kind, st);
 }
@@ -277,17 +285,17 @@ extern "C" int fla_gated_linear_bwd_dw_splits(int64_t M, int64_t F, int64_t K, i
   return M <= 0 || F <= 0 || K <= 0 ? 1 : plan_dw(M, F, K, both ? 2 : 1).splits;
 }
 
-extern "C" int fla_gated_linear_bwd_dw(const void* dgate, const void* dup, const void* x, void* dgate_weight, void* dup_weight, int64_t ld, int64_t M,
-                                       int64_t F, int64_t K, int dtype, float* workspace, fla_stream_t stream) {
+extern "C" int fla_gated_linear_bwd_dw(const void* dgate, const void* dup, const void* x, void* dgate_weight, void* dup_weight, int64_t ld,
+                                       int64_t columns, int64_t M, int64_t F, int64_t K, int dtype, float* workspace, fla_stream_t stream) {
   FLA_REQUIRE(x && (dgate_weight || dup_weight) && (!dgate_weight || dgate) && (!dup_weight || dup) && M > 0 && F > 0 && K > 0, FLA_E_INVALID);
   FLA_REQUIRE(dtype == FLA_BF16 || dtype == FLA_F16, FLA_E_UNSUPPORTED);
-  FLA_REQUIRE(sizes_ok(M, F, K) && K % 8 == 0 && ld >= F && ld % 8 == 0 && ld < F + 8, FLA_E_UNSUPPORTED);
-  FLA_REQUIRE(aligned16({dgate, dup, x, dgate_weight, dup_weight, workspace}), FLA_E_ALIGNMENT);
+  FLA_REQUIRE(sizes_ok(M, F, K) && K % 8 == 0 && ld >= F && ld % 8 == 0 && ld < F + 8 && columns > 0 && columns <= K, FLA_E_UNSUPPORTED);
+  FLA_REQUIRE(aligned16({dgate, dup, x, columns == K ? dgate_weight : nullptr, columns == K ? dup_weight : nullptr, workspace}), FLA_E_ALIGNMENT);
   const TilePlan plan = plan_dw(M, F, K, dgate_weight && dup_weight ? 2 : 1);
   FLA_REQUIRE(plan.splits == 1 || workspace, FLA_E_INVALID);
   GradParams p{};
   p.dg = (const char*)dgate, p.du = (const char*)dup, p.a = (const char*)x, p.y = dgate_weight, p.y2 = dup_weight, p.part = workspace;
-  p.M = M, p.F = F, p.K = K, p.ld = ld, p.splits = plan.splits;
+  p.M = M, p.F = F, p.K = K, p.ld = ld, p.columns = columns, p.splits = plan.splits;
   hipStream_t st = (hipStream_t)stream;
   return dtype == FLA_BF16 ? launch_dw<bf16>(p, plan.kind, st) : launch_dw<f16>(p, plan.kind, st);
 }

@@ -873,21 +873,25 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
     int64_t F;
     long act;
   };
-  // kept: g and u [2, M, ld] for a backward, or NULL
-  static Tensor run(const Tensor& x_, const Tensor& wg_, const Tensor& wu_, const Tensor& bg_, const Tensor& bu_, long act, Tensor* kept) {
+  // kept: g and u [2, M, ld] for a backward, and the operands as the kernels took them; or NULL
+  struct Kept {
+    Tensor gu, x, wg, wu;
+  };
+  static Tensor run(const Tensor& x_, const Tensor& wg_, const Tensor& wu_, const Tensor& bg_, const Tensor& bu_, long act, Kept* kept) {
     const int64_t F = wg_.size(0), K0 = x_.size(-1), M = x_.numel() / K0, ld = (F + 7) / 8 * 8;
     auto shape = x_.sizes().vec();
     shape.back() = F;
     Tensor h = fresh(shape, x_, x_.scalar_type());
-    if (kept) *kept = fresh({2, M, ld}, x_, x_.scalar_type());
+    if (kept) kept->gu = fresh({2, M, ld}, x_, x_.scalar_type());
     if (M == 0) return h;
     const Tensor x = whole_rows(x_, 8), wg = whole_rows(wg_, 8), wu = whole_rows(wu_, 8);
+    if (kept) kept->x = x, kept->wg = wg, kept->wu = wu;
     const bool same = (!bg_.defined() || bg_.scalar_type() == x.scalar_type()) && (!bu_.defined() || bu_.scalar_type() == x.scalar_type());
     const Tensor bg = whole_bias(same ? bg_ : f32(bg_)), bu = whole_bias(same ? bu_ : f32(bu_));
     const int64_t K = x.size(-1);
     const int splits = fla_gated_linear_splits(M, F, K, 2);
     const Tensor sums = splits > 1 ? fresh({splits, M, 2, F}, x, at::kFloat) : Tensor();
-    char* keep = kept ? (char*)kept->data_ptr() : nullptr;
+    char* keep = kept ? (char*)kept->gu.data_ptr() : nullptr;
     check(fla_gated_linear_fwd(ptr(x), ptr(wg), ptr(wu), ptr(bg), ptr(bu), same ? dt(x) : FLA_F32, ptr(h), keep,
                                keep ? keep + M * ld * 2 : nullptr, ld, M, F, K, (int)act, dt(x), ptr(sums), stream_of(x)),
           "fla_gated_linear_fwd");
@@ -896,12 +900,15 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu, const Maybe& bg_, const Maybe& bu_, long act) {
     at::AutoDispatchBelowADInplaceOrView guard;
     const Tensor bg = given(bg_), bu = given(bu_);
-    Tensor kept;
+    Kept kept;
     Tensor h = run(x, wg, wu, bg, bu, act, &kept);
     const Rest r{asks(x), asks(wg), asks(wu), asks(bg), asks(bu), bg.defined() ? bg.scalar_type() : at::kFloat, bu.defined() ? bu.scalar_type() : at::kFloat,
                  wg.size(0), act};
     // (x for the weights' gradients, the weights for x's)
-    ctx->save_for_backward({r.wg || r.wu ? x : Tensor(), r.x ? wg : Tensor(), r.x ? wu : Tensor(), kept});
+    // The operands themselves are saved, so that a backward after they were written to is refused, and beside them what they were copied into, if they were.
+    auto copy = [](bool wanted, const Tensor& k, const Tensor& t) { return wanted && k.defined() && !k.is_same(t) && k.data_ptr() != t.data_ptr() ? k : Tensor(); };
+    const bool w = r.wg || r.wu;
+    ctx->save_for_backward({w ? x : Tensor(), r.x ? wg : Tensor(), r.x ? wu : Tensor(), kept.gu, copy(w, kept.x, x), copy(r.x, kept.wg, wg), copy(r.x, kept.wu, wu)});
     ctx->saved_data["shape"] = x.sizes().vec();
     hold(ctx, r);
     return h;
@@ -931,22 +938,19 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
           "fla_gated_linear_bwd_gate");
     part.sums(&dbg, &dbu);
     if (r.x) {
-      const Tensor wg = whole_rows(saved[1], 8), wu = whole_rows(saved[2], 8);
-      dx = fresh({M, K}, kept, type);
+      const Tensor wg = saved[5].defined() ? saved[5] : whole_rows(saved[1], 8), wu = saved[6].defined() ? saved[6] : whole_rows(saved[2], 8);
+      dx = fresh(shape, kept, type);
       const int splits = fla_gated_linear_bwd_dx_splits(M, F, K);
       const Tensor sums = splits > 1 ? fresh({splits, M, K}, kept, at::kFloat) : Tensor();
-      check(fla_gated_linear_bwd_dx(dg, dg + half, ptr(wg), ptr(wu), ptr(dx), ld, M, F, K, dt(kept), fptr(sums), stream), "fla_gated_linear_bwd_dx");
-      dx = (K == K0 ? dx : dx.narrow(1, 0, K0).contiguous()).view(shape);
+      check(fla_gated_linear_bwd_dx(dg, dg + half, ptr(wg), ptr(wu), ptr(dx), ld, K0, M, F, K, dt(kept), fptr(sums), stream), "fla_gated_linear_bwd_dx");
     }
     if (r.wg || r.wu) {
-      const Tensor x = whole_rows(saved[0], 8);
-      if (r.wg) dwg = fresh({F, K}, kept, type);
-      if (r.wu) dwu = fresh({F, K}, kept, type);
+      const Tensor x = saved[4].defined() ? saved[4] : whole_rows(saved[0], 8);
+      if (r.wg) dwg = fresh({F, K0}, kept, type);
+      if (r.wu) dwu = fresh({F, K0}, kept, type);
       const int splits = fla_gated_linear_bwd_dw_splits(M, F, K, r.wg && r.wu);
       const Tensor sums = splits > 1 ? fresh({r.wg && r.wu ? 2 : 1, splits, F, K}, kept, at::kFloat) : Tensor();
-      check(fla_gated_linear_bwd_dw(dg, dg + half, ptr(x), ptr(dwg), ptr(dwu), ld, M, F, K, dt(kept), fptr(sums), stream), "fla_gated_linear_bwd_dw");
-      if (K != K0 && r.wg) dwg = dwg.narrow(1, 0, K0).contiguous();
-      if (K != K0 && r.wu) dwu = dwu.narrow(1, 0, K0).contiguous();
+      check(fla_gated_linear_bwd_dw(dg, dg + half, ptr(x), ptr(dwg), ptr(dwu), ld, K0, M, F, K, dt(kept), fptr(sums), stream), "fla_gated_linear_bwd_dw");
     }
     return {dx, dwg, dwu, dbg, dbu, Tensor()};
   }

@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define FLA_ABI_VERSION 28
+#define FLA_ABI_VERSION 29
 
 enum fla_dtype { FLA_F32 = 0, FLA_BF16 = 1, FLA_F16 = 2 };
 
@@ -903,6 +903,7 @@ int fla_int8_linear(const void* x, const float* x_scale, const void* weight, con
  * Backward, in three steps:
  *   _bwd_gate: dgate = dh u act'(g), dup = dh act(g), both [M,ld] with zeros behind F, from the kept g and u; *_bias_partial: fp32
  *     [ceil(M / fla_gated_linear_bwd_rows(M)), F], rows partial_ld elements apart, or NULL, their column sums are the biases' gradients.
+ *   Of operands that were brought to a multiple of 8 columns by zeros, results have the `columns` that are wanted (otherwise K) and any address.
  *   _bwd_dx: dx [M,K] = dgate gate_weight + dup up_weight; workspace: fp32 [splits, M, K] where _dx_splits is more than one.
  *   _bwd_dw: dgate_weight = dgate' x, dup_weight = dup' x [F,K], either may be NULL (both: whether both are asked for); workspace: fp32
  *     [1 or 2, splits, F, K] where _dw_splits is more than one. */
@@ -921,10 +922,10 @@ int fla_gated_linear_bwd_gate(const void* dh, const void* gate, const void* up, 
                               fla_stream_t stream);
 int fla_gated_linear_bwd_dx_splits(int64_t M, int64_t F, int64_t K);
 int fla_gated_linear_bwd_dx(const void* dgate, const void* dup, const void* gate_weight, const void* up_weight, void* dx, int64_t ld,
-                            int64_t M, int64_t F, int64_t K, int dtype, float* workspace, fla_stream_t stream);
+                            int64_t columns, int64_t M, int64_t F, int64_t K, int dtype, float* workspace, fla_stream_t stream);
 int fla_gated_linear_bwd_dw_splits(int64_t M, int64_t F, int64_t K, int both);
-int fla_gated_linear_bwd_dw(const void* dgate, const void* dup, const void* x, void* dgate_weight, void* dup_weight, int64_t ld, int64_t M,
-                            int64_t F, int64_t K, int dtype, float* workspace, fla_stream_t stream);
+int fla_gated_linear_bwd_dw(const void* dgate, const void* dup, const void* x, void* dgate_weight, void* dup_weight, int64_t ld,
+                            int64_t columns, int64_t M, int64_t F, int64_t K, int dtype, float* workspace, fla_stream_t stream);
 
 /* Diagnostics: C[M,N] (fp32) = A[M,Kd] * B[N,Kd]^T with bf16 operands, computed
  * with the same MFMA fragment helpers the kernels use (mode 0: 32x32x16 tiles,

@@ -86,8 +86,9 @@ def test_library_entries_refuse():
     assert lib.fla_gated_linear_bwd_gate(at, at, at, at, at, None, None, 0, 20, 2, 24, 1, 1, None) == -2
     assert lib.fla_gated_linear_bwd_gate(at, at, at + 4, at, at, None, None, 0, 24, 2, 24, 1, 1, None) == -3
     assert lib.fla_gated_linear_bwd_gate(at, at, at, at, at, at, None, 8, 24, 2, 24, 1, 1, None) == -1
-    assert lib.fla_gated_linear_bwd_dx(at, at, at, at, at, 24, 2, 24, 12, 1, None, None) == -2
-    assert lib.fla_gated_linear_bwd_dw(at, at, at, None, None, 24, 2, 24, 16, 1, None, None) == -1
-    assert lib.fla_gated_linear_bwd_dw(at, at, at, at, at, 24, 0, 24, 16, 1, None, None) == -1
+    assert lib.fla_gated_linear_bwd_dx(at, at, at, at, at, 24, 12, 2, 24, 12, 1, None, None) == -2
+    assert lib.fla_gated_linear_bwd_dx(at, at, at, at, at, 24, 17, 2, 24, 16, 1, None, None) == -2
+    assert lib.fla_gated_linear_bwd_dw(at, at, at, None, None, 24, 16, 2, 24, 16, 1, None, None) == -1
+    assert lib.fla_gated_linear_bwd_dw(at, at, at, at, at, 24, 16, 0, 24, 16, 1, None, None) == -1
     split = lib.fla_gated_linear_bwd_dw_splits(8192, 256, 256, 1)
-    assert split > 1 and lib.fla_gated_linear_bwd_dw(at, at, at, at, at, 256, 8192, 256, 256, 1, None, None) == -1      # no workspace
+    assert split > 1 and lib.fla_gated_linear_bwd_dw(at, at, at, at, at, 256, 256, 8192, 256, 256, 1, None, None) == -1      # no workspace
