@@ -69,6 +69,18 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+// A leaf's accumulation node stays on the stream that was current when it was made, for as long as a graph holds it.  One of the default stream, which
+// cannot be captured, makes a captured backward pass end the process: the call is refused while it is only a call.
+void refuse_eager_leaves(std::initializer_list<const Tensor*> ts, const char* who) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  for (const Tensor* t : ts) {
+    if (!t->defined() || !t->is_leaf() || !t->requires_grad()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    const auto stream = node ? node->stream() : std::nullopt;
+    TORCH_CHECK(!stream || stream->id() != 0, "fla_amd ", who, ": an eager graph of the default stream still holds these leaves, and a backward pass "
+                "of theirs cannot be captured: drop its results ahead of the capture, or call this under torch.no_grad()");
+  }
+}
 bool on_gpu(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->defined() && !t->is_cuda()) return false;
@@ -1388,6 +1400,7 @@ PyObject* py_norm(PyObject*, PyObject* const* p, Py_ssize_t n) {
   const bool grad = wants_grad({&x, &w, &b, &res});
   TORCH_CHECK(!(grad && a.rows8), "fla_amd: rows in 8 bits have no gradient; call it under torch.no_grad()");
   c10::DeviceGuard on_device(x.device());
+  if (grad && a.kind == kLayer) refuse_eager_leaves({&x, &w, &b, &res}, "layer_norm");
   // one type for both, x's or fp32
   auto fits = [&](const Tensor& t) { return !t.defined() || t.scalar_type() == x.scalar_type(); };
   if (!fits(w) || !fits(b)) w = f32(w), b = f32(b);
@@ -1549,7 +1562,9 @@ PyObject* py_gated_linear(PyObject*, PyObject* const* p, Py_ssize_t n) {
                               "fla_amd gated_linear: weights of at most 2^22 rows and columns, x of less than 2^31 rows");
   need_gpu({&x, &wg, &wu, &bg, &bu});
   c10::DeviceGuard on_device(x.device());
-  if (wants_grad({&x, &wg, &wu, &bg, &bu})) return THPVariable_Wrap(GatedNode::apply(x, wg, wu, maybe(bg), maybe(bu), act));
+  const bool grad = wants_grad({&x, &wg, &wu, &bg, &bu});
+  if (grad) refuse_eager_leaves({&x, &wg, &wu, &bg, &bu}, "gated_linear");
+  if (grad) return THPVariable_Wrap(GatedNode::apply(x, wg, wu, maybe(bg), maybe(bu), act));
   at::AutoDispatchBelowADInplaceOrView guard;
   return THPVariable_Wrap(GatedNode::run(x, wg, wu, bg, bu, act, nullptr));
   END_HANDLE_TH_ERRORS

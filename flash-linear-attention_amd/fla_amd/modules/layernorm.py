@@ -32,7 +32,8 @@ def rms_norm(x, weight, bias=None, residual=None, prenorm=False, residual_in_fp3
 
 def layer_norm(x, weight, bias=None, residual=None, prenorm=False, residual_in_fp32=False, eps=1e-6, quantize=False):
     """``y = (s - mean(s)) / sqrt(var(s) + eps) * weight (+ bias)`` over the last dimension, ``s = x + residual``, ``var`` the mean square of
-    ``s - mean(s)``; one launch each way.  Arguments, results and limits as those of :func:`rms_norm`."""
+    ``s - mean(s)``; one launch each way.  Arguments, results and limits as those of :func:`rms_norm`.
+    Under capture a call with gradients is refused while an eager graph of the default stream holds one of its leaves: a backward could not be captured."""
     return host().norm(x, weight, bias, residual, eps, prenorm, residual_in_fp32, _rows8(quantize), _LAYER)
 
 

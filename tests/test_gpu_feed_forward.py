@@ -152,3 +152,33 @@ def test_captured_serving(device):
         torch.cuda.synchronize()
         assert torch.equal(out, eager[i]), i
         _serve(*block, *data[2])
+
+
+def test_capture_refuses_leaves_of_an_eager_graph(device):
+    """Refused ahead of any launch: the backward pass is never reached.  Without gradients, and once the eager graph is gone, the calls are captured."""
+    from fla_amd.modules import gated_linear, layer_norm
+    g = torch.Generator().manual_seed(3)
+    leaf = lambda *s: torch.randn(*s, generator=g).to(device, torch.bfloat16).requires_grad_()
+    x, wg, wu, bg, w, b = leaf(40, 64), leaf(96, 64), leaf(96, 64), leaf(96), leaf(64), leaf(64)
+    calls = [lambda: gated_linear(x.detach(), wg, wu, bg), lambda: gated_linear(x.detach(), wg.detach(), wu.detach(), bg),
+             lambda: layer_norm(x, w, b), lambda: layer_norm(x.detach(), w.detach(), b)]
+    for call in calls:
+        y = call()
+        torch.cuda.synchronize()
+        expected = y.detach().clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            still = torch.ones(1, device=device)
+            with pytest.raises(RuntimeError, match="eager graph"):
+                call()
+            with torch.no_grad():
+                out = call()
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, expected) and still.item() == 1
+        del y, out
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            out = call()
+        assert out.requires_grad
+        del out
