@@ -1,6 +1,8 @@
 // Products with few rows of x:  c[m,n] = sum_k x[m,k] w[n,k]  for at most MT x 16 rows m and 16 rows n of one matrix w, or of each of two.
 // The bytes of w bound it, and those of x out of L2 from 32 rows on.  The waves take slices of 128 bytes of k in turn, each through RING pieces of LDS of
 // its own, waiting for nobody until the sums are added in the waves' order.
+// Measured (bf16, two weights, out of HBM, in a captured graph): 1 x 4096 to 11008 37.4 us (4.8 TB/s of the weights), 16 rows 38.3, 32 42.9, 48 45.8, 64 51.9 (x comes once for
+// every 16 columns: at 64 rows twice the weights' bytes); 1 x 2048 to 5632 12.1.  One or two waves a workgroup and rings of three and four were none faster.
 #pragma once
 #include "matrix_tiles.h"
 

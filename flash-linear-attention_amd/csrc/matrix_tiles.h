@@ -9,6 +9,13 @@
 // A wave's quarter of 128 x 128 reads 32 fragments for 64 instructions: 128 KB a slice and CU, half of what LDS passes in that time.  (Eight waves
 // of 128 x 64 read 192 KB, which with the 64 KB of the copies is all of it.)
 //
+// Measured (bf16): 8192^3 812 us, 1.35 PFLOP/s (torch 706 - 717; with the contraction strided in both operands 810 - 817, torch 949 - 960), 8192 x 11264 x 2048 340 us (torch 395),
+// 8192 x 2048 x 11264 with it strided in one 296 (torch 329), 5632 x 2048 x 8192 with it strided in both 178 (torch 207 - 214).  The card holds 1.55 GHz under 8192^3
+// (GRBM_GUI_ACTIVE); of 1.37M cycles 1.05M are matrix instructions.  With copies of the same lines again and again it takes 1.21M: what is lost is memory's side.
+// Tried and slower or no faster: the 16x16 instruction (the compiler moves accumulators between the loops' registers), slices of 64 bytes in rings of three to five (of 1.41M cycles
+// copies and LDS reads cost 0.22M), pointers instead of descriptors (three vector instructions a copy), a barrier every second slice, copies that the waves issue in turn,
+// a load a line some slices ahead (L2), a ring of three for one operand.
+//
 // Memory is read through buffer descriptors that end where the operand ends: rows and pieces behind it are zeros, by the hardware's range check.
 #pragma once
 #include "fla_common.h"

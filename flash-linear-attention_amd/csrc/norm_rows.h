@@ -365,6 +365,8 @@ __global__ __launch_bounds__(bwd_block(TPR)) void norm_bwd_kernel(NormParams p) 
   else if (N <= 8192) CALL(1024, 1) \
   else CALL(1024, 2)
 
+// Layer norm, bf16 with residual and bias: 16384 rows of 2048 forward 54 - 56 us (4.9 TB/s), backward 59 - 61 (4.5), 4.9 for the launch that adds the partial sums of both gradients.
+// Its backward spills registers in unaligned rows: 2 - 17 in one pass with an fp32 stream, 1 - 70 in two passes (above 8192 elements).
 constexpr int64_t kFewRows = 1024;
 constexpr int64_t kMaxN = 512 * 4 * VEC;         // of rows that stay in registers
 constexpr int64_t kMaxRow8 = 1 << 23;            // of rows that are brought to 8 bits and nothing else: as many as the product takes
