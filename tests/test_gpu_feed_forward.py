@@ -182,3 +182,70 @@ def test_capture_refuses_leaves_of_an_eager_graph(device):
             out = call()
         assert out.requires_grad
         del out
+
+
+MANY, LAST = 1_100_003, 2000      # rows of 2048 elements: offsets of the last ones pass 2^31
+
+
+def test_rows_behind_32_bit_offsets_of_the_norm(device):
+    """The last rows of 2.25e9 elements.  One rounding to bf16 (2^-8 of the value), and below it some tens of fp32 roundings of values of at most 8."""
+    from fla_amd.modules import layer_norm
+    g = torch.Generator().manual_seed(5)
+    some = lambda *s: torch.randn(*s, generator=g).to(device, torch.bfloat16)
+    x, dy = (torch.zeros(MANY, 2048, device=device, dtype=torch.bfloat16) for _ in range(2))
+    x[-LAST:], dy[-LAST:] = some(LAST, 2048), some(LAST, 2048)
+    w, b = some(2048), some(2048)
+    x.requires_grad_()
+    y = layer_norm(x, w, b)
+    dx, = torch.autograd.grad(y, x, dy)
+    xs, ws, bs, ds = (t.detach()[-LAST:].double().cpu() if t.dim() == 2 else t.double().cpu() for t in (x, w, b, dy))
+    c = xs - xs.mean(1, keepdim=True)
+    r = (c.square().mean(1, keepdim=True) + 1e-6).rsqrt()
+    h, d = c * r, ds * ws
+    for a, e in ((y, h * ws + bs), (dx, r * (d - d.mean(1, keepdim=True) - h * (d * h).mean(1, keepdim=True)))):
+        a = a.detach()[-LAST:].double().cpu()
+        assert ((a - e).abs() <= e.abs() / 256 + 2.0 ** -16).all()
+
+
+def test_rows_behind_32_bit_offsets_of_the_gated_product(device):
+    """The last rows of 2.25e9 elements of h and of what is kept, against the same rows by themselves: one slice of K, so the same sums; one row with a
+    gradient, so one product in each of the weights'.  Those of x are sums of 4096 products in two orders, each rounded once to bf16."""
+    from fla_amd.modules import gated_linear
+    g = torch.Generator().manual_seed(6)
+    some = lambda *s: torch.randn(*s, generator=g).to(device, torch.bfloat16)
+    x, dh = torch.zeros(MANY, 64, device=device, dtype=torch.bfloat16), torch.zeros(MANY, 2048, device=device, dtype=torch.bfloat16)
+    x[-LAST:], dh[-1] = some(LAST, 64), some(2048)
+    wg, wu = ((some(2048, 64) / 8).requires_grad_() for _ in range(2))
+    results = []
+    for rows in (MANY, LAST):
+        xs = x[-rows:].detach().requires_grad_()
+        h = gated_linear(xs, wg, wu)
+        dx, dwg, dwu = torch.autograd.grad(h, (xs, wg, wu), dh[-rows:])
+        results.append([h.detach()[-LAST:].clone(), dx[-LAST:].clone(), dwg, dwu])
+        del h, dx
+    (h, dx, dwg, dwu), (h0, dx0, dwg0, dwu0) = results
+    assert h0.abs().sum() > 0 and torch.equal(h, h0) and torch.equal(dwg, dwg0) and torch.equal(dwu, dwu0)
+    p, q = wg.detach().double().cpu(), wu.detach().double().cpu()
+    a, d = x[-1].double().cpu(), dh[-1].double().cpu()
+    gate, up = p @ a, q @ a
+    s = gate.sigmoid()
+    terms = (d * up * s * (1 + gate * (1 - s))).abs() @ p.abs() + (d * gate * s).abs() @ q.abs()
+    assert not dx[:-1].any() and dx0[-1].abs().sum() > 0
+    assert ((dx[-1].double() - dx0[-1].double()).abs().cpu() <= dx0[-1].double().abs().cpu() / 128 + 2 * 4096 * 2.0 ** -24 * 1.02 * terms).all()
+
+
+@pytest.mark.parametrize("K, N", ((2048, 48), (64, 2048)))
+def test_rows_behind_32_bit_offsets_of_integers(device, K, N):
+    """The last rows of 2.25e9 elements of x, or of the results: sums are exact, so the same bits as by themselves."""
+    from fla_amd.modules import quant_gated_linear, quant_linear
+    g = torch.Generator().manual_seed(7)
+    ints = lambda *s: torch.randint(-127, 128, s, generator=g, dtype=torch.int8).to(device)
+    scales = lambda n: (torch.rand(n, generator=g) / 100 + 0.001).to(device)
+    x, sx = torch.zeros(MANY, K, device=device, dtype=torch.int8), torch.ones(MANY, device=device)
+    x[-LAST:], sx[-LAST:] = ints(LAST, K), scales(LAST)
+    w, wu, sw, su = ints(N, K), ints(N, K), scales(N), scales(N)
+    with torch.no_grad():
+        for call in (lambda r: quant_linear((x[-r:], sx[-r:]), (w, sw)),
+                     lambda r: quant_gated_linear((x[-r:], sx[-r:]), (w, sw), (wu, su))):
+            y = call(MANY)[-LAST:].clone()
+            assert y.abs().sum() > 0 and torch.equal(y, call(LAST))
