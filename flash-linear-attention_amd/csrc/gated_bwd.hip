@@ -10,7 +10,8 @@
 namespace {
 
 struct GatedBwdParams {
-  const void *dh, *g, *u;     // [M,F], [M,ld], [M,ld]
+  const void* dh;             // [M,F]
+  const float *g, *u;         // [M,ld]
   void *dg, *du;              // [M,ld]: columns behind F are zeros
   float *pg, *pu;             // partial sums [gridDim.y, F], rows pld apart, or NULL
   int64_t M, F, ld, pld, rows;     // rows: of a workgroup
@@ -18,7 +19,7 @@ struct GatedBwdParams {
 };
 
 // HBM-bound: 8192 x 5632 in 86 - 90 us, 5.1 - 5.4 TB/s of dh, g, u, dg and du, the rate of a large copy.  dg and du leave in the operands' type, since the matrix instructions take
-// nothing wider: half a step each, beside that of g and u.  The biases' gradients are sums of what was not rounded.
+// nothing wider: half a step each.  The biases' gradients are sums of what was not rounded.
 // 512 columns, eight a thread, of `rows` rows, four at a time
 template <typename T>
 __global__ __launch_bounds__(256) void gated_bwd_kernel(GatedBwdParams p) {
@@ -36,8 +37,8 @@ __global__ __launch_bounds__(256) void gated_bwd_kernel(GatedBwdParams p) {
       for (int64_t m = first + rl; m < end; m += 4) {
         float d[8], g[8], u[8];
         Row8<T>::unpack(load_raw8<T, false>((const T*)p.dh + m * p.F + col, valid), d);
-        Row8<T>::load((const T*)p.g + m * p.ld + col, g);
-        Row8<T>::load((const T*)p.u + m * p.ld + col, u);
+        Row8<float>::load(p.g + m * p.ld + col, g);
+        Row8<float>::load(p.u + m * p.ld + col, u);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           float slope;
@@ -246,7 +247,7 @@ int launch_dw(const GradParams& p, TileKind kind, hipStream_t st) {
 
 extern "C" int fla_gated_linear_bwd_rows(int64_t M) { return M <= 0 ? 1 : (int)(fla_cdiv(M, 256) < 32 ? 32 : fla_cdiv(M, 256)); }
 
-extern "C" int fla_gated_linear_bwd_gate(const void* dh, const void* gate, const void* up, void* dgate, void* dup, float* dgate_bias_partial,
+extern "C" int fla_gated_linear_bwd_gate(const void* dh, const float* gate, const float* up, void* dgate, void* dup, float* dgate_bias_partial,
                                          float* dup_bias_partial, int64_t partial_ld, int64_t ld, int64_t M, int64_t F, int activation, int dtype,
                                          fla_stream_t stream) {
   FLA_REQUIRE(dh && gate && up && dgate && dup && M >= 0 && F > 0, FLA_E_INVALID);

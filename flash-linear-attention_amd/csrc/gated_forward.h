@@ -1,7 +1,7 @@
 // The gated product of a feed-forward block:   g = x Wg' + bg,   u = x Wu' + bu,   h = act(g) u      x [M,K], Wg, Wu [F,K], act: none, silu, gelu, relu
 // One launch on the tiles of matrix_tiles.h.  The rows of the two weights alternate in a tile, 32 of each, so that the lane that holds sums of
-// the gate holds those of the same m and n of the other projection, and neither goes through memory.  For the backward g and u are kept in the
-// operands' type: dg and du then carry that rounding beside their own, each half a step.  h itself comes from the fp32 sums.
+// the gate holds those of the same m and n of the other projection, and neither goes through memory.  For the backward g and u are kept in fp32, as they
+// are summed: the slope of a gate that fp16 does not hold is right, and dg and du carry their own rounding to 16 bits alone.
 // Measured: 8191 x 2048 to 5632 with gelu and biases 358 - 371 us (1.02 - 1.06 PFLOP/s; torch's product alone of that size 395), with silu and g, u kept 385 - 398, in integers 204 - 224
 // (1.7 - 1.85 POP/s).  Its 1408 tiles are five and a half rounds of some 65 us, of which 32 slices at 1.6 are 51.  What
 // bounds it: the rate of slices (matrix_tiles.h), then the ends of tiles: activations, and stores of 16 bytes a lane.
@@ -19,7 +19,7 @@ struct GatedParams {
   const float *sx, *sg, *su;     // scales of rows of 8-bit integers
   const void *bg, *bu;           // [F] or NULL
   void *h;                       // [M,F]
-  void *g, *u;                   // [M,ldk], kept for the backward, or NULL
+  float *g, *u;                  // [M,ldk], kept for the backward, or NULL
   void* part;                    // sums of slices of K [splits, M, 2, F], fp32 or int32, or NULL
   int64_t M, F, K, ldk;
   int act, bias_f32, splits;
@@ -116,7 +116,7 @@ struct GatedJob {
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
             const int nl = t.wn * (TN / 2) + h * 32 + 16 * q + 4 * lh;     // of the first run of four; the second is eight further
-            u32x2 hv[2], gv[2], uv[2];
+            u32x2 hv[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const f32x4 bg = bias4(side, 0, nl + 8 * e), bu = bias4(side, 1, nl + 8 * e);
@@ -130,18 +130,16 @@ struct GatedJob {
                 else g[r] += bg[r], u[r] += bu[r];
                 v[r] = activate_gate<decltype(act)::value>(g[r]) * u[r];
               }
-              hv[e] = pack4<O>(v), gv[e] = pack4<O>(g), uv[e] = pack4<O>(u);
+              hv[e] = pack4<O>(v);
+              const int64_t n = n0 + nl + 8 * e;
+              if (!INT && p.g && m < p.M && n < p.ldk) {     // (ldk is a multiple of 8)
+                *(f32x4*)(p.g + m * p.ldk + n) = f32x4{g[0], g[1], g[2], g[3]};
+                *(f32x4*)(p.u + m * p.ldk + n) = f32x4{u[0], u[1], u[2], u[3]};
+              }
             }
             const i32x4 ho = mat_join(hv[0], hv[1]);
             const int64_t n = n0 + t.wn * (TN / 2) + h * 32 + 16 * q + 8 * lh;
             if (m < p.M) store_piece((O*)p.h + m * p.F, n, p.F, ho);
-            if (!INT && p.g) {
-              const i32x4 go = mat_join(gv[0], gv[1]), uo = mat_join(uv[0], uv[1]);
-              if (m < p.M) {
-                store_piece((O*)p.g + m * p.ldk, n, p.ldk, go);
-                store_piece((O*)p.u + m * p.ldk, n, p.ldk, uo);
-              }
-            }
             mat_piece_end();
           }
         }
@@ -205,8 +203,8 @@ __global__ __launch_bounds__(256) void gated_finish_kernel(GatedParams p) {
       if (n0 + i < p.F) h[i] = (O)v[i];
   }
   if (!INT && p.g && n0 < p.ldk) {     // (ldk is a multiple of 8)
-    *(u32x2*)((O*)p.g + m * p.ldk + n0) = pack4<O>(gf);
-    *(u32x2*)((O*)p.u + m * p.ldk + n0) = pack4<O>(uf);
+    *(f32x4*)(p.g + m * p.ldk + n0) = f32x4{gf[0], gf[1], gf[2], gf[3]};
+    *(f32x4*)(p.u + m * p.ldk + n0) = f32x4{uf[0], uf[1], uf[2], uf[3]};
   }
 }
 
@@ -244,8 +242,8 @@ __global__ __launch_bounds__(WAVES * 64) void gated_panel_kernel(GatedParams p) 
         if (n + r < p.F) h[r] = (O)v[r];
     }
     if (!INT && p.g && n < p.ldk) {     // (ldk is a multiple of 8)
-      *(u32x2*)((O*)p.g + m * p.ldk + n) = pack4<O>(g);
-      *(u32x2*)((O*)p.u + m * p.ldk + n) = pack4<O>(u);
+      *(f32x4*)(p.g + m * p.ldk + n) = f32x4{g[0], g[1], g[2], g[3]};
+      *(f32x4*)(p.u + m * p.ldk + n) = f32x4{u[0], u[1], u[2], u[3]};
     }
   });
 }

@@ -8,7 +8,7 @@ extern "C" int fla_gated_linear_splits(int64_t M, int64_t F, int64_t K, int elem
 }
 
 extern "C" int fla_gated_linear_fwd(const void* x, const void* gate_weight, const void* up_weight, const void* gate_bias, const void* up_bias,
-                                    int bias_dtype, void* h, void* gate_out, void* up_out, int64_t ld, int64_t M, int64_t F, int64_t K,
+                                    int bias_dtype, void* h, float* gate_out, float* up_out, int64_t ld, int64_t M, int64_t F, int64_t K,
                                     int activation, int dtype, void* workspace, fla_stream_t stream) {
   FLA_REQUIRE(x && gate_weight && up_weight && h && (!gate_out == !up_out) && M >= 0 && F > 0 && K > 0, FLA_E_INVALID);
   FLA_REQUIRE(activation >= FLA_ACT_NONE && activation <= FLA_ACT_RELU, FLA_E_INVALID);

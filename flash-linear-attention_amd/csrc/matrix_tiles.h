@@ -170,7 +170,7 @@ struct MatTile {
       for (int q = 0; q < kCopies; ++q) copy(c, q);
     }
   }
-  // Slices first .. last - 1, at least one, behind begin().  LATER, three times LATER: with `later` 1 and 2 so many memory operations of this wave were
+  // Slices first .. last - 1, at least one, behind begin().  LATER, five times LATER: with `later` 1 and 2 so many memory operations of this wave were
   // issued behind it (the stores of the tile before, which need not be waited for).
   template <int LATER, typename F>
   FLA_DEVICE void multiply(char* lds, int first, int last, int later, const F& source, acc_t (&acc)[MT][NT]) const {
@@ -204,7 +204,7 @@ struct MatTile {
     };
     constexpr int kNewer = (RING - 1) * kCopies;
     constexpr auto most = [](int n) { return n < 63 ? n : 63; };   // (the counter's largest value)
-    if (later == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(most(kNewer + 3 * LATER)) : "memory");
+    if (later == 2) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(most(kNewer + 5 * LATER)) : "memory");
     else if (later) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(most(kNewer + LATER)) : "memory");
     else asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kNewer) : "memory");
     asm volatile("s_barrier" ::: "memory");
@@ -216,7 +216,7 @@ struct MatTile {
     for (int s = first; s < last; ++s) {
       half(f[0], f[1], lds + piece * kPiece, 1, c, false);
       // this wave's copies of slice s + 1 have arrived and its fragments of s are read; then everybody's
-      if (later == 2 && s == first) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(most((RING - 2) * kCopies + 3 * LATER)) : "memory");
+      if (later == 2 && s == first) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(most((RING - 2) * kCopies + 5 * LATER)) : "memory");
       else if (later && s == first) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(most((RING - 2) * kCopies + LATER)) : "memory");
       else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"((RING - 2) * kCopies) : "memory");
       asm volatile("s_barrier" ::: "memory");
@@ -248,7 +248,7 @@ struct MatGrid {
 };
 // A workgroup's tiles, one behind the other.  The first copies of a tile are on their way while the sums of the one before are brought out: what is waited for
 // between two tiles is a barrier.  Half of the workgroups take their half tile first: then not all of them write at the same time.  JOB:
-//   Whole, Half        MatTile types;  LATER  memory operations of a wave that finish() of a whole tile issues where it returns 1, a third of those where it returns 2
+//   Whole, Half        MatTile types;  LATER  memory operations of a wave that finish() of a whole tile issues where it returns 1, a fifth of those where it returns 2
 //   at(tm, n)          remembers where the tile lies: row of tiles tm, first column n (in units of half tiles)
 //   columns(side)      sends what goes by row and column into LDS, half `side` of it (a load in finish() would wait for the copies ahead of it);   source(s, m, n)   as for MatTile
 //   finish(tile, acc, side)   brings a tile out

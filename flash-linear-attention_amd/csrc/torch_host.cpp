@@ -881,11 +881,11 @@ Tensor whole_bias(const Tensor& b) {
 struct GatedNode : torch::autograd::Function<GatedNode> {
   struct Rest {
     bool x, wg, wu, bg, bu;  // whether they have a gradient
-    at::ScalarType bg_type, bu_type;
+    at::ScalarType type, bg_type, bu_type;
     int64_t F;
     long act;
   };
-  // kept: g and u [2, M, ld] for a backward, and the operands as the kernels took them; or NULL
+  // kept: g and u [2, M, ld] in fp32 for a backward, and the operands as the kernels took them; or NULL
   struct Kept {
     Tensor gu, x, wg, wu;
   };
@@ -894,7 +894,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
     auto shape = x_.sizes().vec();
     shape.back() = F;
     Tensor h = fresh(shape, x_, x_.scalar_type());
-    if (kept) kept->gu = fresh({2, M, ld}, x_, x_.scalar_type());
+    if (kept) kept->gu = fresh({2, M, ld}, x_, at::kFloat);
     if (M == 0) return h;
     const Tensor x = whole_rows(x_, 8), wg = whole_rows(wg_, 8), wu = whole_rows(wu_, 8);
     if (kept) kept->x = x, kept->wg = wg, kept->wu = wu;
@@ -903,9 +903,9 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
     const int64_t K = x.size(-1);
     const int splits = fla_gated_linear_splits(M, F, K, 2);
     const Tensor sums = splits > 1 ? fresh({splits, M, 2, F}, x, at::kFloat) : Tensor();
-    char* keep = kept ? (char*)kept->gu.data_ptr() : nullptr;
+    float* keep = kept ? fptr(kept->gu) : nullptr;
     check(fla_gated_linear_fwd(ptr(x), ptr(wg), ptr(wu), ptr(bg), ptr(bu), same ? dt(x) : FLA_F32, ptr(h), keep,
-                               keep ? keep + M * ld * 2 : nullptr, ld, M, F, K, (int)act, dt(x), ptr(sums), stream_of(x)),
+                               keep ? keep + M * ld : nullptr, ld, M, F, K, (int)act, dt(x), ptr(sums), stream_of(x)),
           "fla_gated_linear_fwd");
     return h;
   }
@@ -914,7 +914,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
     const Tensor bg = given(bg_), bu = given(bu_);
     Kept kept;
     Tensor h = run(x, wg, wu, bg, bu, act, &kept);
-    const Rest r{asks(x), asks(wg), asks(wu), asks(bg), asks(bu), bg.defined() ? bg.scalar_type() : at::kFloat, bu.defined() ? bu.scalar_type() : at::kFloat,
+    const Rest r{asks(x), asks(wg), asks(wu), asks(bg), asks(bu), x.scalar_type(), bg.defined() ? bg.scalar_type() : at::kFloat, bu.defined() ? bu.scalar_type() : at::kFloat,
                  wg.size(0), act};
     // (x for the weights' gradients, the weights for x's)
     // The operands themselves are saved, so that a backward after they were written to is refused, and beside them what they were copied into, if they were.
@@ -933,7 +933,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
     const auto shape = ctx->saved_data["shape"].toIntVector();
     c10::DeviceGuard on_device(kept.device());
     const int64_t M = kept.size(1), ld = kept.size(2), F = r.F, K0 = shape.back(), K = (K0 + 7) / 8 * 8;
-    const auto type = kept.scalar_type();
+    const auto type = r.type;
     Tensor dx, dwg, dwu, dbg, dbu;
     if (M == 0) {
       auto zeros = [&](bool wanted, at::IntArrayRef sizes, at::ScalarType t) { return wanted ? at::zeros(sizes, kept.options().dtype(t)) : Tensor(); };
@@ -941,12 +941,13 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
               Tensor()};
     }
     const Tensor dh = as(grads[0], type).contiguous();
-    const Tensor d = fresh_like(kept);
+    const Tensor d = fresh(kept.sizes(), kept, type);
     const int64_t rows = fla_gated_linear_bwd_rows(M), parts = (M + rows - 1) / rows, half = M * ld * 2;
     const PartialPair part(r.bg, r.bu, r.bg_type, r.bu_type, parts, F, kept);
     const fla_stream_t stream = stream_of(kept);
-    char *g = (char*)kept.data_ptr(), *dg = (char*)d.data_ptr();
-    check(fla_gated_linear_bwd_gate(ptr(dh), g, g + half, dg, dg + half, part.first(), part.second(), part.ld, ld, M, F, (int)r.act, dt(kept), stream),
+    const float* g = fptr(kept);
+    char* dg = (char*)d.data_ptr();
+    check(fla_gated_linear_bwd_gate(ptr(dh), g, g + M * ld, dg, dg + half, part.first(), part.second(), part.ld, ld, M, F, (int)r.act, dt(d), stream),
           "fla_gated_linear_bwd_gate");
     part.sums(&dbg, &dbu);
     if (r.x) {
@@ -954,7 +955,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
       dx = fresh(shape, kept, type);
       const int splits = fla_gated_linear_bwd_dx_splits(M, F, K);
       const Tensor sums = splits > 1 ? fresh({splits, M, K}, kept, at::kFloat) : Tensor();
-      check(fla_gated_linear_bwd_dx(dg, dg + half, ptr(wg), ptr(wu), ptr(dx), ld, K0, M, F, K, dt(kept), fptr(sums), stream), "fla_gated_linear_bwd_dx");
+      check(fla_gated_linear_bwd_dx(dg, dg + half, ptr(wg), ptr(wu), ptr(dx), ld, K0, M, F, K, dt(d), fptr(sums), stream), "fla_gated_linear_bwd_dx");
     }
     if (r.wg || r.wu) {
       const Tensor x = saved[4].defined() ? saved[4] : whole_rows(saved[0], 8);
@@ -962,7 +963,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
       if (r.wu) dwu = fresh({F, K0}, kept, type);
       const int splits = fla_gated_linear_bwd_dw_splits(M, F, K, r.wg && r.wu);
       const Tensor sums = splits > 1 ? fresh({r.wg && r.wu ? 2 : 1, splits, F, K}, kept, at::kFloat) : Tensor();
-      check(fla_gated_linear_bwd_dw(dg, dg + half, ptr(x), ptr(dwg), ptr(dwu), ld, K0, M, F, K, dt(kept), fptr(sums), stream), "fla_gated_linear_bwd_dw");
+      check(fla_gated_linear_bwd_dw(dg, dg + half, ptr(x), ptr(dwg), ptr(dwu), ld, K0, M, F, K, dt(d), fptr(sums), stream), "fla_gated_linear_bwd_dw");
     }
     return {dx, dwg, dwu, dbg, dbu, Tensor()};
   }

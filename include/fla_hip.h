@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define FLA_ABI_VERSION 29
+#define FLA_ABI_VERSION 30
 
 enum fla_dtype { FLA_F32 = 0, FLA_BF16 = 1, FLA_F16 = 2 };
 
@@ -896,12 +896,12 @@ int fla_int8_linear(const void* x, const float* x_scale, const void* weight, con
  *   g = x gate_weight' + gate_bias,  u = x up_weight' + up_bias,  h[m,f] = act(g) u.
  * x [M,K], weights [F,K], h [M,F] in `dtype`, bf16 or fp16; K % 8 == 0, K, F <= 2^22; x and the weights at 16-byte addresses, any F and address of h (multiples of 8
  * and of 16 bytes take the wide stores).  Biases [F] in `dtype` or fp32 (one type for both) at 4-byte addresses, or NULL.  activation: enum fla_activation.
- * gate_out, up_out [M,ld], both or neither: g and u for the backward, ld = F rounded up to a multiple of 8, columns behind F unspecified.  A product of few tiles and
+ * gate_out, up_out fp32 [M,ld], both or neither: g and u for the backward, ld = F rounded up to a multiple of 8, columns behind F unspecified.  A product of few tiles and
  * a long K is summed in slices of K: fla_gated_linear_splits (element_bytes: 2, or 1 for rows in 8 bits) gives their number, and where it is more
  * than one `workspace` holds [splits, M, 2, F] fp32 (int32 for rows of integers) at a 16-byte address.
  *
  * Backward, in three steps:
- *   _bwd_gate: dgate = dh u act'(g), dup = dh act(g), both [M,ld] with zeros behind F, from the kept g and u; *_bias_partial: fp32
+ *   _bwd_gate: dgate = dh u act'(g), dup = dh act(g), both [M,ld] in `dtype` with zeros behind F, from the kept g and u; *_bias_partial: fp32
  *     [ceil(M / fla_gated_linear_bwd_rows(M)), F], rows partial_ld elements apart, or NULL, their column sums are the biases' gradients.
  *   Of operands that were brought to a multiple of 8 columns by zeros, results have the `columns` that are wanted (otherwise K) and any address.
  *   _bwd_dx: dx [M,K] = dgate gate_weight + dup up_weight; workspace: fp32 [splits, M, K] where _dx_splits is more than one.
@@ -909,7 +909,7 @@ int fla_int8_linear(const void* x, const float* x_scale, const void* weight, con
  *     [1 or 2, splits, F, K] where _dw_splits is more than one. */
 int fla_gated_linear_splits(int64_t M, int64_t F, int64_t K, int element_bytes);
 int fla_gated_linear_fwd(const void* x, const void* gate_weight, const void* up_weight, const void* gate_bias, const void* up_bias,
-                         int bias_dtype, void* h, void* gate_out, void* up_out, int64_t ld, int64_t M, int64_t F, int64_t K,
+                         int bias_dtype, void* h, float* gate_out, float* up_out, int64_t ld, int64_t M, int64_t F, int64_t K,
                          int activation, int dtype, void* workspace, fla_stream_t stream);
 /* The same of rows in 8-bit integers, x and both weights with a scale per row (see fla_int8_linear); h in bf16 or fp16. */
 int fla_int8_gated_linear_fwd(const void* x, const float* x_scale, const void* gate_weight, const float* gate_scale,
@@ -917,7 +917,7 @@ int fla_int8_gated_linear_fwd(const void* x, const float* x_scale, const void* g
                               int bias_dtype, void* h, int64_t M, int64_t F, int64_t K, int activation, int dtype, void* workspace,
                               fla_stream_t stream);
 int fla_gated_linear_bwd_rows(int64_t M);
-int fla_gated_linear_bwd_gate(const void* dh, const void* gate, const void* up, void* dgate, void* dup, float* dgate_bias_partial,
+int fla_gated_linear_bwd_gate(const void* dh, const float* gate, const float* up, void* dgate, void* dup, float* dgate_bias_partial,
                               float* dup_bias_partial, int64_t partial_ld, int64_t ld, int64_t M, int64_t F, int activation, int dtype,
                               fla_stream_t stream);
 int fla_gated_linear_bwd_dx_splits(int64_t M, int64_t F, int64_t K);

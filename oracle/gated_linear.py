@@ -5,7 +5,7 @@
 Bounds, in units of 2^-24.  A sum of K products of 16-bit values: the products are exact in fp32, an instruction adds sixteen of them, and for each instruction four
 roundings of the running sum are allowed, which is at most the sum of the magnitudes: ``(K / 4 + 32)`` of that sum.  Activations: slopes of at most 1.13,
 second derivatives of at most 0.8, and errors of the evaluation of 3e-7 |g| (the published erf's 1.5e-7, two of the hardware's exponentials and reciprocals).
-The backward reads g and u rounded to the operands' type, half a step each, and rounds dg and du likewise.  Those roundings are independent and of either sign:
+The backward reads g and u as they were summed and rounds dg and du to the operands' type, half a step each.  Those roundings are independent and of either sign:
 by Hoeffding's inequality a sum of such errors, each at most c, exceeds 7 sqrt(sum c^2) with a probability below 5e-11."""
 import math
 
@@ -54,7 +54,6 @@ def backward(x, wg, wu, state, dh, name, half):
     """Gradients and bounds of their errors ahead of their own rounding; ``half``: half a step of the operands' type, relative."""
     g, eg, u, eu, a, slope = state
     M, F = g.shape
-    eg, eu = eg + half * (g.abs() + eg), eu + half * (u.abs() + eu)
     es = CURVE * eg + 1e-6 * (1 + g.abs())
     if name == "relu":
         es = torch.where(g.abs() <= eg, 1.0, 0.0) + 0 * es
@@ -64,7 +63,8 @@ def backward(x, wg, wu, state, dh, name, half):
     dg, du = dh * u * slope, dh * a
     edg = dh.abs() * (u.abs() * es + slope.abs() * eu + es * eu) + 4 * UNIT * dg.abs()
     edu = dh.abs() * ea + 2 * UNIT * du.abs()
-    rdg, rdu = edg + half * (dg.abs() + edg), edu + half * (du.abs() + edu)       # as they are stored
+    step = 2.0 ** -25 if half == 2.0 ** -11 else 0.0      # half of fp16's smallest step
+    rdg, rdu = edg + half * (dg.abs() + edg) + step, edu + half * (du.abs() + edu) + step       # as they are stored
     out = {"dx": dg @ wg + du @ wu, "dwg": dg.t() @ x, "dwu": du.t() @ x, "dbg": dg.sum(0), "dbu": du.sum(0)}
     root = lambda c, w: 7 * torch.sqrt((c * c) @ (w * w))
     tiny = 1e-30
