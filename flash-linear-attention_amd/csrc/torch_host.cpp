@@ -15,11 +15,13 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <map>
 #include <mutex>
 #include <optional>
+#include <unordered_set>
 #include <vector>
 
 #include "../../include/fla_hip.h"
@@ -70,15 +72,24 @@ bool wants_grad(std::initializer_list<const Tensor*> ts) {
   return false;
 }
 // A leaf's accumulation node stays on the stream that was current when it was made, for as long as a graph holds it.  One of the default stream, which
-// cannot be captured, makes a captured backward pass end the process: the call is refused while it is only a call.
+// cannot be captured, makes a captured backward pass end the process: the call is refused while it is only a call.  Leaves are looked for through the
+// whole graph behind the operands (a cast of autocast, the layers ahead), in a call under capture alone.
 void refuse_eager_leaves(std::initializer_list<const Tensor*> ts, const char* who) {
   if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-  for (const Tensor* t : ts) {
-    if (!t->defined() || !t->is_leaf() || !t->requires_grad()) continue;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-    const auto stream = node ? node->stream() : std::nullopt;
-    TORCH_CHECK(!stream || stream->id() != 0, "fla_amd ", who, ": an eager graph of the default stream still holds these leaves, and a backward pass "
-                "of theirs cannot be captured: drop its results ahead of the capture, or call this under torch.no_grad()");
+  std::vector<std::shared_ptr<torch::autograd::Node>> open;
+  std::unordered_set<const torch::autograd::Node*> seen;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) open.push_back(t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn());
+  while (!open.empty()) {
+    const auto node = std::move(open.back());
+    open.pop_back();
+    if (!node || !seen.insert(node.get()).second) continue;
+    if (dynamic_cast<const torch::autograd::AccumulateGrad*>(node.get())) {
+      const auto stream = node->stream();
+      TORCH_CHECK(!stream || stream->id() != 0, "fla_amd ", who, ": an eager graph of the default stream still holds these leaves, or some behind them, and a "
+                  "backward pass of theirs cannot be captured: drop its results ahead of the capture, or call this under torch.no_grad()");
+    }
+    for (const auto& edge : node->next_edges()) open.push_back(edge.function);
   }
 }
 bool on_gpu(std::initializer_list<const Tensor*> ts) {

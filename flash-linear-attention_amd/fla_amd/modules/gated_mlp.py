@@ -27,7 +27,8 @@ def gated_linear(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Te
     ``activation``: ``"silu"`` (``"swish"``), ``"gelu"`` (of the error function), ``"relu"`` (its slope at 0 is 0) or ``None``; biases in any floating type.
     For a backward both pre-activations are kept in fp32, ``2 F`` values a row; it rounds the gradients of both to x's type, in its range, ahead of the
     products that form those of x and the weights.  Gradients of operands that do not ask for one are not formed.  There are no second derivatives.
-    Under capture a call with gradients is refused while an eager graph of the default stream holds one of its leaves: a backward could not be captured.
+    Under capture a call with gradients is refused while an eager graph of the default stream holds one of its leaves, or one behind them (the parameters that
+    autocast casts, those of the layers ahead): a backward could not be captured.
     Under autocast the operands are cast to its type, as ``torch.nn.functional.linear`` does."""
     code = _activation(activation, "gated_linear")
     if torch.is_autocast_enabled("cuda") and x.is_cuda:

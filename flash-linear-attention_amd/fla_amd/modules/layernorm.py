@@ -26,14 +26,17 @@ def rms_norm(x, weight, bias=None, residual=None, prenorm=False, residual_in_fp3
     ``quantize``: in the place of ``y`` the pair ``(q, scale)``, ``scale`` fp32 ``[...]`` without the last dimension and ``y ~ q * scale[..., None]``.
     ``True`` or ``torch.float8_e4m3fn``: ``q`` in that type, ``scale = max(max|y|, 1e-30) / 448``; ``torch.int8``: ``q`` the nearest whole numbers (halves to
     even), ``scale = max(max|y|, 1e-30) / 127``, infinite or NaN where the row holds such a value.  It has no gradient and is refused where one
-    is wanted.  Rows of at most 16384 elements; weight and bias may be ``None``; the residual is in x's dtype or in fp32."""
+    is wanted.  Rows of at most 16384 elements; weight and bias may be ``None``; the residual is in x's dtype or in fp32.
+    A backward cannot be captured while an eager graph of the default stream holds one of the leaves (torch ends the process); unlike :func:`layer_norm`, this
+    function does not look: its forward alone may be captured then."""
     return host().norm(x, weight, bias, residual, eps, prenorm, residual_in_fp32, _rows8(quantize), _RMS)
 
 
 def layer_norm(x, weight, bias=None, residual=None, prenorm=False, residual_in_fp32=False, eps=1e-6, quantize=False):
     """``y = (s - mean(s)) / sqrt(var(s) + eps) * weight (+ bias)`` over the last dimension, ``s = x + residual``, ``var`` the mean square of
     ``s - mean(s)``; one launch each way.  Arguments, results and limits as those of :func:`rms_norm`.
-    Under capture a call with gradients is refused while an eager graph of the default stream holds one of its leaves: a backward could not be captured."""
+    Under capture a call with gradients is refused while an eager graph of the default stream holds one of its leaves, or one behind them: a backward could
+    not be captured."""
     return host().norm(x, weight, bias, residual, eps, prenorm, residual_in_fp32, _rows8(quantize), _LAYER)
 
 
