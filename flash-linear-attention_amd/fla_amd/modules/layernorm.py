@@ -7,7 +7,7 @@ import torch.nn as nn
 
 from .._native import host
 
-_ROWS8 = {False: 0, True: 1, torch.float8_e4m3fn: 1, torch.int8: 2}     # FLA_ROWS_*
+_ROWS8 = {None: 0, False: 0, True: 1, torch.float8_e4m3fn: 1, torch.int8: 2}     # FLA_ROWS_*
 _ROWS_ONLY, _RMS, _LAYER = 0, 1, 2
 
 
