@@ -4,7 +4,7 @@
 
 Bounds, in units of 2^-24.  A sum of K products of 16-bit values: the products are exact in fp32, an instruction adds sixteen of them, and for each instruction four
 roundings of the running sum are allowed, which is at most the sum of the magnitudes: ``(K / 4 + 32)`` of that sum.  Activations: slopes of at most 1.13,
-second derivatives of at most 0.8, and errors of the evaluation of 3e-7 |g| (the published erf's 1.5e-7, two of the hardware's exponentials and reciprocals).
+second derivatives of at most 0.8, and errors of the evaluation of 3e-7 |g| (the normal distribution within 1.5e-7, two of the hardware's exponentials and reciprocals).
 The backward reads g and u as they were summed and rounds dg and du to the operands' type, half a step each.  Those roundings are independent and of either sign:
 by Hoeffding's inequality a sum of such errors, each at most c, exceeds 7 sqrt(sum c^2) with a probability below 5e-11."""
 import math
