@@ -204,9 +204,6 @@ __global__ __launch_bounds__(256) void grad_finish_kernel(const float* part, T* 
   }
 }
 
-TilePlan plan_dx(int64_t M, int64_t F, int64_t K) { return plan_tiles(M, K, 2 * fla_cdiv(F * 2, kSliceBytes), 1, false); }
-TilePlan plan_dw(int64_t M, int64_t F, int64_t K, int batch) { return plan_tiles(F, K, fla_cdiv(M, 64), batch, false); }
-
 template <typename T>
 int launch_dx(const GradParams& p, TileKind kind, hipStream_t st) {
   MatGrid g{};

@@ -268,8 +268,6 @@ int launch_forward(const GatedParams& p, TileKind kind, hipStream_t st) {
   }
   return FLA_OK;
 }
-// Up to this many rows of x go to the panels
-constexpr int64_t kPanelRows = 64;
 template <typename T, typename O>
 int launch_panel(const GatedParams& p, hipStream_t st) {
   const int64_t grid = fla_cdiv(p.F, 16);
@@ -280,7 +278,6 @@ int launch_panel(const GatedParams& p, hipStream_t st) {
   FLA_CHECK_LAUNCH();
   return FLA_OK;
 }
-TilePlan plan_gated(int64_t M, int64_t F, int64_t row_bytes) { return plan_tiles(M, 2 * F, fla_cdiv(row_bytes, kSliceBytes), 1, true); }
 template <typename T, typename O>
 int gated_forward(GatedParams& p, hipStream_t st) {
   if (p.M <= kPanelRows) return launch_panel<T, O>(p, st);

@@ -236,10 +236,6 @@ __global__ __launch_bounds__(256) void int8_finish_kernel(Int8Params p) {
   int8_store4<O>(p, m, n, v);
 }
 
-constexpr int64_t kPanelRows = 64;   // of x; more go to the tiles
-// (fp32 results leave in 128 x 128 tiles: the big one is built for 16 bits)
-TilePlan plan_int8(int64_t M, int64_t N, int64_t K, bool big) { return plan_tiles(M, N, fla_cdiv(K, kSliceBytes), 1, true, big ? kBig : kMiddle); }
-
 template <typename O>
 int launch_int8(Int8Params& p, hipStream_t st) {
   if (p.M <= kPanelRows) {

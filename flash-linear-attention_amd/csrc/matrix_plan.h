@@ -47,6 +47,14 @@ TilePlan plan_tiles(int64_t M, int64_t N, int64_t slices, int batch, bool contig
   return best;
 }
 
+// ... of the products there are.  Up to kPanelRows rows of x those of contiguous operands go to the panels instead.
+constexpr int64_t kPanelRows = 64;
+TilePlan plan_gated(int64_t M, int64_t F, int64_t row_bytes) { return plan_tiles(M, 2 * F, fla_cdiv(row_bytes, kSliceBytes), 1, true); }
+TilePlan plan_dx(int64_t M, int64_t F, int64_t K) { return plan_tiles(M, K, 2 * fla_cdiv(F * 2, kSliceBytes), 1, false); }
+TilePlan plan_dw(int64_t M, int64_t F, int64_t K, int batch) { return plan_tiles(F, K, fla_cdiv(M, 64), batch, false); }
+// (fp32 results leave in 128 x 128 tiles: the big one is built for 16 bits)
+TilePlan plan_int8(int64_t M, int64_t N, int64_t K, bool big) { return plan_tiles(M, N, fla_cdiv(K, kSliceBytes), 1, true, big ? kBig : kMiddle); }
+
 // The launch of tm rows of tn tiles
 int grid_of(TileKind kind, int64_t tm, int64_t tn, int splits, MatGrid* g, dim3* grid) {
   const int64_t tiles = tm * tn;

@@ -16,7 +16,7 @@ _lib = None
 
 FLA_F32, FLA_BF16, FLA_F16 = 0, 1, 2
 FLA_H_ROW_MAJOR, FLA_H_FRAGMENT, FLA_H_FRAGMENT_T = 0, 1, 2
-ABI_VERSION = 30
+ABI_VERSION = 31
 
 _DTYPES = {torch.float32: FLA_F32, torch.bfloat16: FLA_BF16, torch.float16: FLA_F16}
 
@@ -132,6 +132,7 @@ SIGNATURES = {
     "fla_gated_linear_bwd_dw": (c_int, [P] * 5 + [I64, I64, I64, I64, I64, I, P, P]),
     "fla_selftest_mfma": (c_int, [P, P, P, I64, I64, I64, I, P]),
     "fla_selftest_stream_tiles": (c_int, [P, I64, I, P, I64, I64, I64, I, P]),
+    "fla_selftest_matrix_plan": (c_int, [I, I64, I64, I64, P]),
 }
 
 

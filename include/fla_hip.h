@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define FLA_ABI_VERSION 30
+#define FLA_ABI_VERSION 31
 
 enum fla_dtype { FLA_F32 = 0, FLA_BF16 = 1, FLA_F16 = 2 };
 
@@ -941,6 +941,19 @@ int fla_selftest_mfma(const void* A, const void* B, float* C, int64_t M, int64_t
  * all 32-bit words each workgroup read.  T a multiple of 64. */
 int fla_selftest_stream_tiles(const void* x, int64_t tensor_bytes, int n_tensors, uint32_t* sink, int64_t B,
                               int64_t T, int64_t H, int share, fla_stream_t stream);
+
+/* Diagnostics: the launch that a product of the gated block or of rows in integers takes, without making it (host only).  M rows of x, N rows of a weight (F), K
+ * columns of both.  plan[5]: rows of a tile (0: the panels of few rows), slices of the contraction, workgroups a slice, whole tiles, half tiles. */
+enum fla_product {
+  FLA_PRODUCT_GATED = 0,      /* fla_gated_linear_fwd */
+  FLA_PRODUCT_GATED_INT8 = 1, /* fla_int8_gated_linear_fwd */
+  FLA_PRODUCT_GATED_DX = 2,   /* fla_gated_linear_bwd_dx */
+  FLA_PRODUCT_GATED_DW = 3,   /* fla_gated_linear_bwd_dw, both weights; _DW1: one of them */
+  FLA_PRODUCT_GATED_DW1 = 4,
+  FLA_PRODUCT_INT8 = 5,       /* fla_int8_linear, results in 16 bits; _F32: in fp32 */
+  FLA_PRODUCT_INT8_F32 = 6
+};
+int fla_selftest_matrix_plan(int product, int64_t M, int64_t N, int64_t K, int* plan);
 
 #ifdef __cplusplus
 }

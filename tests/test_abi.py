@@ -35,7 +35,7 @@ def test_library_exports_every_declared_symbol():
 INTERFACES = {15: "b7a4f7cfed6a371e", 16: "ecb9b6be8de7c997", 17: "8d259aba7a1ce02b", 18: "d280e32277841484",
               19: "ffed6d79950c4a2c", 20: "7277003d13de7e6d", 21: "88fd3932e6552668", 22: "491ca6ca57f1a4d8", 23: "6120caa44fecd8de",
               24: "ebb39d695c9338ce", 25: "d92b5fd525fdd6be", 26: "d6269a688c65b21f", 27: "feda75803ad19577",
-              28: "fada585f709e5f17", 29: "4388684e9be98185", 30: "dfb88e22877aba3f"}
+              28: "fada585f709e5f17", 29: "4388684e9be98185", 30: "dfb88e22877aba3f", 31: "dc79ec538fc7afb4"}
 
 
 def _interface():
