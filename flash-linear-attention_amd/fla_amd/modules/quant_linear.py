@@ -92,6 +92,15 @@ class QuantLinear(nn.Module):
             self.weight_scale = rows[1].to(self.weight_scale.device)
         return self
 
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        # rows of another type would be converted number by number, and their scales are for the type that they were made in
+        rows = state_dict.get(prefix + "weight")
+        if rows is not None and rows.dtype != self.weight.dtype and not local_metadata.get("assign_to_params_buffers", False):
+            error_msgs.append(f"fla_amd QuantLinear: {prefix}weight holds {rows.dtype}, the layer {self.weight.dtype}: make it with dtype={rows.dtype}, "
+                              "or load with assign=True")
+            return
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+
     def extra_repr(self) -> str:
         return f"{self.in_features}, {self.out_features}, bias={self.bias is not None}, activation={self.activation}"
 
