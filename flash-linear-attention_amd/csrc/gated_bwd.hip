@@ -18,7 +18,7 @@ struct GatedBwdParams {
   int act;
 };
 
-// HBM-bound: 8192 x 5632 in 86 - 90 us, 5.1 - 5.4 TB/s of dh, g, u, dg and du, the rate of a large copy.  dg and du leave in the operands' type, since the matrix instructions take
+// HBM-bound: 8192 x 5632 in 152 - 156 us, 4.1 - 4.2 TB/s of dh, g, u, dg and du (646 MB, of them 369 for g and u in fp32; a large copy reaches 5.1; four columns a thread, whole kilobytes a wave, was no faster).  dg and du leave in the operands' type, since the matrix instructions take
 // nothing wider: half a step each.  The biases' gradients are sums of what was not rounded.
 // 512 columns, eight a thread, of `rows` rows, four at a time
 template <typename T>
@@ -105,7 +105,7 @@ FLA_DEVICE int grad_store(const Tile& t, const typename Tile::acc_t (&acc)[Tile:
   return !part && m0 + Tile::MT * 64 <= rows && n0 + Tile::NT * 64 <= columns;
 }
 
-// 8192 x 2048 from 2 x 5632: 312 - 326 us, 1.2 PFLOP/s, one tile for each CU: 2 x 88 slices at 1.8 us, first copies and stores included.
+// 8192 x 2048 from 2 x 5632: 304 - 326 us, 1.2 PFLOP/s, one tile for each CU: 2 x 88 slices at 1.8 us, first copies and stores included.
 // dx = dg Wg + du Wu: the slices of the first product, then those of the second
 template <typename T, int BM, int BN, bool HALVES>
 struct DxJob {
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PER_SIMD, P
   mat_run(lds, grid, job);
 }
 
-// 2 x 5632 x 2048 from 8192 rows: 334 - 349 us; 352 tiles for 256 CUs, of which 96 go as half tiles (as 352 workgroups of a tile each: 371 - 379).
+// 2 x 5632 x 2048 from 8192 rows: 325 - 349 us; 352 tiles for 256 CUs, of which 96 go as half tiles (as 352 workgroups of a tile each: 371 - 379).
 // dWg = dg' x and dWu = du' x, the rows of tiles of the one and then those of the other (or one of them alone)
 template <typename T, int BM, int BN, bool HALVES>
 struct DwJob {

@@ -2,9 +2,10 @@
 // One launch on the tiles of matrix_tiles.h.  The rows of the two weights alternate in a tile, 32 of each, so that the lane that holds sums of
 // the gate holds those of the same m and n of the other projection, and neither goes through memory.  For the backward g and u are kept in fp32, as they
 // are summed: the slope of a gate that fp16 does not hold is right, and dg and du carry their own rounding to 16 bits alone.
-// Measured: 8191 x 2048 to 5632 with gelu and biases 358 - 371 us (1.02 - 1.06 PFLOP/s; torch's product alone of that size 395), with silu and g, u kept 385 - 398, in integers 204 - 224
-// (1.7 - 1.85 POP/s).  Its 1408 tiles are five and a half rounds of some 65 us, of which 32 slices at 1.6 are 51.  What
-// bounds it: the rate of slices (matrix_tiles.h), then the ends of tiles: activations, and stores of 16 bytes a lane.
+// Measured: 8191 x 2048 to 5632 with gelu and biases 356 - 374 us (1.01 - 1.06 PFLOP/s; torch's product alone of that size 395 - 401), with silu and g, u kept 411 - 416 (of which
+// the 369 MB of g and u against as much in 16 bits 20 - 30), in integers 202 - 224 (1.7 - 1.87 POP/s).  Its 1408 tiles are five and a half rounds of some 65 us, of which 32 slices at 1.6
+// are 51.  What bounds it: matrix instructions are busy in 0.49 of its cycles (0.76 at 8192^3): slices wait for memory, and the ends of tiles
+// (activations, stores of 16 bytes a lane that take a row in pieces of 32) have none.
 // Of rows in 8-bit integers the sums are exact, and scaled where the biases are added.
 #pragma once
 #include "linear_epilogue.h"

@@ -22,6 +22,7 @@ constexpr bool rest_in_halves(int64_t tiles) { return tiles % kCUs != 0 && tiles
 //   both contiguous      1.05 (few CUs) to 1.6     1.25  1.7                0.9   1.5   1.95
 //   one or both strided  1.05 to 1.6               0.72  0.97               0.58  0.65  0.9
 // Rows of 128 bytes out of two weights come slower than the strided operand's 256 and 512 bytes on end: where both are contiguous the tile with the fewest bytes wins early.
+// Rows in 8-bit integers are decided by the same rates, which were not measured for them: a slice has the same bytes, and bytes are what bounds the smaller tiles.
 // Ends: 12, 8 and 7 us for the first tile of a CU, half of that for each further one; sums of slices go out and in at 5 TB/s behind 5 us.
 // Measured with all three tiles and 1 to 8 slices (us; M x K to F): forward 70 x 2048 to 5632: 28 - 47, taken 30; 200 x 4096 to 11008: 70 - 168, taken 70; 500 x 4096 to 4096: 65 - 140, taken 65;
 // 1003 x 1000 to 2731: 35 - 95, taken 35.  dx of the last: 29 - 120, taken 29; of 2048 x 2048 to 5632: 100 - 208, taken 100; its weights' gradients 92 - 146, taken 92.

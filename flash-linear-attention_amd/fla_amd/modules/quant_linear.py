@@ -52,7 +52,7 @@ def quant_gated_linear(x: Rows, gate_weight: Rows, up_weight: Rows, gate_bias: O
 class QuantLinear(nn.Module):
     """A ``torch.nn.Linear`` for serving with its weight in 8 bits: ``forward(x, residual=None)`` takes 16-bit or fp32 rows, which it quantises first,
     or the pair that a norm with ``quantize`` returned.  ``dtype``: ``torch.float8_e4m3fn`` or ``torch.int8``, of the weight and of the rows.
-    ``in_features`` in multiples of 16, at most 2^23, of integers at most 131056."""
+    ``in_features`` in multiples of 16, at most 2^23, of integers at most 131056.  ``load_state_dict`` refuses rows of another type than the layer's."""
 
     def __init__(self, in_features: int, out_features: int, bias: bool = True, activation: Optional[str] = None,
                  output_dtype: torch.dtype = torch.bfloat16, device=None, dtype: torch.dtype = torch.float8_e4m3fn):
